@@ -352,7 +352,7 @@ def _mul24(total, f):
 
 
 def _plain_sample(s):
-    """A token's weight is the whole part of 2^40 exp((logit - largest) / temperature), so that every
+    """A token's weight is the whole part of 2^36 exp((logit - largest) / temperature), so that every
     sum below is a sum of whole numbers and does not depend on its order.  Tokens are ranked by logit
     (ties: the lower index first).  Kept are the top_k first ones (0: all); of these the shortest run
     of first ones whose weight reaches the part top_p of theirs; of these the ones with
@@ -364,7 +364,7 @@ def _plain_sample(s):
     top = x.amax(-1, keepdim=True)
     temp = s["temperature"][:, None]
     e = torch.where(x == top, 1.0, torch.exp((x - top) * (1.0 / temp)))
-    w = (e * float(1 << 40)).long()
+    w = (e * float(1 << 36)).long()
     rank = torch.sort(x, dim=-1, descending=True, stable=True).indices
     ws = w.gather(1, rank)
     place = torch.arange(vocab, device="cuda")[None]
