@@ -459,6 +459,110 @@ M1MOE_API m1moe_status m1moe_cuda_prefill_step(m1moe_dense_ctx *ctx, m1moe_cuda_
                                      const int32_t *d_tokens, int32_t tokens,
                                      int32_t *d_next_token, float *d_logits, void *stream);
 
+/* ================== a paged key/value cache for ragged batches ==================
+ * The reference keeps one contiguous cache and one position (seqPos,
+ * InferenceEngine.swift:23-24; MetalContext.swift:134-152) and samples on the
+ * CPU (:550-575).  These entry points serve many sequences of different
+ * lengths together.  They are stateless: the caller owns the pools, the page
+ * table and the plan buffer.
+ *
+ * One layer's cache is two bf16 pools [num_pages][num_kv_heads][page_size]
+ * [head_dim].  Position p of sequence b lies in page
+ * page_table[b][p / page_size] (int32 [num_seqs][max_pages_per_seq]; entries
+ * past a sequence's length, or wholly before its window, are never read).
+ * A batch is num_seqs sequences: sequence b's new tokens are rows
+ * cu_q[b] .. cu_q[b+1]-1 of the packed inputs (int32 [num_seqs + 1], from 0
+ * to total_q; a sequence may have none), the last ones of its kv_len[b]
+ * positions.  A sequence shorter than its new tokens (kv_len 0 for an idle
+ * slot of a fixed-size batch) has rows before position 0: they are stored
+ * nowhere and their attention is zero. */
+typedef struct m1moe_paged_cfg {
+    int32_t num_heads;
+    int32_t num_kv_heads;      /* num_heads / num_kv_heads at most 16            */
+    int32_t head_dim;          /* 64 or 128                                      */
+    int32_t page_size;         /* a power of two, 16 to 1024                     */
+    int32_t num_pages;         /* pages of a pool                                */
+    int32_t num_seqs;
+    int32_t max_pages_per_seq; /* columns of the page table                      */
+    int32_t total_q;           /* new tokens of the batch                        */
+    int32_t max_q;             /* at least the most new tokens of one sequence   */
+    int32_t window;            /* positions a token sees, itself included; 0: all */
+    int32_t shared_prefix;     /* positions (whole pages) that all sequences may
+                                  share; a hint that changes no result           */
+} m1moe_paged_cfg;
+
+/* Bytes of the plan buffer of such a batch on the current device (0, with a
+ * message, if the shape is refused). */
+M1MOE_API size_t m1moe_cuda_paged_plan_bytes(const m1moe_paged_cfg *cfg);
+
+/* Make a batch's plan from its device-side lengths (stream-ordered, no
+ * synchronisation, capturable): the lengths checked and copied, each token's
+ * place, the attention's work split over the SMs, and room for its partial
+ * results.  Every layer's append and attention of the step read it; after a
+ * change of cu_q, kv_len or the page table make it again.  d_plan is
+ * 256-byte aligned.  Lengths that contradict cfg raise status bit 1 and the
+ * batch is treated as empty. */
+M1MOE_API m1moe_status m1moe_cuda_paged_plan(const m1moe_paged_cfg *cfg, const int32_t *d_cu_q,
+                                   const int32_t *d_kv_len, const int32_t *d_page_table, void *d_plan,
+                                   size_t plan_bytes, void *stream);
+
+/* Append the batch's new tokens to one layer's pools.  d_qkv [total_q] rows
+ * of q|k|v projections (f32 or bf16, qkv_stride elements apart, the layout of
+ * m1moe_cuda_dense_attention): each query and key head is normalised
+ * (x * rsqrt(mean(x^2) + eps) * w; bf16 w [head_dim], NULL: not at all) and
+ * the first rot_dim elements rotated by d_rope [rope_rows][rot_dim / 2][2]
+ * (f32 cosines and sines of each position; scaled tables for long contexts
+ * are the caller's): element i with element i + rot_dim / 2, or with
+ * rope_pairs 2i with 2i + 1.  k and v rows are stored at their positions,
+ * d_q_out is bf16 [total_q][num_heads][head_dim].  One rounding to bf16.  A
+ * position past rope_rows raises status bit 4 (its rotation is position 0's),
+ * a page id outside the pool bit 2 (not stored).  Replaces the CPU QK-norm,
+ * RoPE and KV store of InferenceEngine.swift:194-220, 521-548. */
+M1MOE_API m1moe_status m1moe_cuda_paged_append(const m1moe_paged_cfg *cfg, const void *d_plan,
+                                     const int32_t *d_page_table, const void *d_qkv, int32_t qkv_dtype,
+                                     int64_t qkv_stride, const uint16_t *d_q_norm, const uint16_t *d_k_norm,
+                                     float eps, const float *d_rope, int32_t rope_rows, int32_t rot_dim,
+                                     int32_t rope_pairs, uint16_t *d_k_pages, uint16_t *d_v_pages,
+                                     uint16_t *d_q_out, void *stream);
+
+/* Causal attention of the batch's new tokens over their sequences:
+ *   out = softmax(c(scale * q . k)) . v over positions max(0, p - window + 1) .. p,
+ * c(s) = softcap * tanh(s / softcap), or s if softcap is 0.  d_q bf16, rows
+ * q_stride elements apart, heads contiguous; d_out likewise (f32 or bf16).
+ * fp32 scores, maxima, sums and accumulators; the weights enter the second
+ * product as bf16.  The split over SMs depends on the lengths alone and
+ * partials are merged in position order: the result is the same every time.
+ * It uses the plan's partials, so calls on one plan must be ordered on one
+ * stream.  Replaces encodeAttention (InferenceEngine.swift:349-399). */
+M1MOE_API m1moe_status m1moe_cuda_paged_attention(const m1moe_paged_cfg *cfg, void *d_plan,
+                                        const int32_t *d_page_table, const uint16_t *d_q, int64_t q_stride,
+                                        const uint16_t *d_k_pages, const uint16_t *d_v_pages, float scale,
+                                        float softcap, void *d_out, int32_t out_dtype, int64_t out_stride,
+                                        void *stream);
+
+/* Wait for the stream and report (then clear) the plan's status word:
+ * M1MOE_ERR_DEVICE if a kernel of the batch raised a bit. */
+M1MOE_API m1moe_status m1moe_cuda_paged_status(void *d_plan, void *stream);
+
+/* One token per row of logits [rows][vocab] (f32 or bf16, row_stride
+ * elements apart; vocab at most 2^20) from one uniform number in [0, 1) per
+ * row.  Settings per row (device arrays [rows]) or, where the array is NULL,
+ * the scalar for all.  A token's weight is floor(2^36 exp((l - max) /
+ * temperature)), ranks go by logit, equal ones by index.  Kept are the top_k
+ * first (<= 0: all); of these the shortest run of first ones whose weight
+ * reaches the part top_p of theirs (>= 1: all); of these the ones with
+ * exp(...) >= min_p.  The token is the first by index whose running kept
+ * weight exceeds the part u of the kept weight (u and top_p in units of
+ * 2^-24).  All sums are of whole numbers: the token depends on nothing but
+ * its row and settings.  Temperature 0 (or below) takes the first rank; -inf
+ * and NaN logits are never chosen; a row without any other gives -1.
+ * Replaces the sampling of InferenceEngine.swift:550-575. */
+M1MOE_API m1moe_status m1moe_cuda_sample(const void *d_logits, int32_t dtype, int64_t row_stride, int32_t rows,
+                               int32_t vocab, const float *d_u, const float *d_temperature,
+                               float temperature, const int32_t *d_top_k, int32_t top_k,
+                               const float *d_top_p, float top_p, const float *d_min_p, float min_p,
+                               int32_t *d_tokens, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

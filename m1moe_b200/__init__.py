@@ -9,7 +9,8 @@ from . import _lib
 from .spec import MIXTRAL_8X7B, OLMOE_1B_7B, ModelSpec, expert_bytes, expert_offsets
 
 __all__ = ["ModelSpec", "OLMOE_1B_7B", "MIXTRAL_8X7B", "expert_bytes", "expert_offsets",
-           "MoEBlock", "matvec4", "matvec4_strided", "unpack4", "M1MoECudaError", "library"]
+           "MoEBlock", "matvec4", "matvec4_strided", "unpack4", "PagedKVCache", "PagedBatch",
+           "paged_append", "paged_attention", "rope_table", "sample", "M1MoECudaError", "library"]
 
 M1MoECudaError = _lib.M1MoECudaError
 
@@ -27,4 +28,10 @@ def __getattr__(name):
     if name in ("matvec4", "matvec4_strided", "unpack4"):
         from . import expert_ffn
         return getattr(expert_ffn, name)
+    if name in ("PagedKVCache", "PagedBatch", "paged_append", "paged_attention", "rope_table"):
+        from . import paged
+        return getattr(paged, name)
+    if name == "sample":
+        from .sampling import sample
+        return sample
     raise AttributeError(name)

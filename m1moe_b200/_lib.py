@@ -42,6 +42,12 @@ class DenseCfg(ctypes.Structure):
                 ("max_seq", ctypes.c_int32), ("device", ctypes.c_int32)]
 
 
+class PagedCfg(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_int32) for n in (
+        "num_heads", "num_kv_heads", "head_dim", "page_size", "num_pages", "num_seqs",
+        "max_pages_per_seq", "total_q", "max_q", "window", "shared_prefix")]
+
+
 # m1moe_dense_tensor
 W_EMBED, W_FINAL_NORM, W_LM_HEAD, W_INPUT_NORM, W_POST_NORM = 0, 1, 2, 3, 4
 W_Q, W_K, W_V, W_O, W_Q_NORM, W_K_NORM = 5, 6, 7, 8, 9, 10
@@ -51,6 +57,8 @@ _lib = None
 # (name, restype, argtypes) for every entry point in include/m1moe_cuda.h.
 _vp = ctypes.c_void_p
 _i32 = ctypes.c_int32
+_i64 = ctypes.c_int64
+_f32 = ctypes.c_float
 _SIGS = [
     ("m1moe_cuda_abi_version", ctypes.c_int32, []),
     ("m1moe_cuda_last_error", ctypes.c_char_p, []),
@@ -101,6 +109,15 @@ _SIGS = [
     ("m1moe_cuda_dense_lm_head", ctypes.c_int, [_vp, _vp, _i32, _vp, _vp, _vp]),
     ("m1moe_cuda_decode_step", ctypes.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _vp]),
     ("m1moe_cuda_prefill_step", ctypes.c_int, [_vp, _vp, _vp, _i32, _vp, _vp, _vp]),
+    ("m1moe_cuda_paged_plan_bytes", ctypes.c_size_t, [_vp]),
+    ("m1moe_cuda_paged_plan", ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, ctypes.c_size_t, _vp]),
+    ("m1moe_cuda_paged_append", ctypes.c_int,
+     [_vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _f32, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
+    ("m1moe_cuda_paged_attention", ctypes.c_int,
+     [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _f32, _f32, _vp, _i32, _i64, _vp]),
+    ("m1moe_cuda_paged_status", ctypes.c_int, [_vp, _vp]),
+    ("m1moe_cuda_sample", ctypes.c_int,
+     [_vp, _i32, _i64, _i32, _i32, _vp, _vp, _f32, _vp, _i32, _vp, _f32, _vp, _f32, _vp, _vp]),
 ]
 
 

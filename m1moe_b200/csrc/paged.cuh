@@ -1,0 +1,386 @@
+// paged.cuh — a paged bf16 key/value cache for a ragged batch: the batch's
+// plan and the append of new tokens (sm_100a).
+//
+// Cache of one layer: K and V, each bf16 [num_pages][nkv][page_size][hd], so
+// that the rows of one (page, KV head) are one contiguous run.  Position p of
+// sequence b lies in page table[b][p / page_size], row p % page_size.  The
+// pool's rows are numbered ((page * nkv) + g) * page_size + row; a row number
+// fits 31 bits (checked by the host), a byte offset does not and is formed
+// in 64.
+//
+// Plan (k_paged_plan, k_paged_tokens).  One device buffer per batch, made
+// from cu_q and kv_len and used by every layer of a step: a checked copy of
+// the lengths, each token's (sequence, position), and the attention's work
+// split.  The work is a list of items -- a sequence's rows (token, head of
+// the KV head's group), `rows` at a time -- per KV head; an item's cost is
+// the number of position units its rows can see; the units of all KV heads'
+// items, concatenated, are cut into equal runs, one per CTA (and, for the
+// 16-row kernel, per warp), whatever the lengths are.  A run that starts or
+// ends inside an item leaves a partial (maximum, sum, weighted values); the
+// last CTA to finish an item merges its partials in position order, so the
+// result does not depend on which one that is.
+#pragma once
+
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+#include "common.cuh"
+#include "pipeline.cuh"
+
+namespace m1 {
+
+// Status bits of a plan (m1moe_cuda_paged_status).
+constexpr int kPagedErrLengths = 1;   // cu_q or kv_len out of range or inconsistent
+constexpr int kPagedErrPage = 2;      // a page id outside the pool
+constexpr int kPagedErrPosition = 4;  // a position outside the rotation table
+constexpr int kPagedErrWait = 8;      // a bounded wait gave up
+
+constexpr int kPagedWarps = 8;      // consumer warps of the 16-row kernel
+constexpr int kPagedRowsSmall = 16; // rows of an item there: one m16n8k16 tile
+constexpr int kPagedUnitSmall = 16; // positions of a unit there
+
+// Words of the plan's header.
+enum PagedHeader {
+    kPhStatus = 0,
+    kPhItems = 1,   // items per KV head
+    kPhUnits = 2,   // units per KV head
+    kPhPer = 3,     // units per CTA
+    kPhPrefix = 4,  // positions of the shared prefix in use (0: none)
+    kPhPrefixUnits = 5,
+    kPhPrefixPer = 6,
+    kPhWords = 16
+};
+
+// One item: rows row0 .. row0 + nrows - 1 of sequence `seq` (row = token
+// offset * group + head offset), position units [unit0, unit0 + units).
+struct PagedItem {
+    int seq, row0, nrows, unit0;
+};
+
+struct PagedPlanView {
+    int *header;
+    int *cu_q;           // [B + 1]
+    int *kv_len;         // [B]
+    int2 *tokens;        // [total_q]: (sequence, position)
+    PagedItem *items;    // [max_items]
+    int *item_at;        // [B + 1]: first item of each sequence
+    int *unit_at;        // [max_items + 1]: units before each item
+    int *start;          // [workers]: the item each worker starts in
+    int *count;          // [nkv * max_items]: partials that have arrived
+    float *part;         // [2 * ctas][rows][hd] weighted values
+    float2 *part_ml;     // [2 * ctas][rows] maximum and sum
+};
+
+struct PagedShape {
+    int nh, nkv, group, hd;
+    int page_size, page_shift, num_pages;
+    int num_seqs, max_pages, total_q, max_q;
+    int window, prefix;
+    int rows, unit;      // the attention kernel's item rows and unit positions
+    int ctas, workers;   // CTAs of the attention grid, and plan start entries
+    int min_per;         // fewest units per CTA
+    int max_items;
+};
+
+// Pool row of position p of sequence b and KV head g, or -1 (with the status
+// bit) if the page table names no page of the pool.
+__device__ __forceinline__ int paged_row(const PagedShape &s, const int *table, int b, int g, int p, int *status) {
+    const int page = __ldg(table + (size_t)b * s.max_pages + (p >> s.page_shift));
+    if ((unsigned)page >= (unsigned)s.num_pages) {
+        atomicOr(status, kPagedErrPage);
+        return -1;
+    }
+    return (page * s.nkv + g) * s.page_size + (p & (s.page_size - 1));
+}
+
+// Exclusive block scan of one int per thread (1024 threads); returns the
+// exclusive prefix and the total.
+__device__ __forceinline__ int block_scan_1024(int v, int *sm, int &total) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();  // sm is free
+    if (lane == 31) sm[warp] = x;
+    __syncthreads();
+    if (warp == 0) {
+        int y = sm[lane];
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int z = __shfl_up_sync(0xffffffffu, y, o);
+            if (lane >= o) y += z;
+        }
+        sm[lane] = y;
+    }
+    __syncthreads();
+    total = sm[31];
+    return x - v + (warp ? sm[warp - 1] : 0);
+}
+
+// Largest i in [0, n) with a[i] <= v (a ascending, a[0] <= v).
+__device__ __forceinline__ int upper_index(const int *a, int n, int v) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (a[mid] <= v)
+            lo = mid;
+        else
+            hi = mid;
+    }
+    return lo;
+}
+
+// One CTA: the checked lengths, the items and the work split of one batch.
+// Lengths that cannot be right raise the status bit and make the batch an
+// empty one, so that no later kernel leaves the buffers.  A sequence may be
+// shorter than its new tokens (an idle slot of a fixed-size batch has none
+// at all): the tokens before position 0 see nothing and are stored nowhere.
+__global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const PagedPlanView p, const int *cu_q,
+                                                     const int *kv_len, const int *table) {
+    __shared__ int sm[32];
+    __shared__ int sm_bad, sm_noprefix;
+    const int tid = threadIdx.x;
+    if (tid == 0) sm_bad = 0, sm_noprefix = 0;
+    __syncthreads();
+    pdl_wait();
+    const int capacity = s.max_pages * s.page_size;
+    int items = 0;
+    for (int b0 = 0; b0 < s.num_seqs; b0 += 1024) {
+        const int b = b0 + tid;
+        int n = 0;
+        if (b < s.num_seqs) {
+            const int q0 = cu_q[b], q1 = cu_q[b + 1], t = kv_len[b];
+            const bool good = q0 >= 0 && q1 >= q0 && q1 <= s.total_q && q1 - q0 <= s.max_q && t >= 0 &&
+                              t <= capacity && (b > 0 || q0 == 0) && (b + 1 < s.num_seqs || q1 == s.total_q);
+            if (!good) sm_bad = kPagedErrLengths;
+            p.cu_q[b] = q0;
+            p.kv_len[b] = t;
+            if (b + 1 == s.num_seqs) p.cu_q[b + 1] = q1;
+            n = good ? ((q1 - q0) * s.group + s.rows - 1) / s.rows : 0;
+            if (q1 > q0 && t - (q1 - q0) < s.prefix) sm_noprefix = 1;
+        }
+        int total;
+        const int at = block_scan_1024(n, sm, total);
+        if (b < s.num_seqs) p.item_at[b] = items + at;
+        items += total;
+    }
+    if (tid == 0) p.item_at[s.num_seqs] = items;
+    __syncthreads();
+    if (sm_bad) {  // an empty batch
+        items = 0;
+        for (int b = tid; b <= s.num_seqs; b += 1024) {
+            p.cu_q[b] = 0;
+            if (b < s.num_seqs) p.kv_len[b] = 0;
+        }
+    }
+    // the prefix is shared only where every sequence's page table agrees
+    if (s.prefix > 0) {
+        const int np = s.prefix >> s.page_shift;
+        for (int i = tid; i < np * s.num_seqs; i += 1024) {
+            const int b = i / np, j = i - b * np;
+            if (table[(size_t)b * s.max_pages + j] != table[j]) sm_noprefix = 1;
+        }
+    }
+    __syncthreads();
+    const int prefix = sm_noprefix ? 0 : s.prefix;
+    int units = 0;
+    for (int i0 = 0; i0 < items; i0 += 1024) {
+        const int i = i0 + tid;
+        int n = 0;
+        if (i < items) {
+            const int b = upper_index(p.item_at, s.num_seqs + 1, i);
+            const int q0 = p.cu_q[b], q1 = p.cu_q[b + 1], t = p.kv_len[b];
+            const int nrow = (q1 - q0) * s.group, r0 = (i - p.item_at[b]) * s.rows;
+            PagedItem it;
+            it.seq = b;
+            it.row0 = r0;
+            it.nrows = min(s.rows, nrow - r0);
+            const int first = t - (q1 - q0) + r0 / s.group;  // position of the first and the last row
+            const int last = t - (q1 - q0) + (r0 + it.nrows - 1) / s.group;
+            int lo = prefix;
+            if (s.window > 0) lo = max(lo, first - s.window + 1);
+            it.unit0 = max(lo, 0) / s.unit;
+            // at least one unit, so that an item whose rows see nothing is still written
+            n = max(1, (last + s.unit) / s.unit - it.unit0);
+            p.items[i] = it;
+        }
+        int total;
+        const int at = block_scan_1024(n, sm, total);
+        if (i < items) p.unit_at[i] = units + at;
+        units += total;
+    }
+    if (tid == 0) p.unit_at[items] = units;
+    for (int i = tid; i < items * s.nkv; i += 1024) p.count[i] = 0;
+    __syncthreads();
+    const long long all = (long long)units * s.nkv;
+    const int per = (int)max((long long)s.min_per, (all + s.ctas - 1) / s.ctas);
+    const int nw = s.workers / s.ctas;
+    for (int w = tid; w < s.workers && units > 0; w += 1024) {
+        // worker w of CTA c: an equal part of the CTA's run [c * per, ...)
+        const int c = w / nw;
+        const long long c0 = (long long)c * per, c1 = min(all, c0 + per);
+        const int pw = (int)((c1 - c0 + nw - 1) / nw);
+        const long long u = c0 + (long long)(w - c * nw) * pw;
+        p.start[w] = u < c1 ? upper_index(p.unit_at, items + 1, (int)(u % units)) : 0;
+    }
+    if (tid == 0) {
+        p.header[kPhStatus] = sm_bad;
+        p.header[kPhItems] = items;
+        p.header[kPhUnits] = units;
+        p.header[kPhPer] = per;
+        p.header[kPhPrefix] = prefix;
+    }
+}
+
+// Each token's sequence and position, (-1, -1) for a token of no sequence or
+// before position 0.
+__global__ void __launch_bounds__(256) k_paged_tokens(const PagedShape s, const PagedPlanView p) {
+    pdl_wait();
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= s.total_q) return;
+    int2 v = make_int2(-1, -1);
+    if (t >= p.cu_q[0] && t < p.cu_q[s.num_seqs]) {
+        const int b = upper_index(p.cu_q, s.num_seqs + 1, t);
+        const int pos = p.kv_len[b] - p.cu_q[b + 1] + t;
+        if (b < s.num_seqs && pos >= 0) v = make_int2(b, pos);
+    }
+    p.tokens[t] = v;
+}
+
+// ----------------------------------------------------------------- append ----
+struct AppendParams {
+    const void *qkv;
+    int qkv_bf16;
+    long long qkv_stride;  // elements between tokens
+    const uint16_t *q_norm, *k_norm;
+    float eps;
+    const float2 *rope;    // [rope_rows][rot / 2] (cos, sin)
+    int rope_rows, rot, pairs;
+    uint16_t *k, *v;
+    uint16_t *q_out;       // [total_q][nh][hd]
+    const int *table;
+    int heads_per_group;   // heads one group of lanes does of one token
+    int groups;            // groups per token
+};
+
+__device__ __forceinline__ void load8(const void *x, int bf16, long long at, float (&v)[8]) {
+    if (bf16) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(x) + at));
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            v[2 * i] = __uint_as_float(u[i] << 16);
+            v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
+        }
+    } else {
+        const float4 *f = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(x) + at);
+        const float4 a = __ldg(f), b = __ldg(f + 1);
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
+        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    }
+}
+
+__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
+    const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t *>(&v);
+}
+
+__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
+    return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+}
+
+// Append: y = rotate(x * rsqrt(mean(x^2) + eps) * w) of each new query and key
+// head, v as it is; q rows go out bf16, k and v rows into their pages.  A
+// group of HD / 8 lanes takes a head, 8 elements (16 bytes of bf16) a lane;
+// all sums in fp32, one rounding at the end.  The group keeps its token's
+// cosines and sines in registers over its heads.  A head half's partner
+// elements (i, i + rot/2) are rot/16 lanes away, adjacent pairs in the lane.
+template <int HD>
+__global__ void __launch_bounds__(256) k_paged_append(const PagedShape s, const PagedPlanView p,
+                                                      const AppendParams a) {
+    constexpr int L = HD / 8;
+    const int gid = (blockIdx.x * 256 + threadIdx.x) / L, l = threadIdx.x % L;
+    pdl_wait();
+    const int t = gid / a.groups, part = gid - t * a.groups;
+    if (t >= s.total_q) return;  // whole groups leave together
+    const unsigned mask = (L == 16 ? 0xFFFFu : 0xFFu) << ((threadIdx.x & 31) / L * L);
+    const int2 tok = p.tokens[t];
+    const bool in_seq = tok.x >= 0;
+    int pos = in_seq ? tok.y : 0;
+    if (pos >= a.rope_rows) {
+        if (l == 0) atomicOr(&p.header[kPhStatus], kPagedErrPosition);
+        pos = 0;
+    }
+    const int half = a.rot >> 1;
+    // this lane's elements 8l .. 8l+7 and the pairs they belong to
+    const bool turns = 8 * l < a.rot;
+    const bool upper = !a.pairs && 8 * l >= half;  // the second half's elements
+    float2 cs[8];
+    if (turns) {
+        const int i0 = a.pairs ? 4 * l : (upper ? 8 * l - half : 8 * l);
+        const float4 *r = reinterpret_cast<const float4 *>(a.rope + (long long)pos * half + i0);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (a.pairs && i >= 2) break;
+            const float4 w = __ldg(r + i);
+            cs[2 * i] = make_float2(w.x, w.y);
+            cs[2 * i + 1] = make_float2(w.z, w.w);
+        }
+    }
+    const int heads = s.nh + 2 * s.nkv;
+    const int h0 = part * a.heads_per_group, h1 = min(heads, h0 + a.heads_per_group);
+    for (int h = h0; h < h1; ++h) {
+        float x[8];
+        load8(a.qkv, a.qkv_bf16, (long long)t * a.qkv_stride + (long long)h * HD + 8 * l, x);
+        const bool is_q = h < s.nh, is_v = h >= s.nh + s.nkv;
+        if (!is_v) {
+            const uint16_t *w = is_q ? a.q_norm : a.k_norm;
+            if (w) {
+                float ss = 0.f;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+                const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
+                float g[8];
+                load8(w, 1, 8 * l, g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * r * g[i];
+            }
+            if (a.pairs) {
+                if (turns) {
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float u = x[2 * i], v = x[2 * i + 1];
+                        x[2 * i] = u * cs[i].x - v * cs[i].y;
+                        x[2 * i + 1] = v * cs[i].x + u * cs[i].y;
+                    }
+                }
+            } else {
+                const int off = half / 8;
+                const int src = turns ? (upper ? l - off : l + off) : l;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float o = __shfl_sync(mask, x[i], src, L);
+                    // first half a cos - b sin, second half b cos + a sin
+                    if (turns) x[i] = upper ? x[i] * cs[i].x + o * cs[i].y : x[i] * cs[i].x - o * cs[i].y;
+                }
+            }
+        }
+        const uint4 y = pack8(x);
+        if (is_q) {
+            *reinterpret_cast<uint4 *>(a.q_out + ((long long)t * s.nh + h) * HD + 8 * l) = y;
+        } else if (in_seq) {
+            const int g = is_v ? h - s.nh - s.nkv : h - s.nh;
+            const int row = paged_row(s, a.table, tok.x, g, tok.y, &p.header[kPhStatus]);
+            uint16_t *pool = is_v ? a.v : a.k;
+            if (row >= 0) *reinterpret_cast<uint4 *>(pool + (long long)row * HD + 8 * l) = y;
+        }
+    }
+}
+
+}  // namespace m1

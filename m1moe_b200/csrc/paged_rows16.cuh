@@ -1,0 +1,573 @@
+// paged_rows16.cuh — attention of at most 16 rows (new tokens x heads of one
+// KV head) per item over a paged cache: the decode step's kernel (sm_100a).
+//
+//   out[r] = sum_p w(r, p) v[p] / sum_p w(r, p),
+//   w(r, p) = exp(cap(scale q[r] . k[p]) - m_r) over the positions row r sees.
+//
+// It reads each K and V row of a (sequence, KV head) once for all the rows
+// that share it, so HBM bounds it.  Work is cut evenly in units of 16
+// positions (8 KB at hd 128) over every warp of the GPU, whatever the lengths are
+// (paged.cuh); a warp streams its run of units through a ring of its own in
+// shared memory (cp.async, 16 bytes a lane: pages may be as small as 16
+// rows, positions outside the item are filled with zeros, so what lies in a
+// page's unused rows never enters a sum) and no warp waits for another
+// before its run ends.  A unit is two m16n8k16 products for the scores and
+// 16 positions' weights times V; the tile's 16 rows are mostly padding in a
+// decode step, which costs nothing while the copies are the bound.  A
+// 16-byte chunk c of row r is stored at chunk c ^ (r & 7), so that the eight
+// rows of an ldmatrix fall in different banks.  Scores, maxima, sums and
+// weighted values are fp32; the weights are rounded to bf16 for the second
+// product (the sum takes them unrounded), an error of 2^-9 of each weight
+// beside the output's own rounding of 2^-9.
+#pragma once
+
+#include "paged.cuh"
+
+namespace m1 {
+
+struct RowsParams {
+    const uint16_t *q;
+    long long q_stride;  // elements between tokens
+    const uint16_t *k, *v;
+    const int *table;
+    float scale, cap;
+    void *out;
+    int out_bf16;
+    long long out_stride;
+    int stages;          // ring stages per warp
+    int part_rows;       // rows kept of a partial: group * max_q
+    const float *prefix_part;  // [total_q][nh][hd] merged in when the header names a prefix
+    const float2 *prefix_ml;   // [total_q][nh]
+};
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The score in units of log2: cap * tanh(s / cap) * log2(e), or s * log2(e).
+// tanh(x) = 1 - 2 / (1 + e^2x): the absolute error stays near 1e-7.
+__device__ __forceinline__ float score_log2(float dot, float scale_log2, float cap, float two_over_cap_scaled) {
+    if (cap > 0.f) {
+        const float e = exp2_approx(dot * two_over_cap_scaled);
+        return cap * kLog2e * (1.f - __fdividef(2.f, 1.f + e));
+    }
+    return dot * scale_log2;
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
+    const int n = valid ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+
+// Wait until at most n (0..3) of this thread's copy groups are in flight.
+__device__ __forceinline__ void cp_async_wait(int n) {
+    if (n == 0)
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+    else if (n == 1)
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else if (n == 2)
+        asm volatile("cp.async.wait_group 2;" ::: "memory");
+    else
+        asm volatile("cp.async.wait_group 3;" ::: "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr)
+                 : "memory");
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+        "{%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A warp's place in the work: unit u of [u, end) lies in item `item` of KV
+// head g; [seg0, seg1) are that item's units.
+struct UnitCursor {
+    int u, end, g, item, seg0, seg1;
+    __device__ __forceinline__ void locate(const PagedPlanView &p, int units) {
+        seg0 = g * units + p.unit_at[item];
+        seg1 = g * units + p.unit_at[item + 1];
+    }
+    __device__ __forceinline__ void next_item(const PagedPlanView &p, int units, int items) {
+        if (++item == items) item = 0, ++g;
+        locate(p, units);
+    }
+};
+
+// Merge of n partials of one row, 4 (HD 128) or 2 (HD 64) output elements a
+// lane; get(i, m, l, o) gives partial i.
+template <int HD, class Get>
+__device__ __forceinline__ void merge_partials(int n, Get get, float &m, float &l, float (&o)[HD / 32]) {
+    constexpr int E = HD / 32;
+    m = -INFINITY;
+    l = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] = 0.f;
+    for (int i = 0; i < n; ++i) {
+        float mi, li, oi[E];
+        get(i, mi, li, oi);
+        const float mn = fmaxf(m, mi);
+        const float c = m == -INFINITY ? 0.f : exp2_approx(m - mn);
+        const float ci = mi == -INFINITY ? 0.f : exp2_approx(mi - mn);
+        l = l * c + li * ci;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = o[e] * c + oi[e] * ci;
+        m = mn;
+    }
+}
+
+template <int HD>
+__device__ __forceinline__ void load_vec(const float *p, float (&o)[HD / 32]) {
+    if constexpr (HD == 128) {
+        const float4 x = *reinterpret_cast<const float4 *>(p);
+        o[0] = x.x, o[1] = x.y, o[2] = x.z, o[3] = x.w;
+    } else {
+        const float2 x = *reinterpret_cast<const float2 *>(p);
+        o[0] = x.x, o[1] = x.y;
+    }
+}
+template <int HD>
+__device__ __forceinline__ void store_vec(float *p, const float (&o)[HD / 32]) {
+    if constexpr (HD == 128)
+        *reinterpret_cast<float4 *>(p) = make_float4(o[0], o[1], o[2], o[3]);
+    else
+        *reinterpret_cast<float2 *>(p) = make_float2(o[0], o[1]);
+}
+template <int HD>
+__device__ __forceinline__ void store_out(const RowsParams &a, long long at, const float (&o)[HD / 32]) {
+    if (a.out_bf16) {
+        uint16_t *p = reinterpret_cast<uint16_t *>(a.out) + at;
+        if constexpr (HD == 128)
+            *reinterpret_cast<uint2 *>(p) = make_uint2(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]));
+        else
+            *reinterpret_cast<uint32_t *>(p) = pack_bf16(o[0], o[1]);
+    } else {
+        store_vec<HD>(reinterpret_cast<float *>(a.out) + at, o);
+    }
+}
+
+template <int HD>
+__device__ __forceinline__ void load_vec_cg(const float *p, float (&o)[HD / 32]) {
+    if constexpr (HD == 128) {
+        const float4 x = __ldcg(reinterpret_cast<const float4 *>(p));
+        o[0] = x.x, o[1] = x.y, o[2] = x.z, o[3] = x.w;
+    } else {
+        const float2 x = __ldcg(reinterpret_cast<const float2 *>(p));
+        o[0] = x.x, o[1] = x.y;
+    }
+}
+
+// One row's end: the shared prefix's partial (if any) joins, then the row is
+// divided by its sum and written.  A row that saw nothing is zero.
+template <int HD>
+__device__ __forceinline__ void finish_row(const PagedShape &s, const RowsParams &a, int prefix, int token, int head,
+                                           float m, float l, float (&o)[HD / 32]) {
+    constexpr int E = HD / 32;
+    const int lane = threadIdx.x & 31;
+    if (prefix > 0) {
+        const long long r = (long long)token * s.nh + head;
+        const float2 ml = a.prefix_ml[r];
+        float x[E];
+        load_vec<HD>(a.prefix_part + r * HD + lane * E, x);
+        const float mn = fmaxf(m, ml.x);
+        const float c = m == -INFINITY ? 0.f : exp2_approx(m - mn);
+        const float ci = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - mn);
+        l = l * c + ml.y * ci;
+#pragma unroll
+        for (int e = 0; e < E; ++e) o[e] = o[e] * c + x[e] * ci;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] *= inv;
+    store_out<HD>(a, (long long)token * a.out_stride + (long long)head * HD + lane * E, o);
+}
+
+// Shared memory of one warp: `stages` units of K and V, then the rows of a
+// partial that ended before the warp's run did.
+template <int HD>
+__host__ __device__ constexpr int rows16_unit_bytes() {
+    return 2 * kPagedUnitSmall * HD * 2;
+}
+
+// What a warp left unfinished: a first segment begun before its run and
+// ended in it (`front`, kept apart), and a last one that its run did not end.
+struct Rows16Left {
+    int front, front_g, front_item;
+    int open_right, open_left, g, item;
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const PagedShape s, const PagedPlanView p,
+                                                                      const RowsParams a) {
+    constexpr int E = HD / 32, KS = HD / 16, NT = HD / 8, CH = HD / 8;  // CH: 16-byte chunks per row
+    constexpr int kRow = HD * 2, kHalf = kPagedUnitSmall * kRow, kUnit = 2 * kHalf;
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ Rows16Left left[kPagedWarps];
+    __shared__ float2 ml_front[kPagedWarps][kPagedRowsSmall], ml_last[kPagedWarps][kPagedRowsSmall];
+    __shared__ int sm_last;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
+    const int warp_bytes = a.stages * kUnit + a.part_rows * HD * 4;
+    uint8_t *ring = smem + (size_t)warp * warp_bytes;
+    float *front = reinterpret_cast<float *>(ring + a.stages * kUnit);
+    const uint32_t ring_addr = smem_addr(ring);
+    pdl_wait();
+    const int units = p.header[kPhUnits], items = p.header[kPhItems], per = p.header[kPhPer];
+    const int prefix = p.header[kPhPrefix];
+    int *status = &p.header[kPhStatus];
+    const int all = units * s.nkv;
+    const int c0 = min(cta * per, all), c1 = min(all, c0 + per);
+    const int pw = (c1 - c0 + kPagedWarps - 1) / kPagedWarps;
+    UnitCursor cur;
+    cur.u = min(c1, c0 + warp * pw);
+    cur.end = min(c1, cur.u + pw);
+    const bool work = cur.u < cur.end;
+    const int begin = cur.u;
+    Rows16Left mine = {0, 0, 0, 0, 0, 0, 0};
+    if (work) {
+        cur.g = cur.u / units;
+        cur.item = p.start[cta * kPagedWarps + warp];
+        cur.locate(p, units);
+        UnitCursor ld = cur;  // the loader runs ahead
+        PagedItem ld_item = p.items[ld.item];
+        int ld_len = p.kv_len[ld_item.seq], ld_lo = 0;
+        auto item_lo = [&](const PagedItem &it, int len) {  // first position any row of the item sees
+            int lo = prefix;
+            if (s.window > 0) {
+                const int first = len - (p.cu_q[it.seq + 1] - p.cu_q[it.seq]) + it.row0 / s.group;
+                lo = max(lo, first - s.window + 1);
+            }
+            return lo;
+        };
+        ld_lo = item_lo(ld_item, ld_len);
+        int slot = 0;
+        auto load_unit = [&]() {
+            if (ld.u < ld.end) {
+                if (ld.u == ld.seg1) {
+                    ld.next_item(p, units, items);
+                    ld_item = p.items[ld.item];
+                    ld_len = p.kv_len[ld_item.seq];
+                    ld_lo = item_lo(ld_item, ld_len);
+                }
+                const int pos = (ld_item.unit0 + ld.u - ld.seg0) * kPagedUnitSmall;
+                // all 16 positions lie in one page (page sizes are multiples of 16)
+                int row = -1;
+                if (pos < ld_len) row = paged_row(s, a.table, ld_item.seq, ld.g, pos, status);
+                const long long at = (long long)max(row, 0) * HD;
+                const uint32_t dst = ring_addr + slot * kUnit;
+#pragma unroll
+                for (int i = 0; i < kPagedUnitSmall * CH / 32; ++i) {
+                    const int r = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH;
+                    const bool ok = row >= 0 && pos + r < ld_len && pos + r >= ld_lo;
+                    const uint32_t d = dst + r * kRow + ((c ^ (r & 7)) << 4);
+                    const long long src = ok ? at + r * HD + c * 8 : 0;
+                    cp_async16(d, a.k + src, ok);
+                    cp_async16(d + kHalf, a.v + src, ok);
+                }
+                ++ld.u;
+                if (++slot == a.stages) slot = 0;
+            }
+            cp_async_commit();
+        };
+        for (int i = 0; i < a.stages - 1; ++i) load_unit();
+        int use = 0;
+        uint32_t qf[KS][4];
+        float o[NT][4], m[2], l[2];
+        int hi[2], lo[2];  // positions the lane's two rows see
+        int min_hi = 0, max_lo = 0;
+        const float sl2 = a.scale * kLog2e, c2 = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
+        PagedItem it;
+        auto open_segment = [&]() {
+            it = p.items[cur.item];
+            const int q0 = p.cu_q[it.seq], nq = p.cu_q[it.seq + 1] - q0, len = p.kv_len[it.seq];
+            const uint16_t *qr[2];
+            bool ok[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = lane / 4 + 8 * h;
+                ok[h] = r < it.nrows;
+                const int row = it.row0 + (ok[h] ? r : 0), tok = row / s.group;
+                qr[h] = a.q + (long long)(q0 + tok) * a.q_stride + (long long)(cur.g * s.group + row - tok * s.group) * HD;
+                hi[h] = len - nq + tok;
+                lo[h] = prefix;
+                if (s.window > 0) lo[h] = max(lo[h], hi[h] - s.window + 1);
+                m[h] = -INFINITY;
+                l[h] = 0.f;
+            }
+            min_hi = len - nq + it.row0 / s.group;
+            const int max_hi = len - nq + (it.row0 + it.nrows - 1) / s.group;
+            max_lo = prefix;
+            if (s.window > 0) max_lo = max(max_lo, max_hi - s.window + 1);
+#pragma unroll
+            for (int k = 0; k < KS; ++k)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int h = j & 1, at = 16 * k + 8 * (j >> 1) + 2 * (lane & 3);
+                    qf[k][j] = ok[h] ? *reinterpret_cast<const uint32_t *>(qr[h] + at) : 0u;
+                }
+#pragma unroll
+            for (int n = 0; n < NT; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.f;
+        };
+        // this lane's part of the row sums joins its quad's
+        auto row_sums = [&]() {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+                l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+            }
+        };
+        // the segment's rows as a partial in shared memory
+        auto store_partial = [&](float *dst, float2 *ml) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = lane / 4 + 8 * h;
+                if (r < it.nrows) {
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        *reinterpret_cast<float2 *>(dst + r * HD + 8 * n + 2 * (lane & 3)) =
+                            make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                    if ((lane & 3) == 0) ml[r] = make_float2(m[h], l[h]);
+                }
+            }
+            __syncwarp();
+        };
+        // the finished rows of an item, straight from the accumulators
+        auto write_rows = [&]() {
+            const int q0 = p.cu_q[it.seq];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int r = lane / 4 + 8 * h;
+                if (r >= it.nrows) continue;
+                const int row = it.row0 + r, tok = row / s.group;
+                const int token = q0 + tok, head = cur.g * s.group + row - tok * s.group;
+                const long long pr = (long long)token * s.nh + head;
+                float c = 1.f, ci = 0.f, sum = l[h];
+                if (prefix > 0) {
+                    const float2 ml = a.prefix_ml[pr];
+                    const float mn = fmaxf(m[h], ml.x);
+                    c = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - mn);
+                    ci = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - mn);
+                    sum = sum * c + ml.y * ci;
+                }
+                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                const long long at = (long long)token * a.out_stride + (long long)head * HD;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const int col = 8 * n + 2 * (lane & 3);
+                    float x0 = o[n][2 * h] * c, x1 = o[n][2 * h + 1] * c;
+                    if (prefix > 0) {
+                        const float2 y = *reinterpret_cast<const float2 *>(a.prefix_part + pr * HD + col);
+                        x0 += y.x * ci, x1 += y.y * ci;
+                    }
+                    x0 *= inv, x1 *= inv;
+                    if (a.out_bf16)
+                        *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.out) + at + col) = pack_bf16(x0, x1);
+                    else
+                        *reinterpret_cast<float2 *>(reinterpret_cast<float *>(a.out) + at + col) = make_float2(x0, x1);
+                }
+            }
+        };
+        open_segment();
+        for (; cur.u < cur.end; ++cur.u) {
+            load_unit();
+            if (cur.u == cur.seg1) {
+                cur.next_item(p, units, items);
+                open_segment();
+            }
+            cp_async_wait(a.stages - 1);
+            __syncwarp();
+            const uint32_t kb = ring_addr + use * kUnit, vb = kb + kHalf;
+            // scores: two n8 tiles of positions
+            float sc[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            {
+                const int r = (lane & 7) + ((lane >> 4) << 3), cb = (lane >> 3) & 1;
+                const uint32_t base = kb + r * kRow;
+#pragma unroll
+                for (int k = 0; k < KS; ++k) {
+                    uint32_t b[4];
+                    ldsm4(base + (((2 * k + cb) ^ (r & 7)) << 4), b);
+                    mma_bf16(sc[0], qf[k], b[0], b[1]);
+                    mma_bf16(sc[1], qf[k], b[2], b[3]);
+                }
+            }
+            const int pos = (it.unit0 + cur.u - cur.seg0) * kPagedUnitSmall;
+            float mx[2] = {m[0], m[1]};
+            const bool whole = pos >= max_lo && pos + kPagedUnitSmall - 1 <= min_hi;
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int h = j >> 1;
+                    float x = score_log2(sc[t][j], sl2, a.cap, c2);
+                    if (!whole) {
+                        const int at = pos + 8 * t + 2 * (lane & 3) + (j & 1);
+                        if (at > hi[h] || at < lo[h]) x = -INFINITY;
+                    }
+                    sc[t][j] = x;
+                    mx[h] = fmaxf(mx[h], x);
+                }
+            float c[2], ref[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+                mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+                ref[h] = mx[h] == -INFINITY ? 0.f : mx[h];  // nothing seen yet: all weights are 0
+                c[h] = exp2_approx(m[h] - ref[h]);
+                m[h] = mx[h];
+                l[h] *= c[h];
+            }
+            uint32_t pf[4];
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float w[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    w[j] = exp2_approx(sc[t][j] - ref[j >> 1]);
+                    l[j >> 1] += w[j];
+                }
+                pf[2 * t] = pack_bf16(w[0], w[1]);
+                pf[2 * t + 1] = pack_bf16(w[2], w[3]);
+            }
+            if (__any_sync(0xffffffffu, c[0] != 1.f || c[1] != 1.f)) {
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    o[n][0] *= c[0], o[n][1] *= c[0];
+                    o[n][2] *= c[1], o[n][3] *= c[1];
+                }
+            }
+            {
+                const int r = lane & 15, cb = lane >> 4;
+                const uint32_t base = vb + r * kRow;
+#pragma unroll
+                for (int n = 0; n < NT; n += 2) {
+                    uint32_t b[4];
+                    ldsm4_t(base + (((n + cb) ^ (r & 7)) << 4), b);
+                    mma_bf16(o[n], pf, b[0], b[1]);
+                    mma_bf16(o[n + 1], pf, b[2], b[3]);
+                }
+            }
+            __syncwarp();  // the stage may be filled again
+            if (++use == a.stages) use = 0;
+            if (cur.u + 1 == cur.seg1) {
+                row_sums();
+                if (cur.seg0 >= begin) {
+                    write_rows();  // the whole item was this warp's
+                } else {
+                    store_partial(front, ml_front[warp]);
+                    mine.front = 1;
+                    mine.front_g = cur.g;
+                    mine.front_item = cur.item;
+                }
+            } else if (cur.u + 1 == cur.end) {
+                row_sums();
+                store_partial(reinterpret_cast<float *>(ring), ml_last[warp]);  // the ring is drained
+                mine.open_right = 1;
+                mine.open_left = cur.seg0 < begin;
+                mine.g = cur.g;
+                mine.item = cur.item;
+            }
+        }
+    }
+    if (lane == 0) left[warp] = mine;
+    __syncthreads();
+    // The warps' unfinished segments, joined item by item in position order:
+    // a group starts at a warp whose last segment begins its item (or at warp
+    // 0, whatever it begins with) and runs on over the following warps.
+    // Every warp takes every eighth row.
+    auto join = [&](int w0, bool from_front, int n, bool closed, bool open_left, int g, int item) {
+        const PagedItem it = p.items[item];
+        const int q0 = p.cu_q[it.seq];
+        const bool done = closed && !open_left;
+        const int slot = 2 * cta + (open_left ? 0 : 1);
+        for (int r = warp; r < it.nrows; r += kPagedWarps) {
+            float m, l, o[E];
+            merge_partials<HD>(
+                n,
+                [&](int i, float &mi, float &li, float (&oi)[E]) {
+                    const bool f = from_front || (closed && i == n - 1);
+                    const float2 ml = f ? ml_front[w0 + i][r] : ml_last[w0 + i][r];
+                    mi = ml.x, li = ml.y;
+                    const uint8_t *base = smem + (size_t)(w0 + i) * warp_bytes + (f ? a.stages * kUnit : 0);
+                    load_vec<HD>(reinterpret_cast<const float *>(base) + r * HD + lane * E, oi);
+                },
+                m, l, o);
+            const int row = it.row0 + r, tok = row / s.group;
+            if (done) {
+                finish_row<HD>(s, a, prefix, q0 + tok, g * s.group + row - tok * s.group, m, l, o);
+            } else {
+                const size_t at = (size_t)slot * a.part_rows + r;
+                store_vec<HD>(p.part + at * HD + lane * E, o);
+                if (lane == 0) p.part_ml[at] = make_float2(m, l);
+            }
+        }
+    };
+    int open_n = 0, open_g[2], open_item[2];  // groups that other CTAs' partials complete
+    for (int w = 0; w < kPagedWarps; ++w) {
+        const Rows16Left h = left[w];
+        if (w == 0 && h.front) {
+            join(0, true, 1, true, true, h.front_g, h.front_item);
+            open_g[open_n] = h.front_g, open_item[open_n++] = h.front_item;
+        }
+        if (h.open_right && (w == 0 || !h.open_left)) {
+            int n = 1;
+            bool closed = false;
+            for (; w + n < kPagedWarps && !closed; ++n) {
+                const Rows16Left &x = left[w + n];
+                if (x.front)
+                    closed = true;
+                else if (!(x.open_right && x.open_left))
+                    break;
+            }
+            join(w, false, n, closed, h.open_left, h.g, h.item);
+            if ((!closed || h.open_left) && open_n < 2) open_g[open_n] = h.g, open_item[open_n++] = h.item;
+        }
+    }
+    for (int i = 0; i < open_n; ++i) {
+        const int g = open_g[i], item = open_item[i];
+        const int first = (g * units + p.unit_at[item]) / per, last = (g * units + p.unit_at[item + 1] - 1) / per;
+        __threadfence();
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            int *cnt = p.count + g * items + item;
+            sm_last = atomicAdd(cnt, 1) == last - first;
+            if (sm_last) *cnt = 0;  // ready for the next call
+        }
+        __syncthreads();
+        if (!sm_last) continue;
+        __threadfence();
+        const PagedItem it = p.items[item];
+        const int q0 = p.cu_q[it.seq];
+        for (int r = warp; r < it.nrows; r += kPagedWarps) {
+            float m, l, o[E];
+            merge_partials<HD>(
+                last - first + 1,
+                [&](int k, float &mi, float &li, float (&oi)[E]) {
+                    // the item's first CTA begins it, the others begin with it
+                    const size_t at = (size_t)(2 * (first + k) + (k == 0 ? 1 : 0)) * a.part_rows + r;
+                    const float2 ml = __ldcg(p.part_ml + at);
+                    mi = ml.x, li = ml.y;
+                    load_vec_cg<HD>(p.part + at * HD + lane * E, oi);
+                },
+                m, l, o);
+            const int row = it.row0 + r, tok = row / s.group;
+            finish_row<HD>(s, a, prefix, q0 + tok, g * s.group + row - tok * s.group, m, l, o);
+        }
+    }
+}
+
+}  // namespace m1

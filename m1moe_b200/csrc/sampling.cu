@@ -1,0 +1,84 @@
+// sampling.cu — C ABI of the sampler (include/m1moe_cuda.h, m1moe_cuda_sample).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+
+#include "m1moe_cuda.h"
+#include "sampling.cuh"
+
+// The error helpers and launch counter of m1moe_cuda.cu (one library).
+namespace m1abi {
+m1moe_status fail(m1moe_status st, const char *fmt, ...);
+m1moe_status cuda_fail(cudaError_t e, const char *what);
+void count_launch();
+}  // namespace m1abi
+
+using m1abi::cuda_fail;
+using m1abi::fail;
+
+namespace {
+constexpr size_t kSliceCap = 200 * 1024;  // dynamic shared memory beside the histograms
+}
+
+extern "C" {
+
+m1moe_status m1moe_cuda_sample(const void *d_logits, int32_t dtype, int64_t row_stride, int32_t rows, int32_t vocab,
+                               const float *d_u, const float *d_temperature, float temperature,
+                               const int32_t *d_top_k, int32_t top_k, const float *d_top_p, float top_p,
+                               const float *d_min_p, float min_p, int32_t *d_tokens, void *stream) {
+    if (dtype != M1MOE_DTYPE_F32 && dtype != M1MOE_DTYPE_BF16)
+        return fail(M1MOE_ERR_INVALID_ARG, "dtype must be F32 (0) or BF16 (1)");
+    if (rows < 0 || vocab <= 0 || vocab > (1 << 20))
+        return fail(M1MOE_ERR_INVALID_ARG, "rows %d, vocab %d: rows >= 0, vocab 1 to %d", rows, vocab, 1 << 20);
+    if (row_stride < vocab) return fail(M1MOE_ERR_INVALID_ARG, "row_stride is below vocab");
+    if (!(temperature >= 0.f) || !(top_p >= 0.f) || !(min_p >= 0.f && min_p <= 1.f))
+        return fail(M1MOE_ERR_INVALID_ARG, "temperature and top_p must be >= 0, min_p in [0, 1]");
+    if (rows == 0) return M1MOE_OK;
+    if (!d_logits || !d_u || !d_tokens) return fail(M1MOE_ERR_INVALID_ARG, "NULL pointer");
+    m1::SampleParams p{};
+    p.logits = d_logits;
+    p.bf16 = dtype == M1MOE_DTYPE_BF16;
+    p.stride = row_stride;
+    p.vocab = vocab;
+    p.u = d_u;
+    p.temperature = d_temperature;
+    p.top_k = d_top_k;
+    p.top_p = d_top_p;
+    p.min_p = d_min_p;
+    p.temperature1 = temperature;
+    p.top_k1 = top_k;
+    p.top_p1 = top_p;
+    p.min_p1 = min_p;
+    p.tokens = d_tokens;
+    // CTAs per row: enough for the slice to fit in shared memory, more while
+    // SMs would be idle
+    int c = 1;
+    while (c < m1::kSampleMaxCluster && ((size_t)((vocab + c - 1) / c) * 4 > kSliceCap || (long long)rows * c * 2 <= 148))
+        c *= 2;
+    if ((long long)rows * c > 0x7FFFFFFFLL) return fail(M1MOE_ERR_UNSUPPORTED, "%d rows are too many", rows);
+    p.slice = (vocab + c - 1) / c;
+    const size_t bytes = (size_t)p.slice * 4;
+    p.in_smem = bytes <= kSliceCap;
+    cudaError_t e = cudaFuncSetAttribute(m1::k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSliceCap);
+    if (e != cudaSuccess) return cuda_fail(e, "k_sample shared memory");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)rows * c);
+    cfg.blockDim = dim3(m1::kSampleThreads);
+    cfg.dynamicSmemBytes = p.in_smem ? bytes : 0;
+    cfg.stream = reinterpret_cast<cudaStream_t>(stream);
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = c;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 2;
+    e = cudaLaunchKernelEx(&cfg, m1::k_sample, p);
+    if (e != cudaSuccess) return cuda_fail(e, "k_sample launch");
+    m1abi::count_launch();
+    return M1MOE_OK;
+}
+
+}  // extern "C"

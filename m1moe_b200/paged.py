@@ -1,0 +1,235 @@
+"""A paged key/value cache and its operators, for batches of sequences of different lengths.
+
+Thin wrappers over the C ABI (include/m1moe_cuda.h, m1moe_cuda_paged_*); torch supplies
+device memory and streams, every computation runs in libm1moe_cuda.so.
+
+  PagedKVCache     the bf16 pools of every layer, [layers][pages][kv heads][page size][head dim]
+  PagedBatch       one step's sequences: their new tokens, lengths and pages, and the plan that
+                   every layer's calls share
+  paged_append     per-head RMSNorm, rotary embedding and the store of the new keys and values
+                   (InferenceEngine.swift:194-220, 521-548)
+  paged_attention  causal attention over the pages (InferenceEngine.swift:349-399)
+  rope_table       cosines and sines of every position, also scaled for long contexts
+
+A batch's calls use its plan's partial results and so belong on one stream, in order.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import _lib
+from .expert_ffn import _stream, dtype_code
+
+
+class PagedKVCache:
+    def __init__(self, *, num_layers: int, num_kv_heads: int, num_pages: int, page_size: int,
+                 head_dim: int = 128, device: int = 0):
+        shape = (num_layers, num_pages, num_kv_heads, page_size, head_dim)
+        dev = torch.device("cuda", device)
+        self._adopt(torch.zeros(shape, dtype=torch.bfloat16, device=dev),
+                    torch.zeros(shape, dtype=torch.bfloat16, device=dev))
+
+    @classmethod
+    def from_tensors(cls, k: torch.Tensor, v: torch.Tensor) -> "PagedKVCache":
+        """Pools that the caller owns: bf16 [layers][pages][kv heads][page size][head dim]."""
+        self = cls.__new__(cls)
+        self._adopt(k, v)
+        return self
+
+    def _adopt(self, k, v):
+        if k.dim() != 5 or k.shape != v.shape:
+            raise ValueError("k and v are [layers][pages][kv heads][page size][head dim]")
+        for t in (k, v):
+            if not t.is_cuda or t.dtype != torch.bfloat16 or not t.is_contiguous():
+                raise ValueError("the pools are contiguous bfloat16 CUDA tensors")
+        if k.device != v.device:
+            raise ValueError("k and v are on different devices")
+        self.k, self.v = k, v
+        self.num_layers, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
+        self.device = k.device
+        self._layer_bytes = k[0].numel() * 2 if self.num_layers else 0
+        self._k0, self._v0 = k.data_ptr(), v.data_ptr()
+
+    def _ptrs(self, layer: int) -> tuple[int, int]:
+        if not 0 <= layer < self.num_layers:
+            raise ValueError(f"layer {layer} out of range [0,{self.num_layers})")
+        return self._k0 + layer * self._layer_bytes, self._v0 + layer * self._layer_bytes
+
+
+class PagedBatch:
+    """The sequences of one step.
+
+    q_lens      new tokens of each sequence (host integers; 0 is allowed)
+    kv_lens     all tokens of each sequence, the new ones included (host integers or an int32
+                CUDA tensor, kept as `kv_lens`)
+    page_table  int32 CUDA [sequences][most pages]; unused entries are never read
+    window      positions a token sees, itself included (0: all before it)
+    shared_prefix  positions at the start, whole pages, that all page tables share: attention
+                   may then read them once for the batch; a hint that changes no result
+    """
+
+    def __init__(self, cache: PagedKVCache, q_lens, kv_lens, page_table: torch.Tensor, *, num_heads: int,
+                 window: int = 0, shared_prefix: int = 0, stream=None):
+        dev = cache.device
+        q = [int(x) for x in (q_lens.tolist() if isinstance(q_lens, torch.Tensor) else q_lens)]
+        if not q or min(q) < 0:
+            raise ValueError("q_lens: at least one sequence, no negative length")
+        if not isinstance(kv_lens, torch.Tensor):
+            kv_lens = torch.tensor([int(x) for x in kv_lens], dtype=torch.int32, device=dev)
+        for t, name, dim in ((kv_lens, "kv_lens", 1), (page_table, "page_table", 2)):
+            if t.device != dev or t.dtype != torch.int32 or t.dim() != dim or not t.is_contiguous():
+                raise ValueError(f"{name}: a contiguous int32 tensor of {dim} dimension(s) on {dev}")
+            if t.shape[0] != len(q):
+                raise ValueError(f"{name} has {t.shape[0]} rows for {len(q)} sequences")
+        cu = [0]
+        for x in q:
+            cu.append(cu[-1] + x)
+        self.cache, self.page_table, self.kv_lens = cache, page_table, kv_lens
+        self.num_seqs, self.total_q, self.max_q = len(q), cu[-1], max(q)
+        self.num_heads = num_heads
+        self.cu_q = torch.tensor(cu, dtype=torch.int32, device=dev)
+        self.cfg = _lib.PagedCfg(num_heads, cache.num_kv_heads, cache.head_dim, cache.page_size, cache.num_pages,
+                                 len(q), page_table.shape[1], cu[-1], max(q), window, shared_prefix)
+        self._cfg = ctypes.addressof(self.cfg)
+        with torch.cuda.device(dev):
+            nbytes = _lib.lib().m1moe_cuda_paged_plan_bytes(self._cfg)
+            if nbytes == 0:
+                msg = _lib.lib().m1moe_cuda_last_error()
+                raise ValueError(f"paged batch refused: {msg.decode() if msg else ''}")
+            # torch's allocations are 512-byte aligned
+            self.plan = torch.empty(nbytes, dtype=torch.uint8, device=dev)
+        self._home = torch.cuda.current_stream(dev).cuda_stream
+        self._plan, self._table = self.plan.data_ptr(), page_table.data_ptr()
+        self.update(stream=stream)
+
+    def update(self, *, stream=None) -> None:
+        """Make the plan again from `cu_q`, `kv_lens` and `page_table` as they are on the device
+        now (for a next step with the same new tokens per sequence; capturable)."""
+        st = self._use(stream)
+        with torch.cuda.device(self.cache.device):
+            _lib.call("m1moe_cuda_paged_plan", self._cfg, self.cu_q.data_ptr(), self.kv_lens.data_ptr(), self._table,
+                      self._plan, self.plan.numel(), st)
+
+    def check(self, *, stream=None) -> None:
+        """Wait for the stream and raise if a kernel found a length, page or position out of range."""
+        with torch.cuda.device(self.cache.device):
+            _lib.call("m1moe_cuda_paged_status", self._plan, self._use(stream))
+
+    def _use(self, stream) -> int:
+        st = _stream(stream)
+        if st != self._home:  # keep the memory until this stream is done with it
+            s = stream if stream is not None else torch.cuda.current_stream()
+            for t in (self.plan, self.cu_q, self.kv_lens, self.page_table):
+                t.record_stream(s)
+        return st
+
+
+def _empty(shape, dtype, device, stream):
+    """Output memory that belongs to the stream the kernel runs on."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
+def paged_append(cache: PagedKVCache, layer: int, batch: PagedBatch, qkv: torch.Tensor, *, rope: torch.Tensor,
+                 rope_pairs: bool = False, q_norm: torch.Tensor | None = None, k_norm: torch.Tensor | None = None,
+                 eps: float = 1e-5, out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """Store the batch's new keys and values; returns the queries, bf16 [total_q][heads][head dim].
+
+    qkv     f32 or bf16 [total_q][(heads + 2 kv heads) * head dim], rows q | k | v, which may lie
+            further apart than their length
+    rope    f32 [positions][rot/2][2] (rope_table); rot <= head dim elements of each head turn, i
+            with i + rot/2 or, with rope_pairs, 2i with 2i + 1
+    q_norm, k_norm  bf16 [head dim] RMSNorm weights of each head, or None
+    """
+    nh, hd = batch.num_heads, cache.head_dim
+    if qkv.dim() != 2 or qkv.shape[0] != batch.total_q or qkv.shape[1] != (nh + 2 * cache.num_kv_heads) * hd:
+        raise ValueError(f"qkv is {tuple(qkv.shape)}, expected ({batch.total_q}, {(nh + 2 * cache.num_kv_heads) * hd})")
+    if qkv.device != cache.device or qkv.stride(1) != 1:
+        raise ValueError("qkv: rows of contiguous elements on the cache's device")
+    if rope.device != cache.device or rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or \
+            not rope.is_contiguous():
+        raise ValueError("rope: a contiguous float32 [positions][rot/2][2] tensor on the cache's device")
+    for w in (q_norm, k_norm):
+        if w is not None and (w.device != cache.device or w.dtype != torch.bfloat16 or w.shape != (hd,) or
+                              not w.is_contiguous()):
+            raise ValueError(f"norm weights: contiguous bfloat16 [{hd}] on the cache's device")
+    k, v = cache._ptrs(layer)
+    st = batch._use(stream)
+    if out is None:
+        out = _empty((batch.total_q, nh, hd), torch.bfloat16, cache.device, stream)
+    elif out.shape != (batch.total_q, nh, hd) or out.dtype != torch.bfloat16 or not out.is_contiguous() or \
+            out.device != cache.device:
+        raise ValueError(f"out: contiguous bfloat16 ({batch.total_q}, {nh}, {hd}) on the cache's device")
+    if batch.total_q == 0:
+        return out
+    _lib.call("m1moe_cuda_paged_append", batch._cfg, batch._plan, batch._table, qkv.data_ptr(), dtype_code(qkv.dtype),
+              qkv.stride(0), 0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(),
+              eps, rope.data_ptr(), rope.shape[0], 2 * rope.shape[1], 1 if rope_pairs else 0, k, v, out.data_ptr(), st)
+    return out
+
+
+def paged_attention(cache: PagedKVCache, layer: int, batch: PagedBatch, q: torch.Tensor, *,
+                    scale: float | None = None, softcap: float = 0.0, out: torch.Tensor | None = None,
+                    out_dtype: torch.dtype = torch.bfloat16, stream=None) -> torch.Tensor:
+    """Attention of the batch's new tokens (q bf16 [total_q][heads][head dim], tokens may lie
+    further apart) over their sequences; scores are scale * q.k (default 1/sqrt(head dim)), capped
+    as softcap * tanh(score / softcap) if softcap > 0."""
+    nh, hd = batch.num_heads, cache.head_dim
+    for t, name in ((q, "q"), (out, "out")):
+        if t is not None and (t.shape != (batch.total_q, nh, hd) or t.device != cache.device or
+                              (t.numel() and (t.stride(2) != 1 or t.stride(1) != hd))):
+            raise ValueError(f"{name}: ({batch.total_q}, {nh}, {hd}) with contiguous heads on the cache's device")
+    if q.dtype != torch.bfloat16:
+        raise TypeError(f"q must be bfloat16, got {q.dtype}")
+    k, v = cache._ptrs(layer)
+    st = batch._use(stream)
+    if out is None:
+        out = _empty((batch.total_q, nh, hd), out_dtype, cache.device, stream)
+    if batch.total_q == 0:
+        return out
+    _lib.call("m1moe_cuda_paged_attention", batch._cfg, batch._plan, batch._table, q.data_ptr(), q.stride(0), k, v,
+              1.0 / math.sqrt(hd) if scale is None else scale, softcap, out.data_ptr(), dtype_code(out.dtype),
+              out.stride(0), st)
+    return out
+
+
+def rope_table(max_positions: int, rot_dim: int, *, theta: float = 10000.0, scaling: dict | None = None,
+               device=None) -> torch.Tensor:
+    """f32 [max_positions][rot_dim/2][2]: cos and sin of position * theta^(-2i/rot_dim), made in 64 bits.
+
+    scaling, for contexts longer than the model was trained on (original = its trained length):
+      {"type": "linear", "factor": f}  positions divided by f
+      {"type": "ntk", "factor": f}     theta raised so that the slowest pair turns f times slower
+      {"type": "yarn", "factor": f, "original": n, "beta_fast": 32, "beta_slow": 1}
+          pairs that turn more than beta_fast times in n positions stay, those below beta_slow are
+          divided by f, a ramp between; cosines and sines times 0.1 ln f + 1
+    """
+    if rot_dim <= 0 or rot_dim % 2:
+        raise ValueError("rot_dim must be a positive even number")
+    kind = (scaling or {}).get("type")
+    f = float((scaling or {}).get("factor", 1.0))
+    if kind not in (None, "linear", "ntk", "yarn") or f < 1.0:
+        raise ValueError(f"unknown rope scaling {scaling}")
+    i = torch.arange(0, rot_dim, 2, dtype=torch.float64)
+    if kind == "ntk":
+        theta = theta * f ** (rot_dim / max(rot_dim - 2, 1))
+    inv = theta ** (-i / rot_dim)
+    gain = 1.0
+    if kind == "linear":
+        inv = inv / f
+    elif kind == "yarn":
+        n = float(scaling["original"])
+        lo, hi = float(scaling.get("beta_slow", 1.0)), float(scaling.get("beta_fast", 32.0))
+        # linear in the pair's number between the numbers at which it turns hi and lo times
+        at = lambda t: rot_dim * math.log(n / (2 * math.pi * t)) / (2 * math.log(theta))
+        a, b = max(math.floor(at(hi)), 0), min(math.ceil(at(lo)), rot_dim // 2 - 1)
+        ramp = ((i / 2 - a) / max(b - a, 1e-3)).clamp(0, 1)
+        inv = inv * (1 - ramp) + inv / f * ramp
+        gain = 0.1 * math.log(f) + 1.0
+    angle = torch.arange(max_positions, dtype=torch.float64)[:, None] * inv
+    return (torch.stack((angle.cos(), angle.sin()), dim=-1) * gain).float().to(device if device is not None else "cuda")

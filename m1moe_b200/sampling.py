@@ -1,0 +1,48 @@
+"""Token sampling from logits: temperature, top-k, top-p and min-p, one uniform number per row.
+
+Thin wrapper over m1moe_cuda_sample (include/m1moe_cuda.h), which defines the result exactly
+(whole-number weights, ties to the lower index); replaces the CPU sampling of
+InferenceEngine.swift:550-575.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from .expert_ffn import _stream, dtype_code
+from .paged import _empty
+
+
+def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+           out: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+    """int32 tokens [rows] from logits [rows][vocab] (f32 or bf16, rows may lie further apart) and
+    u f32 [rows] in [0, 1).  Each setting is a number or a CUDA tensor [rows] (f32; top_k int32).
+    temperature 0: the largest logit; top_k <= 0, top_p >= 1 and min_p 0 leave that filter off; a
+    row of -inf gives -1."""
+    if logits.dim() != 2 or not logits.is_cuda or (logits.numel() and logits.stride(1) != 1):
+        raise ValueError("logits: a CUDA tensor [rows][vocab] of contiguous rows")
+    rows, vocab = logits.shape
+    dev = logits.device
+    args = []
+    for t, name, dtype in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
+                           (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
+                           (min_p, "min_p", torch.float32)):
+        if isinstance(t, torch.Tensor):
+            if t.device != dev or t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous():
+                raise ValueError(f"{name}: a contiguous {dtype} tensor [{rows}] on {dev}")
+            args.append((t.data_ptr(), 0))
+        elif name == "u":
+            raise ValueError("u is a tensor of one uniform number per row")
+        else:
+            args.append((0, t))
+    st = _stream(stream)
+    if out is None:
+        out = _empty((rows,), torch.int32, dev, stream)
+    elif out.device != dev or out.dtype != torch.int32 or out.shape != (rows,) or not out.is_contiguous():
+        raise ValueError(f"out: a contiguous int32 tensor [{rows}] on {dev}")
+    (pu, _), (pt, vt), (pk, vk), (pp, vp), (pm, vm) = args
+    # one row's stride may be anything; the C side wants at least the row's length
+    stride = logits.stride(0) if rows > 1 else max(logits.stride(0), vocab)
+    _lib.call("m1moe_cuda_sample", logits.data_ptr(), dtype_code(logits.dtype), stride, rows, vocab, pu, pt, vt, pk,
+              vk, pp, vp, pm, vm, out.data_ptr(), st)
+    return out
