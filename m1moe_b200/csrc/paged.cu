@@ -11,6 +11,7 @@
 #include "m1moe_cuda.h"
 #include "paged.cuh"
 #include "paged_rows16.cuh"
+#include "paged_rows256.cuh"
 
 // The error helpers and launch counter of m1moe_cuda.cu (one library).
 namespace m1abi {
@@ -104,10 +105,13 @@ m1moe_status make_shape(const m1moe_paged_cfg *c, int ctas, m1::PagedShape &s) {
     s.max_q = c->max_q;
     s.window = c->window;
     s.ctas = ctas;
-    s.rows = m1::kPagedRowsSmall;
-    s.unit = m1::kPagedUnitSmall;
-    s.workers = ctas * m1::kPagedWarps;
-    s.min_per = m1::kPagedWarps;
+    // 16-row items while a sequence's rows fit one, 256-row ones beyond
+    const bool small = (long long)group * c->max_q <= m1::kPagedRowsSmall;
+    s.rows = small ? m1::kPagedRowsSmall : m1::kPagedRowsLarge;
+    s.unit = small ? m1::kPagedUnitSmall : m1::kPagedUnitLarge;
+    s.workers = small ? ctas * m1::kPagedWarps : ctas;
+    s.min_per = small ? m1::kPagedWarps : 1;
+    s.prefix = small && c->window == 0 ? c->shared_prefix : 0;
     const long long items = c->num_seqs + (long long)c->total_q * group / s.rows;
     const long long cap = (long long)c->max_pages_per_seq * c->page_size;
     if (items * (cap / s.unit + 1) * c->num_kv_heads > 0x7FFFFFFFLL)
@@ -119,16 +123,20 @@ m1moe_status make_shape(const m1moe_paged_cfg *c, int ctas, m1::PagedShape &s) {
 
 size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
 
-// The plan's arrays in its buffer; returns its bytes.
-size_t plan_view(const m1::PagedShape &s, void *base, m1::PagedPlanView &v) {
+// The plan's arrays in its buffer: the main split and, with a shared prefix,
+// the prefix's; returns the buffer's bytes.
+size_t plan_view(const m1::PagedShape &s, void *base, m1::PagedPlanView &v, m1::PagedPlanView &v2,
+                 m1::PagedPrefixView &pre) {
     uint8_t *b = static_cast<uint8_t *>(base);
     size_t at = 0;
     auto take = [&](auto *&ptr, size_t bytes) {
         ptr = reinterpret_cast<std::remove_reference_t<decltype(ptr)>>(b + at);
         at = align256(at + bytes);
     };
-    const size_t part_rows = std::min(s.rows, std::max(1, s.group * s.max_q));
+    const bool large = s.rows == m1::kPagedRowsLarge;
+    const size_t part_rows = large ? s.rows : std::max(1, s.group * s.max_q);
     take(v.header, m1::kPhWords * 4);
+    v.status = v.header + m1::kPhStatus;
     take(v.cu_q, (size_t)(s.num_seqs + 1) * 4);
     take(v.kv_len, (size_t)s.num_seqs * 4);
     take(v.tokens, (size_t)s.total_q * 8);
@@ -136,24 +144,59 @@ size_t plan_view(const m1::PagedShape &s, void *base, m1::PagedPlanView &v) {
     take(v.item_at, (size_t)(s.num_seqs + 1) * 4);
     take(v.unit_at, (size_t)(s.max_items + 1) * 4);
     take(v.start, (size_t)s.workers * 4);
-    take(v.count, (size_t)s.nkv * s.max_items * 4);
+    take(v.count, (size_t)s.nkv * s.max_items * 4 * (large ? 2 : 1));
     take(v.part_ml, (size_t)2 * s.ctas * part_rows * 8);
     take(v.part, (size_t)2 * s.ctas * part_rows * s.hd * 4);
+    v2 = v;
+    if (s.prefix == 0) return at;
+    const size_t items2 = ((size_t)s.total_q * s.group + m1::kPagedRowsLarge - 1) / m1::kPagedRowsLarge;
+    take(v2.header, m1::kPhWords * 4);
+    take(v2.items, items2 * sizeof(m1::PagedItem));
+    take(v2.unit_at, (items2 + 1) * 4);
+    take(v2.start, (size_t)s.ctas * 4);
+    take(v2.count, (size_t)s.nkv * items2 * 2 * 4);
+    take(v2.part_ml, (size_t)2 * s.ctas * m1::kPagedRowsLarge * 8);
+    take(v2.part, (size_t)2 * s.ctas * m1::kPagedRowsLarge * s.hd * 4);
+    take(pre.ml, (size_t)s.total_q * s.nh * 8);
+    take(pre.part, (size_t)s.total_q * s.nh * s.hd * 4);
     return at;
 }
 
-m1moe_status shape_and_plan(const m1moe_paged_cfg *cfg, void *d_plan, m1::PagedShape &s, m1::PagedPlanView &v) {
+struct Plan {
+    m1::PagedShape s;
+    m1::PagedPlanView v, v2;
+    m1::PagedPrefixView pre;
+    size_t bytes;
+};
+
+m1moe_status open_plan(const m1moe_paged_cfg *cfg, void *d_plan, Plan &p) {
     int sms = 0;
     if (sm_count(&sms)) return fail(M1MOE_ERR_CUDA, "no CUDA device");
-    if (m1moe_status st = make_shape(cfg, sms, s)) return st;
-    s.prefix = 0;
+    p = Plan{};
+    if (m1moe_status st = make_shape(cfg, sms, p.s)) return st;
     if (!d_plan || (reinterpret_cast<uintptr_t>(d_plan) & 255))
         return fail(M1MOE_ERR_INVALID_ARG, "the plan buffer is NULL or not 256-byte aligned");
-    plan_view(s, d_plan, v);
+    p.bytes = plan_view(p.s, d_plan, p.v, p.v2, p.pre);
     return M1MOE_OK;
 }
 
 constexpr size_t kRows16SmemCap = 224 * 1024;  // of the CTA's 227 KB; the rest is static
+
+template <int HD>
+m1moe_status launch_rows256(const m1::PagedShape &s, const m1::PagedPlanView &v, const m1::RowsParams &r,
+                            const m1::PagedPrefixView *pre, cudaStream_t st) {
+    m1::Rows256Params a{};
+    a.r = r;
+    if (pre) {
+        a.prefix_run = 1;
+        a.partial = pre->part;
+        a.partial_ml = pre->ml;
+    }
+    auto kern = m1::k_paged_rows256<HD>;
+    constexpr int smem = m1::Rows256<HD>::kSmem;
+    P_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    return launch_pdl(kern, dim3(s.ctas), dim3(m1::kRows256Threads), (size_t)smem, st, "k_paged_rows256 launch", s, v, a);
+}
 
 template <int HD>
 m1moe_status launch_rows16(const m1::PagedShape &s, const m1::PagedPlanView &v, m1::RowsParams a, cudaStream_t st) {
@@ -167,6 +210,18 @@ m1moe_status launch_rows16(const m1::PagedShape &s, const m1::PagedPlanView &v, 
     return launch_pdl(kern, dim3(s.ctas), dim3(m1::kPagedWarps * 32), smem, st, "k_paged_rows16 launch", s, v, a);
 }
 
+template <int HD>
+m1moe_status attention(const Plan &p, m1::RowsParams a, cudaStream_t st) {
+    if (p.s.rows == m1::kPagedRowsLarge) return launch_rows256<HD>(p.s, p.v, a, nullptr, st);
+    if (p.s.prefix > 0) {
+        // one partial per row over the prefix, then the sequences' own parts
+        if (m1moe_status e = launch_rows256<HD>(p.s, p.v2, a, &p.pre, st)) return e;
+        a.prefix_part = p.pre.part;
+        a.prefix_ml = p.pre.ml;
+    }
+    return launch_rows16<HD>(p.s, p.v, a, st);
+}
+
 }  // namespace
 
 extern "C" {
@@ -177,24 +232,22 @@ size_t m1moe_cuda_paged_plan_bytes(const m1moe_paged_cfg *cfg) {
         cudaGetLastError();
         sms = 148;
     }
-    m1::PagedShape s;
-    if (make_shape(cfg, sms, s)) return 0;
-    m1::PagedPlanView v{};
-    return plan_view(s, nullptr, v);
+    Plan p{};
+    if (make_shape(cfg, sms, p.s)) return 0;
+    return plan_view(p.s, nullptr, p.v, p.v2, p.pre);
 }
 
 m1moe_status m1moe_cuda_paged_plan(const m1moe_paged_cfg *cfg, const int32_t *d_cu_q, const int32_t *d_kv_len,
                                    const int32_t *d_page_table, void *d_plan, size_t plan_bytes, void *stream) {
     if (!d_cu_q || !d_kv_len || !d_page_table) return fail(M1MOE_ERR_INVALID_ARG, "NULL pointer");
-    m1::PagedShape s;
-    m1::PagedPlanView v{};
-    if (m1moe_status st = shape_and_plan(cfg, d_plan, s, v)) return st;
-    m1::PagedPlanView none{};
-    const size_t need = plan_view(s, nullptr, none);
-    if (plan_bytes < need)
-        return fail(M1MOE_ERR_INVALID_ARG, "plan buffer: %zu bytes, %zu needed", plan_bytes, need);
+    Plan p;
+    if (m1moe_status st = open_plan(cfg, d_plan, p)) return st;
+    if (plan_bytes < p.bytes)
+        return fail(M1MOE_ERR_INVALID_ARG, "plan buffer: %zu bytes, %zu needed", plan_bytes, p.bytes);
+    const m1::PagedShape &s = p.s;
+    const m1::PagedPlanView &v = p.v;
     if (m1moe_status st = launch_pdl(m1::k_paged_plan, dim3(1), dim3(1024), 0, as_stream(stream), "k_paged_plan launch",
-                                     s, v, (const int *)d_cu_q, (const int *)d_kv_len, (const int *)d_page_table))
+                                     s, v, (const int *)d_cu_q, (const int *)d_kv_len, (const int *)d_page_table, p.v2))
         return st;
     if (s.total_q == 0) return M1MOE_OK;
     return launch_pdl(m1::k_paged_tokens, dim3((s.total_q + 255) / 256), dim3(256), 0, as_stream(stream),
@@ -210,9 +263,10 @@ m1moe_status m1moe_cuda_paged_append(const m1moe_paged_cfg *cfg, const void *d_p
         return fail(M1MOE_ERR_INVALID_ARG, "NULL pointer");
     if (qkv_dtype != M1MOE_DTYPE_F32 && qkv_dtype != M1MOE_DTYPE_BF16)
         return fail(M1MOE_ERR_INVALID_ARG, "dtype must be F32 (0) or BF16 (1)");
-    m1::PagedShape s;
-    m1::PagedPlanView v{};
-    if (m1moe_status st = shape_and_plan(cfg, const_cast<void *>(d_plan), s, v)) return st;
+    Plan p;
+    if (m1moe_status st = open_plan(cfg, const_cast<void *>(d_plan), p)) return st;
+    const m1::PagedShape &s = p.s;
+    const m1::PagedPlanView &v = p.v;
     const int heads = s.nh + 2 * s.nkv;
     const bool bf = qkv_dtype == M1MOE_DTYPE_BF16;
     if (qkv_stride < (int64_t)heads * s.hd || qkv_stride % (bf ? 8 : 4))
@@ -258,9 +312,9 @@ m1moe_status m1moe_cuda_paged_attention(const m1moe_paged_cfg *cfg, void *d_plan
         return fail(M1MOE_ERR_INVALID_ARG, "NULL pointer");
     if (out_dtype != M1MOE_DTYPE_F32 && out_dtype != M1MOE_DTYPE_BF16)
         return fail(M1MOE_ERR_INVALID_ARG, "dtype must be F32 (0) or BF16 (1)");
-    m1::PagedShape s;
-    m1::PagedPlanView v{};
-    if (m1moe_status st = shape_and_plan(cfg, d_plan, s, v)) return st;
+    Plan p;
+    if (m1moe_status st = open_plan(cfg, d_plan, p)) return st;
+    const m1::PagedShape &s = p.s;
     const int64_t width = (int64_t)s.nh * s.hd;
     if (q_stride < width || q_stride % 8 || out_stride < width || out_stride % 8)
         return fail(M1MOE_ERR_INVALID_ARG, "q and out strides: at least %lld, multiples of 8 elements",
@@ -282,7 +336,7 @@ m1moe_status m1moe_cuda_paged_attention(const m1moe_paged_cfg *cfg, void *d_plan
     a.out_bf16 = out_dtype == M1MOE_DTYPE_BF16;
     a.out_stride = out_stride;
     a.part_rows = std::min(s.rows, s.group * s.max_q);
-    return s.hd == 128 ? launch_rows16<128>(s, v, a, as_stream(stream)) : launch_rows16<64>(s, v, a, as_stream(stream));
+    return s.hd == 128 ? attention<128>(p, a, as_stream(stream)) : attention<64>(p, a, as_stream(stream));
 }
 
 m1moe_status m1moe_cuda_paged_status(void *d_plan, void *stream) {

@@ -39,6 +39,8 @@ constexpr int kPagedErrWait = 8;      // a bounded wait gave up
 constexpr int kPagedWarps = 8;      // consumer warps of the 16-row kernel
 constexpr int kPagedRowsSmall = 16; // rows of an item there: one m16n8k16 tile
 constexpr int kPagedUnitSmall = 16; // positions of a unit there
+constexpr int kPagedRowsLarge = 256; // rows of an item of the 256-row kernel: two M-tiles of 128
+constexpr int kPagedUnitLarge = 128; // positions of a unit there: one K or V tile
 
 // Words of the plan's header.
 enum PagedHeader {
@@ -47,8 +49,6 @@ enum PagedHeader {
     kPhUnits = 2,   // units per KV head
     kPhPer = 3,     // units per CTA
     kPhPrefix = 4,  // positions of the shared prefix in use (0: none)
-    kPhPrefixUnits = 5,
-    kPhPrefixPer = 6,
     kPhWords = 16
 };
 
@@ -59,6 +59,7 @@ struct PagedItem {
 };
 
 struct PagedPlanView {
+    int *status;         // the batch's status word (header word 0 of the main split)
     int *header;
     int *cu_q;           // [B + 1]
     int *kv_len;         // [B]
@@ -67,9 +68,16 @@ struct PagedPlanView {
     int *item_at;        // [B + 1]: first item of each sequence
     int *unit_at;        // [max_items + 1]: units before each item
     int *start;          // [workers]: the item each worker starts in
-    int *count;          // [nkv * max_items]: partials that have arrived
+    int *count;          // [nkv * max_items] (two each, 256-row kernel): partials that have arrived
     float *part;         // [2 * ctas][rows][hd] weighted values
     float2 *part_ml;     // [2 * ctas][rows] maximum and sum
+};
+
+// The shared prefix's results, one partial per row, which the 16-row kernel
+// joins to each sequence's own.
+struct PagedPrefixView {
+    float *part;   // [total_q][nh][hd]
+    float2 *ml;    // [total_q][nh]
 };
 
 struct PagedShape {
@@ -140,11 +148,11 @@ __device__ __forceinline__ int upper_index(const int *a, int n, int v) {
 // shorter than its new tokens (an idle slot of a fixed-size batch has none
 // at all): the tokens before position 0 see nothing and are stored nowhere.
 __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const PagedPlanView p, const int *cu_q,
-                                                     const int *kv_len, const int *table) {
+                                                     const int *kv_len, const int *table, const PagedPlanView p2) {
     __shared__ int sm[32];
-    __shared__ int sm_bad, sm_noprefix;
+    __shared__ int sm_bad, sm_noprefix, sm_lead;
     const int tid = threadIdx.x;
-    if (tid == 0) sm_bad = 0, sm_noprefix = 0;
+    if (tid == 0) sm_bad = 0, sm_noprefix = 0, sm_lead = s.num_seqs;
     __syncthreads();
     pdl_wait();
     const int capacity = s.max_pages * s.page_size;
@@ -161,7 +169,11 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
             p.kv_len[b] = t;
             if (b + 1 == s.num_seqs) p.cu_q[b + 1] = q1;
             n = good ? ((q1 - q0) * s.group + s.rows - 1) / s.rows : 0;
-            if (q1 > q0 && t - (q1 - q0) < s.prefix) sm_noprefix = 1;
+            // an idle slot takes no part in the prefix; the others' new tokens follow it
+            if (t > 0) {
+                if (t - (q1 - q0) < s.prefix) sm_noprefix = 1;
+                atomicMin(&sm_lead, b);
+            }
         }
         int total;
         const int at = block_scan_1024(n, sm, total);
@@ -177,16 +189,20 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
             if (b < s.num_seqs) p.kv_len[b] = 0;
         }
     }
-    // the prefix is shared only where every sequence's page table agrees
-    if (s.prefix > 0) {
+    // the prefix is shared only where the page tables agree
+    const int lead = sm_lead;
+    if (s.prefix > 0 && lead < s.num_seqs && !sm_bad) {
         const int np = s.prefix >> s.page_shift;
-        for (int i = tid; i < np * s.num_seqs; i += 1024) {
-            const int b = i / np, j = i - b * np;
-            if (table[(size_t)b * s.max_pages + j] != table[j]) sm_noprefix = 1;
+        for (int b = lead + 1 + (tid >> 5); b < s.num_seqs; b += 32) {
+            if (p.kv_len[b] == 0) continue;
+            bool same = true;
+            for (int j = tid & 31; j < np; j += 32)
+                same = same && table[(size_t)b * s.max_pages + j] == table[(size_t)lead * s.max_pages + j];
+            if (!same) sm_noprefix = 1;
         }
     }
     __syncthreads();
-    const int prefix = sm_noprefix ? 0 : s.prefix;
+    const int prefix = sm_noprefix || sm_bad || lead == s.num_seqs ? 0 : s.prefix;
     int units = 0;
     for (int i0 = 0; i0 < items; i0 += 1024) {
         const int i = i0 + tid;
@@ -214,7 +230,8 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
         units += total;
     }
     if (tid == 0) p.unit_at[items] = units;
-    for (int i = tid; i < items * s.nkv; i += 1024) p.count[i] = 0;
+    const int tiles = s.rows == kPagedRowsLarge ? 2 : 1;
+    for (int i = tid; i < items * s.nkv * tiles; i += 1024) p.count[i] = 0;
     __syncthreads();
     const long long all = (long long)units * s.nkv;
     const int per = (int)max((long long)s.min_per, (all + s.ctas - 1) / s.ctas);
@@ -228,11 +245,31 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
         p.start[w] = u < c1 ? upper_index(p.unit_at, items + 1, (int)(u % units)) : 0;
     }
     if (tid == 0) {
-        p.header[kPhStatus] = sm_bad;
+        *p.status = sm_bad;
         p.header[kPhItems] = items;
         p.header[kPhUnits] = units;
         p.header[kPhPer] = per;
         p.header[kPhPrefix] = prefix;
+    }
+    if (s.prefix == 0) return;
+    // the prefix's own split: all rows of the batch, 256 at a time, against
+    // its positions (no items when it is not shared after all)
+    const int rows = s.total_q * s.group;
+    const int items2 = prefix ? (rows + kPagedRowsLarge - 1) / kPagedRowsLarge : 0;
+    const int n2 = (prefix + kPagedUnitLarge - 1) / kPagedUnitLarge, units2 = items2 * n2;
+    for (int i = tid; i <= items2; i += 1024) {
+        p2.unit_at[i] = i * n2;
+        if (i < items2)
+            p2.items[i] = PagedItem{lead, i * kPagedRowsLarge, min(kPagedRowsLarge, rows - i * kPagedRowsLarge), 0};
+    }
+    for (int i = tid; i < items2 * s.nkv * 2; i += 1024) p2.count[i] = 0;
+    const int all2 = units2 * s.nkv, per2 = max(1, (all2 + s.ctas - 1) / s.ctas);
+    for (int c = tid; c < s.ctas; c += 1024) p2.start[c] = c * per2 < all2 ? (c * per2) % units2 / n2 : 0;
+    if (tid == 0) {
+        p2.header[kPhItems] = items2;
+        p2.header[kPhUnits] = units2;
+        p2.header[kPhPer] = per2;
+        p2.header[kPhPrefix] = prefix;
     }
 }
 
@@ -312,7 +349,7 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedShape s, const 
     const bool in_seq = tok.x >= 0;
     int pos = in_seq ? tok.y : 0;
     if (pos >= a.rope_rows) {
-        if (l == 0) atomicOr(&p.header[kPhStatus], kPagedErrPosition);
+        if (l == 0) atomicOr(p.status, kPagedErrPosition);
         pos = 0;
     }
     const int half = a.rot >> 1;
@@ -376,7 +413,7 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedShape s, const 
             *reinterpret_cast<uint4 *>(a.q_out + ((long long)t * s.nh + h) * HD + 8 * l) = y;
         } else if (in_seq) {
             const int g = is_v ? h - s.nh - s.nkv : h - s.nh;
-            const int row = paged_row(s, a.table, tok.x, g, tok.y, &p.header[kPhStatus]);
+            const int row = paged_row(s, a.table, tok.x, g, tok.y, p.status);
             uint16_t *pool = is_v ? a.v : a.k;
             if (row >= 0) *reinterpret_cast<uint4 *>(pool + (long long)row * HD + 8 * l) = y;
         }

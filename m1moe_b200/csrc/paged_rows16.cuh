@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
     pdl_wait();
     const int units = p.header[kPhUnits], items = p.header[kPhItems], per = p.header[kPhPer];
     const int prefix = p.header[kPhPrefix];
-    int *status = &p.header[kPhStatus];
+    int *status = p.status;
     const int all = units * s.nkv;
     const int c0 = min(cta * per, all), c1 = min(all, c0 + per);
     const int pw = (c1 - c0 + kPagedWarps - 1) / kPagedWarps;
@@ -349,6 +349,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
         // the finished rows of an item, straight from the accumulators
         auto write_rows = [&]() {
             const int q0 = p.cu_q[it.seq];
+            const int pre = p.kv_len[it.seq] > 0 ? prefix : 0;  // an idle slot has none
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int r = lane / 4 + 8 * h;
@@ -357,7 +358,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                 const int token = q0 + tok, head = cur.g * s.group + row - tok * s.group;
                 const long long pr = (long long)token * s.nh + head;
                 float c = 1.f, ci = 0.f, sum = l[h];
-                if (prefix > 0) {
+                if (pre > 0) {
                     const float2 ml = a.prefix_ml[pr];
                     const float mn = fmaxf(m[h], ml.x);
                     c = m[h] == -INFINITY ? 0.f : exp2_approx(m[h] - mn);
@@ -370,7 +371,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                 for (int n = 0; n < NT; ++n) {
                     const int col = 8 * n + 2 * (lane & 3);
                     float x0 = o[n][2 * h] * c, x1 = o[n][2 * h + 1] * c;
-                    if (prefix > 0) {
+                    if (pre > 0) {
                         const float2 y = *reinterpret_cast<const float2 *>(a.prefix_part + pr * HD + col);
                         x0 += y.x * ci, x1 += y.y * ci;
                     }
@@ -491,7 +492,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
     // Every warp takes every eighth row.
     auto join = [&](int w0, bool from_front, int n, bool closed, bool open_left, int g, int item) {
         const PagedItem it = p.items[item];
-        const int q0 = p.cu_q[it.seq];
+        const int q0 = p.cu_q[it.seq], pre = p.kv_len[it.seq] > 0 ? prefix : 0;
         const bool done = closed && !open_left;
         const int slot = 2 * cta + (open_left ? 0 : 1);
         for (int r = warp; r < it.nrows; r += kPagedWarps) {
@@ -508,7 +509,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                 m, l, o);
             const int row = it.row0 + r, tok = row / s.group;
             if (done) {
-                finish_row<HD>(s, a, prefix, q0 + tok, g * s.group + row - tok * s.group, m, l, o);
+                finish_row<HD>(s, a, pre, q0 + tok, g * s.group + row - tok * s.group, m, l, o);
             } else {
                 const size_t at = (size_t)slot * a.part_rows + r;
                 store_vec<HD>(p.part + at * HD + lane * E, o);
@@ -551,7 +552,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
         if (!sm_last) continue;
         __threadfence();
         const PagedItem it = p.items[item];
-        const int q0 = p.cu_q[it.seq];
+        const int q0 = p.cu_q[it.seq], pre = p.kv_len[it.seq] > 0 ? prefix : 0;
         for (int r = warp; r < it.nrows; r += kPagedWarps) {
             float m, l, o[E];
             merge_partials<HD>(
@@ -565,7 +566,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                 },
                 m, l, o);
             const int row = it.row0 + r, tok = row / s.group;
-            finish_row<HD>(s, a, prefix, q0 + tok, g * s.group + row - tok * s.group, m, l, o);
+            finish_row<HD>(s, a, pre, q0 + tok, g * s.group + row - tok * s.group, m, l, o);
         }
     }
 }

@@ -1,0 +1,605 @@
+// paged_rows256.cuh — attention of up to 256 rows (new tokens x heads of one
+// KV head) per item over a paged cache, on the tensor cores: prompts, prompt
+// chunks, mixed batches, and a batch's rows against its shared prefix
+// (sm_100a).
+//
+// The formula of paged_rows16.cuh.  Here the two products and the exponentials
+// bound it: a 128 x 128 tile of scores at hd 128 is 2 x 2.1 M multiply-adds
+// (512 cycles each of a tcgen05 pipe) and 16,384 exponentials (1,024 cycles
+// of an SM's 16 special-function lanes a cycle).
+//
+// One persistent CTA per SM walks its run of 128-position units (paged.cuh).
+// An item's 256 rows are two M-tiles of 128 that share every K and V tile:
+//   warps 0-3, 4-7   softmax of M-tile 0 and 1, a thread per row: scores from
+//                    tensor memory, running maximum and sum, weights back to
+//                    tensor memory as bf16, over the scores they came from
+//   warps 8-11       K and V tiles from the pages into a ring of shared memory
+//   warp 12          issues the products: S = Q K^T (both operands in shared
+//                    memory), O += P V (P from tensor memory, V as it lies:
+//                    MN-major)
+// While one M-tile's warps take exponentials, the tensor cores run the other
+// one's products.  Tensor memory: S0, S1, O0, O1, 128 columns each.
+//
+// The pages are copied with cp.async (16 bytes a lane) rather than TMA boxes:
+// a page may hold 16 rows, 2 KB of a tile, and rows outside the item must be
+// zeros in shared memory (0 * NaN is NaN).  The writing thread's
+// fence.proxy.async makes its copies visible to the tensor cores.
+//
+// A row's accumulator keeps the reference maximum it was started with until
+// the true maximum is more than 2^8 above it in the weights' scale; only then
+// is it rescaled.  Weights are at most 2^8 (bf16 has the same relative error
+// there), sums are fp32.
+#pragma once
+
+#include "paged_rows16.cuh"
+#include "umma.cuh"
+
+namespace m1 {
+
+constexpr int kTileRows = 128;              // an M-tile
+constexpr int kRows256Threads = 13 * 32;
+constexpr int kRows256Loaders = 128;
+constexpr float kRescaleLog2 = 8.f;
+
+template <int HD>
+struct Rows256 {
+    static constexpr int kHalves = HD / 64;                    // 128-byte columns of a tile
+    static constexpr int kTile = 128 * HD * 2;                 // bytes of a Q M-tile, K tile or V tile
+    static constexpr int kStages = HD == 128 ? 5 : 8;
+    static constexpr int kLag = kStages - 2;                   // copy groups a loader keeps in flight
+    static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024;
+};
+
+struct Rows256Params {
+    RowsParams r;
+    int prefix_run;      // this launch is the shared prefix: all rows see [0, prefix)
+    float *partial;      // there: [total_q][nh][hd] weighted values and
+    float2 *partial_ml;  // [total_q][nh] maxima and sums
+};
+
+// Shared-memory descriptor of an MN-major operand, 128-byte swizzle: 64
+// elements of N per 128-byte row, rows along K; 8-row groups 1024 bytes apart
+// (stride byte offset), 64-element column blocks `lead` bytes apart (leading
+// byte offset).
+__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem, uint32_t lead) {
+    return (uint64_t)((smem >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) |
+           ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+}
+
+// Instruction descriptor of kind::f16 with bf16 operands and fp32
+// accumulators; b_mn: B is MN-major.
+__host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N, bool b_mn) {
+    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn ? 1u : 0u) << 16) | ((uint32_t)(N >> 3) << 17) |
+           ((uint32_t)(M >> 4) << 24);
+}
+
+// D[tmem] (+)= A[tmem] . B[smem]: A holds two bf16 of K per 32-bit column.
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                             bool accumulate) {
+    asm volatile(
+        "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d_tmem),
+        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
+          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
+          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
+          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, "
+        "%15, %16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// Bounded wait; once one has given up (the CTA's abort flag), all return false
+// at once and the roles go through the rest of their motions without touching
+// tensor memory or issuing copies, so that every barrier still matches.
+__device__ __forceinline__ bool paged_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
+    for (uint32_t i = 0; i < kWaitLimit; ++i) {
+        if (mbar_try_wait(bar, parity)) return true;
+        if (*abort) return false;
+    }
+    *abort = 1;
+    atomicOr(status, kPagedErrWait);
+    return false;
+}
+
+// One segment of a CTA's run: tiles [ja, jb) of an item, and per M-tile its
+// rows and the tiles [a, b) that any of them sees.
+struct Rows256Segment {
+    int g, item, u0, u1, seg0, seg1;  // its units, the item's units
+    int seq, row0, nrows, q0, len, first;  // first: position of row 0's token
+    int ja, jb, lo;                   // lo: first position any row sees
+    int n[2], a[2], b[2];
+};
+
+// The roles walk the same segments, each on its own.
+struct Rows256Walk {
+    int u, end, g, item, units, items;
+    __device__ __forceinline__ void start(const PagedShape &s, const PagedPlanView &p, int cta) {
+        units = p.header[kPhUnits];
+        items = p.header[kPhItems];
+        const int per = p.header[kPhPer], all = units * s.nkv;
+        u = min(cta * per, all);
+        end = min(all, u + per);
+        g = u < end ? u / units : 0;
+        item = u < end ? p.start[cta] : 0;
+    }
+    __device__ __forceinline__ bool next(const PagedShape &s, const PagedPlanView &p, const Rows256Params &a,
+                                         Rows256Segment &x) {
+        if (u >= end) return false;
+        const PagedItem it = p.items[item];
+        x.g = g;
+        x.item = item;
+        x.seg0 = g * units + p.unit_at[item];
+        x.seg1 = g * units + p.unit_at[item + 1];
+        x.u0 = u;
+        x.u1 = min(end, x.seg1);
+        x.seq = it.seq;
+        x.row0 = it.row0;
+        x.nrows = it.nrows;
+        x.ja = it.unit0 + u - x.seg0;
+        x.jb = it.unit0 + x.u1 - x.seg0;
+        if (a.prefix_run) {
+            x.q0 = 0;
+            x.len = p.header[kPhPrefix];
+            x.first = 0;
+            x.lo = 0;
+        } else {
+            x.q0 = p.cu_q[it.seq];
+            x.len = p.kv_len[it.seq];
+            x.first = x.len - (p.cu_q[it.seq + 1] - x.q0);
+            x.lo = s.window > 0 ? max(0, x.first + it.row0 / s.group - s.window + 1) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            x.n[i] = min(kTileRows, max(0, it.nrows - i * kTileRows));
+            x.a[i] = x.b[i] = x.ja;
+            if (x.n[i] > 0) {
+                const int r = it.row0 + i * kTileRows;
+                const int hi0 = a.prefix_run ? x.len - 1 : x.first + r / s.group;
+                const int hi1 = a.prefix_run ? x.len - 1 : x.first + (r + x.n[i] - 1) / s.group;
+                const int lo = s.window > 0 && !a.prefix_run ? max(0, hi0 - s.window + 1) : 0;
+                x.a[i] = max(x.ja, lo / kPagedUnitLarge);
+                x.b[i] = max(x.a[i], min(x.jb, hi1 < 0 ? 0 : hi1 / kPagedUnitLarge + 1));
+            }
+        }
+        u = x.u1;
+        if (u == x.seg1 && ++item == items) item = 0, ++g;
+        return true;
+    }
+};
+
+template <int HD>
+__global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const PagedShape s, const PagedPlanView p,
+                                                                      const Rows256Params a) {
+    using T = Rows256<HD>;
+    extern __shared__ uint8_t raw[];
+    __shared__ uint64_t kv_full[T::kStages], kv_empty[T::kStages], q_full[2], s_full[2], p_full[2], o_done[2], drain;
+    __shared__ uint32_t tmem_base;
+    __shared__ int abort_flag, sm_last[2];
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
+    uint8_t *sq = smem, *skv = smem + 2 * T::kTile;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    int *status = p.status;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < T::kStages; ++i) {
+            mbar_init(&kv_full[i], kRows256Loaders);
+            mbar_init(&kv_empty[i], 1);
+        }
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&q_full[i], kTileRows);
+            mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], kTileRows);
+            mbar_init(&o_done[i], 1);
+        }
+        mbar_init(&drain, 1);
+        mbar_fence_init();
+        abort_flag = 0;
+    }
+    if (warp == 12) {
+        tmem_alloc(&tmem_base, 512);
+        tmem_relinquish();
+        tc_fence_before_sync();
+    }
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = tmem_base;
+    pdl_wait();
+    Rows256Walk walk;
+    walk.start(s, p, blockIdx.x);
+    Rows256Segment x;
+
+    if (warp >= 8 && warp < 12) {
+        // ------------------------------------------------------ K and V tiles
+        const int t = threadIdx.x - 256;
+        constexpr int kChunks = HD / 8;                    // 16-byte chunks per row
+        constexpr int kRowsAtOnce = kRows256Loaders / kChunks;
+        const int c = t % kChunks, r0 = t / kChunks;
+        const uint32_t kv_addr = smem_addr(skv);
+        int tile = 0;    // K and V tiles so far, K first
+        auto signal = [&](int n) {  // the copies of tile n have landed
+            fence_proxy_async_smem();
+            mbar_arrive(&kv_full[n % T::kStages]);
+        };
+        auto signal_lagged = [&]() {
+            if (tile > T::kLag) {
+                asm volatile("cp.async.wait_group %0;" ::"n"(T::kLag) : "memory");
+                signal(tile - 1 - T::kLag);
+            }
+        };
+        bool ok = true;
+        while (walk.next(s, p, a, x)) {
+            for (int j = x.ja; j < x.jb; ++j) {
+                const int pos0 = j * kPagedUnitLarge;
+                // lane l looks up the page of positions 8 l .. 8 l + 7
+                int mine = -1;
+                if (lane < 16 && pos0 + 8 * lane < x.len && pos0 + 8 * lane + 7 >= x.lo)
+                    mine = paged_row(s, a.r.table, x.seq, x.g, pos0 + 8 * lane, status);
+                for (int kv = 0; kv < 2; ++kv) {
+                    const int st = tile % T::kStages;
+                    if (ok && tile >= T::kStages)
+                        ok = paged_wait(&kv_empty[st], ((tile / T::kStages) - 1) & 1, &abort_flag, status);
+                    ok = __all_sync(0xffffffffu, ok);
+                    const uint16_t *pool = kv ? a.r.v : a.r.k;
+                    const uint32_t base = kv_addr + st * T::kTile + (c >> 3) * 16384;
+#pragma unroll
+                    for (int i = 0; i < 128 / kRowsAtOnce; ++i) {
+                        const int r = r0 + i * kRowsAtOnce;
+                        const int row = __shfl_sync(0xffffffffu, mine, r >> 3);
+                        const bool in = row >= 0 && pos0 + r < x.len && pos0 + r >= x.lo;
+                        const long long src = in ? ((long long)row + (r & 7)) * HD + c * 8 : 0;
+                        if (ok) cp_async16(base + sw128_offset(r, c & 7), pool + src, in);
+                    }
+                    cp_async_commit();
+                    ++tile;
+                    signal_lagged();
+                }
+            }
+        }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        for (int n = max(0, tile - T::kLag); n < tile; ++n) signal(n);
+    } else if (warp == 12) {
+        // ---------------------------------------------------------- products
+        if (lane == 0) {
+            constexpr uint32_t kIdQK = umma_idesc_bf16(128, 128, false), kIdPV = umma_idesc_bf16(128, HD, true);
+            int tile = 0;
+            int nq[2] = {0, 0}, np[2] = {0, 0};
+            bool ok = true;
+            auto wait = [&](uint64_t *bar, int n) {
+                if (ok) ok = paged_wait(bar, n & 1, &abort_flag, status);
+                tc_fence_after_sync();
+            };
+            auto wait_kv = [&](int n) { wait(&kv_full[n % T::kStages], n / T::kStages); };
+            auto qk = [&](int i, int n) {  // S_i = Q_i K^T with K in tile n
+                const uint32_t qa = smem_addr(sq + i * T::kTile), ka = smem_addr(skv + (n % T::kStages) * T::kTile);
+                if (ok) {
+#pragma unroll
+                    for (int k = 0; k < HD / 16; ++k) {
+                        const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
+                        umma_f16(tmem + i * 128, umma_desc_sw128(qa + off), umma_desc_sw128(ka + off), kIdQK, k > 0);
+                    }
+                    umma_commit(&s_full[i]);
+                }
+            };
+            auto pv = [&](int i, int n, bool first) {  // O_i += P_i V with V in tile n
+                const uint32_t va = smem_addr(skv + (n % T::kStages) * T::kTile);
+                if (ok) {
+#pragma unroll
+                    for (int k = 0; k < 8; ++k)
+                        umma_bf16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k,
+                                     umma_desc_mn_sw128(va + k * 2048, 16384), kIdPV, !(first && k == 0));
+                    umma_commit(&o_done[i]);
+                }
+            };
+            auto release = [&](int n) {
+                if (ok) umma_commit(&kv_empty[n % T::kStages]);
+            };
+            while (walk.next(s, p, a, x)) {
+                const int t0 = tile;  // K of tile j is t0 + 2 (j - ja), V the next
+                for (int i = 0; i < 2; ++i)
+                    if (x.b[i] > x.a[i]) wait(&q_full[i], nq[i]++);
+                wait_kv(t0);
+                for (int i = 0; i < 2; ++i)
+                    if (x.a[i] <= x.ja && x.ja < x.b[i]) qk(i, t0);
+                release(t0);
+                for (int j = x.ja; j < x.jb; ++j) {
+                    const int tk = t0 + 2 * (j - x.ja), tv = tk + 1, tn = tk + 2;
+                    bool have_v = false, have_k = false;
+                    for (int i = 0; i < 2; ++i) {
+                        if (x.a[i] <= j && j < x.b[i]) {
+                            wait(&p_full[i], np[i]++);
+                            if (!have_v) wait_kv(tv), have_v = true;
+                            pv(i, tv, j == x.a[i]);
+                        }
+                        if (j + 1 < x.jb && x.a[i] <= j + 1 && j + 1 < x.b[i]) {
+                            if (!have_k) wait_kv(tn), have_k = true;
+                            qk(i, tn);
+                        }
+                    }
+                    if (!have_v) wait_kv(tv);
+                    release(tv);
+                    if (j + 1 < x.jb) {
+                        if (!have_k) wait_kv(tn);
+                        release(tn);
+                    }
+                }
+                tile = t0 + 2 * (x.jb - x.ja);
+            }
+            // every product has ended before tensor memory is given back
+            umma_commit(&drain);
+            for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(&drain, 0); ++i) {
+            }
+        }
+    } else {
+        // ----------------------------------------------------------- softmax
+        const int i = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const uint32_t ts = tmem + i * 128 + lanes, to = tmem + 256 + i * 128 + lanes;
+        const bool capped = a.r.cap > 0.f;
+        const float mult = capped ? 1.f : a.r.scale * kLog2e;
+        const float c2 = capped ? 2.f * a.r.scale / a.r.cap * kLog2e : 0.f;
+        int ns = 0;  // score tiles so far
+        bool ok = true;
+        while (walk.next(s, p, a, x)) {
+            const int n = x.n[i];
+            const int r = x.row0 + i * kTileRows + row, tok = r / s.group;  // packed row and its token
+            const int head = x.g * s.group + r - tok * s.group;
+            const bool live = row < n;
+            const int hi = a.prefix_run ? x.len - 1 : x.first + tok;
+            const int lo = s.window > 0 && !a.prefix_run ? hi - s.window + 1 : 0;
+            // limits that hold for the M-tile's every row
+            const int rf = x.row0 + i * kTileRows;
+            const int min_hi = a.prefix_run ? x.len - 1 : x.first + rf / s.group;
+            const int max_lo = s.window > 0 && !a.prefix_run ? x.first + (rf + max(n, 1) - 1) / s.group - s.window + 1 : 0;
+            float m = -INFINITY, l = 0.f;  // the reference maximum (raw scale) and the sum
+            const bool active = x.b[i] > x.a[i];
+            if (active) {
+                // this row of Q, zeros past the item's rows
+                const uint16_t *src = a.r.q + (long long)(x.q0 + tok) * a.r.q_stride + (long long)head * HD;
+                uint8_t *dst = sq + i * T::kTile;
+#pragma unroll
+                for (int c = 0; c < HD / 8; ++c) {
+                    const uint4 v = live ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
+                    *reinterpret_cast<uint4 *>(dst + (c >> 3) * 16384 + sw128_offset(row, c & 7)) = v;
+                }
+                fence_proxy_async_smem();
+                mbar_arrive(&q_full[i]);
+            }
+            for (int j = x.a[i]; j < x.b[i]; ++j) {
+                if (ok) ok = paged_wait(&s_full[i], ns & 1, &abort_flag, status);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok) {
+                    tc_fence_after_sync();
+                    const int pos0 = j * kPagedUnitLarge;
+                    const bool masked = pos0 < max_lo || pos0 + kPagedUnitLarge - 1 > min_hi;
+                    float mx = -INFINITY;
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t v[32];
+                        tmem_ld32(ts + 32 * q, v);
+                        tmem_wait_ld();
+                        if (capped) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e)
+                                v[e] = __float_as_uint(score_log2(__uint_as_float(v[e]), 0.f, a.r.cap, c2));
+                        }
+                        if (masked) {
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) {
+                                const int at = pos0 + 32 * q + e;
+                                if (at > hi || at < lo) v[e] = 0xFF800000u;  // -inf
+                            }
+                        }
+                        if (capped || masked) tmem_st32(ts + 32 * q, v);
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(v[e]));
+                    }
+                    if (capped || masked) tmem_wait_st();
+                    bool grow = false;
+                    float f = 1.f;
+                    if (m == -INFINITY) {
+                        m = mx;
+                    } else if ((mx - m) * mult > kRescaleLog2) {
+                        grow = true;
+                        f = exp2_approx((m - mx) * mult);
+                        m = mx;
+                        l *= f;
+                    }
+                    // j > a: the products of the tiles before are in O
+                    if (__any_sync(0xffffffffu, grow) && j > x.a[i]) {
+                        if (ok) ok = paged_wait(&o_done[i], (ns - 1) & 1, &abort_flag, status);
+                        ok = __all_sync(0xffffffffu, ok);
+                        if (ok) {
+                            tc_fence_after_sync();
+#pragma unroll
+                            for (int q = 0; q < HD / 32; ++q) {
+                                uint32_t v[32];
+                                tmem_ld32(to + 32 * q, v);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
+                                tmem_st32(to + 32 * q, v);
+                            }
+                            tmem_wait_st();
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.f : m * mult;
+                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        uint32_t v[32], w[16];
+                        tmem_ld32(ts + 32 * q, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
+                            const float x0 = exp2_approx(fmaf(__uint_as_float(v[e]), mult, -ref));
+                            const float x1 = exp2_approx(fmaf(__uint_as_float(v[e + 1]), mult, -ref));
+                            l4[(e >> 1) & 3] += x0 + x1;
+                            w[e >> 1] = pack_bf16(x0, x1);
+                        }
+                        tmem_st16(ts + 16 * q, w);  // over scores already read
+                    }
+                    l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                    tmem_wait_st();
+                    tc_fence_before_sync();
+                }
+                mbar_arrive(&p_full[i]);
+                ++ns;
+            }
+            // ------------------------------------------------ the segment's end
+            if (active) {
+                if (ok) ok = paged_wait(&o_done[i], (ns - 1) & 1, &abort_flag, status);
+                ok = __all_sync(0xffffffffu, ok);
+                if (ok) tc_fence_after_sync();
+            }
+            const bool has_o = active && ok;
+            const bool whole = x.u0 == x.seg0 && x.u1 == x.seg1;
+            const long long token = x.q0 + tok;
+            auto write_row = [&](float inv, int q, const float (&o)[32]) {  // 32 columns of the row
+                if (a.prefix_run) {
+                    float *d = a.partial + (token * s.nh + head) * HD + 32 * q;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4 *>(d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+                } else if (a.r.out_bf16) {
+                    uint16_t *d = reinterpret_cast<uint16_t *>(a.r.out) + token * a.r.out_stride + (long long)head * HD + 32 * q;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+                        *reinterpret_cast<uint4 *>(d + e) =
+                            make_uint4(pack_bf16(o[e] * inv, o[e + 1] * inv), pack_bf16(o[e + 2] * inv, o[e + 3] * inv),
+                                       pack_bf16(o[e + 4] * inv, o[e + 5] * inv), pack_bf16(o[e + 6] * inv, o[e + 7] * inv));
+                } else {
+                    float *d = reinterpret_cast<float *>(a.r.out) + token * a.r.out_stride + (long long)head * HD + 32 * q;
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4)
+                        *reinterpret_cast<float4 *>(d + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+                }
+            };
+            // partials: [slot][M-tile][hd / 4][row] float4, so that a warp's rows are one run
+            auto part_at = [&](int slot) {
+                return reinterpret_cast<float4 *>(p.part) + ((size_t)slot * 2 + i) * (HD / 4) * kTileRows + row;
+            };
+            auto part_ml_at = [&](int slot) { return p.part_ml + ((size_t)slot * 2 + i) * kTileRows + row; };
+            const int slot = 2 * blockIdx.x + (x.u0 == x.seg0 ? 1 : 0);
+            const float ml_m = m == -INFINITY ? m : m * mult;  // log2 scale
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (n > 0) {
+#pragma unroll
+                for (int q = 0; q < HD / 32; ++q) {
+                    float o[32];
+                    if (has_o) {
+                        uint32_t v[32];
+                        tmem_ld32(to + 32 * q, v);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(v[e]);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                    }
+                    if (live) {
+                        if (whole) {
+                            write_row(inv, q, o);
+                        } else if (active) {
+                            float4 *d = part_at(slot) + 8 * q * kTileRows;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e)
+                                d[e * kTileRows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                        }
+                    }
+                }
+                if (has_o) tc_fence_before_sync();
+                if (live) {
+                    if (!whole)
+                        *part_ml_at(slot) = make_float2(active ? ml_m : -INFINITY, l);
+                    else if (a.prefix_run)
+                        a.partial_ml[token * s.nh + head] = make_float2(ml_m, l);
+                }
+            }
+            if (!whole) {
+                // the last M-tile of the item to finish joins its partials, in position order
+                const int per = p.header[kPhPer];
+                const int first = x.seg0 / per, last = (x.seg1 - 1) / per;
+                __threadfence();
+                named_sync(1 + i, kTileRows);
+                if (row == 0) {
+                    int *cnt = p.count + ((size_t)x.g * walk.items + x.item) * 2 + i;
+                    sm_last[i] = atomicAdd(cnt, 1) == last - first;
+                    if (sm_last[i]) *cnt = 0;  // ready for the next call
+                }
+                named_sync(1 + i, kTileRows);
+                if (sm_last[i]) {
+                    __threadfence();
+                    if (live) {
+                        auto slot_of = [&](int c) { return 2 * c + (c == first ? 1 : 0); };
+                        float mm = -INFINITY, ll = 0.f;
+                        for (int c = first; c <= last; ++c) {
+                            const float2 v = __ldcg(part_ml_at(slot_of(c)));
+                            const float mn = fmaxf(mm, v.x);
+                            if (mn != -INFINITY) ll = ll * exp2_approx(mm - mn) + v.y * exp2_approx(v.x - mn);
+                            mm = mn;
+                        }
+                        const float iv = ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll 1
+                        for (int q = 0; q < HD / 32; ++q) {
+                            float o[32];
+#pragma unroll
+                            for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                            for (int c = first; c <= last; ++c) {
+                                const float2 v = __ldcg(part_ml_at(slot_of(c)));
+                                if (v.x == -INFINITY) continue;
+                                const float w = exp2_approx(v.x - mm);
+                                const float4 *d = part_at(slot_of(c)) + 8 * q * kTileRows;
+#pragma unroll
+                                for (int e = 0; e < 8; ++e) {
+                                    const float4 y = __ldcg(d + e * kTileRows);
+                                    o[4 * e] = fmaf(y.x, w, o[4 * e]);
+                                    o[4 * e + 1] = fmaf(y.y, w, o[4 * e + 1]);
+                                    o[4 * e + 2] = fmaf(y.z, w, o[4 * e + 2]);
+                                    o[4 * e + 3] = fmaf(y.w, w, o[4 * e + 3]);
+                                }
+                            }
+                            write_row(iv, q, o);
+                        }
+                        if (a.prefix_run) a.partial_ml[token * s.nh + head] = make_float2(mm, ll);
+                    }
+                }
+            }
+        }
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == 12) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace m1

@@ -427,3 +427,46 @@ def test_refusals():
         paged_append(cache, 0, batch, qkv, rope=rope_table(64, 24))
     with pytest.raises(ValueError):
         paged_append(cache, 0, batch, qkv, rope=rope, q_norm=torch.ones(hd, device="cuda"))
+
+
+# ----------------------------------------------------------- shared prefix --
+@pytest.mark.parametrize("nh,nkv,hd,page,share,q_lens,kv_lens,cap", [
+    (16, 16, 128, 16, 16, [1, 1], [17, 40], 0.0),
+    (16, 16, 128, 16, 208, [1] * 5, [209, 220, 300, 224, 209], 0.0),
+    (32, 8, 128, 64, 1024, [1] * 70, [1025 + 7 * i for i in range(70)], 0.0),
+    (32, 8, 64, 32, 4000, [1] * 33, [4001 + i for i in range(33)], 30.0),
+    (16, 1, 128, 128, 256, [1] * 40, [257 + 3 * i for i in range(40)], 0.0),
+    (24, 8, 64, 16, 640, [1, 3, 2, 1], [641, 643, 900, 700], 0.0),
+    (32, 8, 128, 16, 512, [1, 1, 1, 1, 1], [0, 600, 513, 0, 530], 0.0),  # idle slots, the first among them
+    (16, 1, 64, 16, 1600, [1], [2000], 0.0),
+])
+def test_shared_prefix_vs_formula(nh, nkv, hd, page, share, q_lens, kv_lens, cap):
+    cache, table, dense = make(nkv, hd, page, q_lens, kv_lens, seed=21, share=share)
+    g = torch.Generator(device="cuda").manual_seed(22)
+    q = (1.5 * torch.randn((sum(q_lens), nh, hd), generator=g, device="cuda")).bfloat16()
+    batch = PagedBatch(cache, q_lens, kv_lens, table, num_heads=nh, shared_prefix=share)
+    ref, mag = attention_ref(q, dense, q_lens, kv_lens, nkv, hd ** -0.5, 0, cap)
+    for dt in (torch.bfloat16, torch.float32):
+        out = paged_attention(cache, 0, batch, q, softcap=cap, out_dtype=dt)
+        batch.check()
+        check_attention(out, ref, mag)
+        assert torch.equal(out, paged_attention(cache, 0, batch, q, softcap=cap, out_dtype=dt))
+
+
+@pytest.mark.parametrize("why", ["tables differ", "a sequence ends inside it", "windowed", "long new tokens"])
+def test_a_prefix_that_cannot_be_shared_changes_nothing(why):
+    nh, nkv, hd, page, share = 16, 4, 128, 16, 64
+    q_lens, kv_lens, window = [1, 1, 1], [100, 90, 300], 0
+    if why == "a sequence ends inside it":
+        kv_lens = [100, 64, 300]
+    if why == "windowed":
+        window = 50
+    if why == "long new tokens":
+        q_lens = [1, 26, 200]
+    cache, table, dense = make(nkv, hd, page, q_lens, kv_lens, seed=23, share=0 if why == "tables differ" else share)
+    q = torch.randn((sum(q_lens), nh, hd), device="cuda").bfloat16()
+    batch = PagedBatch(cache, q_lens, kv_lens, table, num_heads=nh, shared_prefix=share, window=window)
+    out = paged_attention(cache, 0, batch, q)
+    batch.check()
+    ref, mag = attention_ref(q, dense, q_lens, kv_lens, nkv, hd ** -0.5, window)
+    check_attention(out, ref, mag)
