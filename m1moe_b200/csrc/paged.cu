@@ -2,6 +2,7 @@
 // m1moe_cuda_paged_*): the batch plan, the append of new tokens and the
 // attention over the pages.  Stateless: the caller owns the pools, the page
 // table and the plan buffer.
+#include <cuda.h>
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -182,6 +183,32 @@ m1moe_status open_plan(const m1moe_paged_cfg *cfg, void *d_plan, Plan &p) {
 
 constexpr size_t kRows16SmemCap = 224 * 1024;  // of the CTA's 227 KB; the rest is static
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_t, void *, const cuuint64_t *,
+                                   const cuuint64_t *, const cuuint32_t *, const cuuint32_t *, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+
+// A pool as rows of hd elements; a box is 64 columns of a page's rows (128 at
+// most), 128-byte swizzled.
+m1moe_status pool_map(const m1::PagedShape &s, const uint16_t *pool, CUtensorMap *map) {
+    static EncodeTiledFn encode = nullptr;  // one address for the process
+    if (!encode) {
+        void *fn = nullptr;
+        cudaDriverEntryPointQueryResult q{};
+        P_CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
+        if (!fn || q != cudaDriverEntryPointSuccess)
+            return fail(M1MOE_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
+        encode = reinterpret_cast<EncodeTiledFn>(fn);
+    }
+    const cuuint64_t dims[2] = {(cuuint64_t)s.hd, (cuuint64_t)s.num_pages * s.nkv * s.page_size};
+    const cuuint64_t strides[1] = {(cuuint64_t)s.hd * 2};
+    const cuuint32_t box[2] = {64, (cuuint32_t)std::min(s.page_size, m1::kPagedUnitLarge)}, one[2] = {1, 1};
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<uint16_t *>(pool), dims, strides, box,
+                              one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(M1MOE_ERR_CUDA, "page pool tensor map: error %d", (int)r);
+    return M1MOE_OK;
+}
+
 template <int HD>
 m1moe_status launch_rows256(const m1::PagedShape &s, const m1::PagedPlanView &v, const m1::RowsParams &r,
                             const m1::PagedPrefixView *pre, cudaStream_t st) {
@@ -192,10 +219,14 @@ m1moe_status launch_rows256(const m1::PagedShape &s, const m1::PagedPlanView &v,
         a.partial = pre->part;
         a.partial_ml = pre->ml;
     }
+    CUtensorMap kmap, vmap;
+    if (m1moe_status e = pool_map(s, r.k, &kmap)) return e;
+    if (m1moe_status e = pool_map(s, r.v, &vmap)) return e;
     auto kern = m1::k_paged_rows256<HD>;
     constexpr int smem = m1::Rows256<HD>::kSmem;
     P_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    return launch_pdl(kern, dim3(s.ctas), dim3(m1::kRows256Threads), (size_t)smem, st, "k_paged_rows256 launch", s, v, a);
+    return launch_pdl(kern, dim3(s.ctas), dim3(m1::kRows256Threads), (size_t)smem, st, "k_paged_rows256 launch", s, v, a,
+                      kmap, vmap);
 }
 
 template <int HD>

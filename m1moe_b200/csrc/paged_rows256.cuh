@@ -14,16 +14,18 @@
 //                    tensor memory, running maximum and sum, weights back to
 //                    tensor memory as bf16, over the scores they came from
 //   warps 8-11       K and V tiles from the pages into a ring of shared memory
-//   warp 12          issues the products: S = Q K^T (both operands in shared
+//   warps 12-15      warp 12 issues the products: S = Q K^T (both operands in shared
 //                    memory), O += P V (P from tensor memory, V as it lies:
 //                    MN-major)
 // While one M-tile's warps take exponentials, the tensor cores run the other
 // one's products.  Tensor memory: S0, S1, O0, O1, 128 columns each.
 //
-// The pages are copied with cp.async (16 bytes a lane) rather than TMA boxes:
-// a page may hold 16 rows, 2 KB of a tile, and rows outside the item must be
-// zeros in shared memory (0 * NaN is NaN).  The writing thread's
-// fence.proxy.async makes its copies visible to the tensor cores.
+// A tile whose 128 positions all belong to the item comes by TMA, one box per
+// page (or 128 rows of one) and 64 columns.  A tile at an item's edge is
+// copied with cp.async, 16 bytes a lane, with zeros in the rows outside: what
+// lies in a page's unused rows may be anything, and 0 * NaN is NaN.  The
+// writing thread's fence.proxy.async makes those copies visible to the tensor
+// cores.
 //
 // A row's accumulator keeps the reference maximum it was started with until
 // the true maximum is more than 2^8 above it in the weights' scale; only then
@@ -37,16 +39,20 @@
 namespace m1 {
 
 constexpr int kTileRows = 128;              // an M-tile
-constexpr int kRows256Threads = 13 * 32;
+constexpr int kRows256Threads = 16 * 32;
 constexpr int kRows256Loaders = 128;
 constexpr float kRescaleLog2 = 8.f;
+// Registers a thread: the block is launched with 128 each (65,536 / 512); the
+// loader and product warpgroups give theirs up to the two softmax ones, which
+// hold a row of 128 scores: 2 * 200 + 2 * 56 = 4 * 128.
+constexpr int kRegsSoftmax = 200, kRegsOther = 56;
+static_assert(2 * kRegsSoftmax + 2 * kRegsOther <= 4 * 128, "the split must fit the launch's registers");
 
 template <int HD>
 struct Rows256 {
     static constexpr int kHalves = HD / 64;                    // 128-byte columns of a tile
     static constexpr int kTile = 128 * HD * 2;                 // bytes of a Q M-tile, K tile or V tile
     static constexpr int kStages = HD == 128 ? 5 : 8;
-    static constexpr int kLag = kStages - 2;                   // copy groups a loader keeps in flight
     static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024;
 };
 
@@ -57,13 +63,35 @@ struct Rows256Params {
     float2 *partial_ml;  // [total_q][nh] maxima and sums
 };
 
-// Shared-memory descriptor of an MN-major operand, 128-byte swizzle: 64
-// elements of N per 128-byte row, rows along K; 8-row groups 1024 bytes apart
-// (stride byte offset), 64-element column blocks `lead` bytes apart (leading
-// byte offset).
-__device__ __forceinline__ uint64_t umma_desc_mn_sw128(uint32_t smem, uint32_t lead) {
-    return (uint64_t)((smem >> 4) & 0x3FFFu) | ((uint64_t)((lead >> 4) & 0x3FFFu) << 16) |
-           ((uint64_t)(1024u >> 4) << 32) | ((uint64_t)1u << 46) | ((uint64_t)2u << 61);
+// Shared-memory descriptors, 128-byte swizzle, as two words: the high one
+// (stride byte offset 1024 between 8-row groups, version 1, layout type 2) is
+// the same for all operands here, the low one names the start address and
+// the leading byte offset (bits 16-29).  K-major operands do not use that
+// offset.  An MN-major one (V as it lies: rows along K, 64 elements of N per
+// 128-byte row) has its 64-element column blocks `lead` bytes apart.
+constexpr uint32_t kUmmaDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+__device__ __forceinline__ uint32_t umma_desc_lo(uint32_t smem, uint32_t lead) {
+    return ((smem >> 4) & 0x3FFFu) | ((lead >> 4) << 16);
+}
+
+// The value of lane 0, known to the compiler to be the same in every lane.
+__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
+
+// True in one lane of the warp.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{ .reg .pred p; elect.sync _|p, 0xFFFFFFFF; selp.u32 %0, 1, 0, p; }" : "=r"(r));
+    return r != 0;
+}
+
+// 2-D tiled load of the map's box at element coordinates (x, y); completes the
+// box's bytes on `bar`.
+__device__ __forceinline__ void tma_load_2d(void *dst, const CUtensorMap *map, int x, int y, uint64_t *bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_addr(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(smem_addr(bar))
+        : "memory");
 }
 
 // Instruction descriptor of kind::f16 with bf16 operands and fp32
@@ -73,13 +101,23 @@ __host__ __device__ constexpr uint32_t umma_idesc_bf16(int M, int N, bool b_mn) 
            ((uint32_t)(M >> 4) << 24);
 }
 
-// D[tmem] (+)= A[tmem] . B[smem]: A holds two bf16 of K per 32-bit column.
-__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+// D[tmem] (+)= A[smem] . B[smem]^T, operands by their descriptors' low words.
+__device__ __forceinline__ void umma_bf16_ss(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,
                                              bool accumulate) {
     asm volatile(
-        "{ .reg .pred p; setp.ne.b32 p, %4, 0; "
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p; }" ::"r"(d_tmem),
-        "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"((uint32_t)accumulate)
+        "{ .reg .pred p; .reg .b64 da, db; setp.ne.b32 p, %4, 0; mov.b64 da, {%1, %5}; mov.b64 db, {%2, %5}; "
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %3, p; }" ::"r"(d_tmem),
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"((uint32_t)accumulate), "r"(kUmmaDescHi)
+        : "memory");
+}
+
+// D[tmem] (+)= A[tmem] . B[smem]: A holds two bf16 of K per 32-bit column.
+__device__ __forceinline__ void umma_bf16_ts(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t idesc,
+                                             bool accumulate) {
+    asm volatile(
+        "{ .reg .pred p; .reg .b64 db; setp.ne.b32 p, %4, 0; mov.b64 db, {%2, %5}; "
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p; }" ::"r"(d_tmem),
+        "r"(a_tmem), "r"(b_lo), "r"(idesc), "r"((uint32_t)accumulate), "r"(kUmmaDescHi)
         : "memory");
 }
 
@@ -114,6 +152,17 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
         : "memory");
 }
+
+template <int N>
+__device__ __forceinline__ void regs_more() {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N));
+}
+template <int N>
+__device__ __forceinline__ void regs_less() {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -198,7 +247,9 @@ struct Rows256Walk {
 
 template <int HD>
 __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const PagedShape s, const PagedPlanView p,
-                                                                      const Rows256Params a) {
+                                                                      const Rows256Params a,
+                                                                      const __grid_constant__ CUtensorMap kmap,
+                                                                      const __grid_constant__ CUtensorMap vmap) {
     using T = Rows256<HD>;
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t kv_full[T::kStages], kv_empty[T::kStages], q_full[2], s_full[2], p_full[2], o_done[2], drain;
@@ -238,104 +289,142 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
 
     if (warp >= 8 && warp < 12) {
         // ------------------------------------------------------ K and V tiles
+        regs_less<kRegsOther>();
         const int t = threadIdx.x - 256;
         constexpr int kChunks = HD / 8;                    // 16-byte chunks per row
         constexpr int kRowsAtOnce = kRows256Loaders / kChunks;
         const int c = t % kChunks, r0 = t / kChunks;
         const uint32_t kv_addr = smem_addr(skv);
-        int tile = 0;    // K and V tiles so far, K first
-        auto signal = [&](int n) {  // the copies of tile n have landed
-            fence_proxy_async_smem();
-            mbar_arrive(&kv_full[n % T::kStages]);
-        };
-        auto signal_lagged = [&]() {
-            if (tile > T::kLag) {
-                asm volatile("cp.async.wait_group %0;" ::"n"(T::kLag) : "memory");
-                signal(tile - 1 - T::kLag);
-            }
-        };
+        const int box_shift = min(s.page_shift, 7), boxes = 128 >> box_shift;  // rows of a box, boxes along a tile
+        int tile = 0;  // K and V tiles so far, K first
         bool ok = true;
+        auto claim = [&]() {  // the next tile's stage, free
+            const int st = tile % T::kStages;
+            if (ok && tile >= T::kStages)
+                ok = paged_wait(&kv_empty[st], ((tile / T::kStages) - 1) & 1, &abort_flag, status);
+            ok = __all_sync(0xffffffffu, ok);
+            ++tile;
+            return st;
+        };
         while (walk.next(s, p, a, x)) {
             for (int j = x.ja; j < x.jb; ++j) {
                 const int pos0 = j * kPagedUnitLarge;
-                // lane l looks up the page of positions 8 l .. 8 l + 7
+                // every warp looks up all of the tile's pages: lane b that of box b
                 int mine = -1;
-                if (lane < 16 && pos0 + 8 * lane < x.len && pos0 + 8 * lane + 7 >= x.lo)
-                    mine = paged_row(s, a.r.table, x.seq, x.g, pos0 + 8 * lane, status);
-                for (int kv = 0; kv < 2; ++kv) {
-                    const int st = tile % T::kStages;
-                    if (ok && tile >= T::kStages)
-                        ok = paged_wait(&kv_empty[st], ((tile / T::kStages) - 1) & 1, &abort_flag, status);
-                    ok = __all_sync(0xffffffffu, ok);
-                    const uint16_t *pool = kv ? a.r.v : a.r.k;
-                    const uint32_t base = kv_addr + st * T::kTile + (c >> 3) * 16384;
-#pragma unroll
-                    for (int i = 0; i < 128 / kRowsAtOnce; ++i) {
-                        const int r = r0 + i * kRowsAtOnce;
-                        const int row = __shfl_sync(0xffffffffu, mine, r >> 3);
-                        const bool in = row >= 0 && pos0 + r < x.len && pos0 + r >= x.lo;
-                        const long long src = in ? ((long long)row + (r & 7)) * HD + c * 8 : 0;
-                        if (ok) cp_async16(base + sw128_offset(r, c & 7), pool + src, in);
+                bool inside = pos0 >= x.lo && pos0 + kPagedUnitLarge <= x.len;
+                if (inside && lane < boxes)
+                    mine = paged_row(s, a.r.table, x.seq, x.g, pos0 + (lane << box_shift), status);
+                inside = inside && __all_sync(0xffffffffu, lane >= boxes || mine >= 0);
+                if (inside) {
+                    // op o = (box, 64-column half) is lane o / 4 of warp o % 4's
+                    const int o = lane * 4 + (warp - 8);
+                    const bool mine_op = o < boxes * T::kHalves;
+                    const int box = mine_op ? o / T::kHalves : 0, half = o % T::kHalves;
+                    const int row = __shfl_sync(0xffffffffu, mine, box);
+                    for (int kv = 0; kv < 2; ++kv) {
+                        const int st = claim();
+                        if (ok) {
+                            if (t == 0)
+                                mbar_arrive_expect_tx(&kv_full[st], T::kTile);
+                            else
+                                mbar_arrive(&kv_full[st]);
+                            if (mine_op)
+                                tma_load_2d(skv + st * T::kTile + half * 16384 + (box << box_shift) * 128,
+                                            kv ? &vmap : &kmap, half * 64, row, &kv_full[st]);
+                        }
                     }
-                    cp_async_commit();
-                    ++tile;
-                    signal_lagged();
+                } else {
+                    int mine8 = -1;  // the page of positions 8 lane .. 8 lane + 7
+                    if (lane < 16 && pos0 + 8 * lane < x.len && pos0 + 8 * lane + 7 >= x.lo)
+                        mine8 = paged_row(s, a.r.table, x.seq, x.g, pos0 + 8 * lane, status);
+                    int st[2];
+#pragma unroll
+                    for (int kv = 0; kv < 2; ++kv) {
+                        st[kv] = claim();
+                        const uint16_t *pool = kv ? a.r.v : a.r.k;
+                        const uint32_t base = kv_addr + st[kv] * T::kTile + (c >> 3) * 16384;
+#pragma unroll 4
+                        for (int i = 0; i < 128 / kRowsAtOnce; ++i) {
+                            const int r = r0 + i * kRowsAtOnce;
+                            const int row = __shfl_sync(0xffffffffu, mine8, r >> 3);
+                            const bool in = row >= 0 && pos0 + r < x.len && pos0 + r >= x.lo;
+                            const long long src = in ? ((long long)row + (r & 7)) * HD + c * 8 : 0;
+                            if (ok) cp_async16(base + sw128_offset(r, c & 7), pool + src, in);
+                        }
+                        cp_async_commit();
+                    }
+                    cp_async_wait(1);
+                    fence_proxy_async_smem();
+                    mbar_arrive(&kv_full[st[0]]);
+                    cp_async_wait(0);
+                    fence_proxy_async_smem();
+                    mbar_arrive(&kv_full[st[1]]);
                 }
             }
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
-        for (int n = max(0, tile - T::kLag); n < tile; ++n) signal(n);
-    } else if (warp == 12) {
+    } else if (warp >= 12) {
         // ---------------------------------------------------------- products
-        if (lane == 0) {
+        // The whole warp follows the schedule; one elected lane issues.
+        regs_less<kRegsOther>();
+        if (warp == 12) {
             constexpr uint32_t kIdQK = umma_idesc_bf16(128, 128, false), kIdPV = umma_idesc_bf16(128, HD, true);
+            const bool elected = elect_one();
+            const uint32_t q_lo = umma_desc_lo(smem_addr(sq), 16), k_lo = umma_desc_lo(smem_addr(skv), 16);
+            const uint32_t v_lo = umma_desc_lo(smem_addr(skv), 16384);
             int tile = 0;
             int nq[2] = {0, 0}, np[2] = {0, 0};
             bool ok = true;
             auto wait = [&](uint64_t *bar, int n) {
                 if (ok) ok = paged_wait(bar, n & 1, &abort_flag, status);
+                ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after_sync();
             };
             auto wait_kv = [&](int n) { wait(&kv_full[n % T::kStages], n / T::kStages); };
             auto qk = [&](int i, int n) {  // S_i = Q_i K^T with K in tile n
-                const uint32_t qa = smem_addr(sq + i * T::kTile), ka = smem_addr(skv + (n % T::kStages) * T::kTile);
-                if (ok) {
+                const uint32_t off = uniform((n % T::kStages) * (T::kTile >> 4));
+                if (ok && elected) {
 #pragma unroll
                     for (int k = 0; k < HD / 16; ++k) {
-                        const uint32_t off = (k >> 2) * 16384 + (k & 3) * 32;
-                        umma_f16(tmem + i * 128, umma_desc_sw128(qa + off), umma_desc_sw128(ka + off), kIdQK, k > 0);
+                        const uint32_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                        umma_bf16_ss(tmem + i * 128, q_lo + i * (T::kTile >> 4) + step, k_lo + off + step, kIdQK, k > 0);
                     }
                     umma_commit(&s_full[i]);
                 }
+                __syncwarp();
             };
             auto pv = [&](int i, int n, bool first) {  // O_i += P_i V with V in tile n
-                const uint32_t va = smem_addr(skv + (n % T::kStages) * T::kTile);
-                if (ok) {
+                const uint32_t off = uniform((n % T::kStages) * (T::kTile >> 4));
+                if (ok && elected) {
 #pragma unroll
                     for (int k = 0; k < 8; ++k)
-                        umma_bf16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k,
-                                     umma_desc_mn_sw128(va + k * 2048, 16384), kIdPV, !(first && k == 0));
+                        umma_bf16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, v_lo + off + k * (2048 >> 4), kIdPV,
+                                     !(first && k == 0));
                     umma_commit(&o_done[i]);
                 }
+                __syncwarp();
             };
             auto release = [&](int n) {
-                if (ok) umma_commit(&kv_empty[n % T::kStages]);
+                if (ok && elected) umma_commit(&kv_empty[n % T::kStages]);
+                __syncwarp();
             };
             while (walk.next(s, p, a, x)) {
                 const int t0 = tile;  // K of tile j is t0 + 2 (j - ja), V the next
+#pragma unroll
                 for (int i = 0; i < 2; ++i)
                     if (x.b[i] > x.a[i]) wait(&q_full[i], nq[i]++);
                 wait_kv(t0);
+#pragma unroll
                 for (int i = 0; i < 2; ++i)
                     if (x.a[i] <= x.ja && x.ja < x.b[i]) qk(i, t0);
                 release(t0);
                 for (int j = x.ja; j < x.jb; ++j) {
                     const int tk = t0 + 2 * (j - x.ja), tv = tk + 1, tn = tk + 2;
                     bool have_v = false, have_k = false;
+#pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         if (x.a[i] <= j && j < x.b[i]) {
-                            wait(&p_full[i], np[i]++);
                             if (!have_v) wait_kv(tv), have_v = true;
+                            wait(&p_full[i], np[i]++);
                             pv(i, tv, j == x.a[i]);
                         }
                         if (j + 1 < x.jb && x.a[i] <= j + 1 && j + 1 < x.b[i]) {
@@ -353,12 +442,14 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 tile = t0 + 2 * (x.jb - x.ja);
             }
             // every product has ended before tensor memory is given back
-            umma_commit(&drain);
+            if (elected) umma_commit(&drain);
+            __syncwarp();
             for (uint32_t i = 0; i < kWaitLimit && !mbar_try_wait(&drain, 0); ++i) {
             }
         }
     } else {
         // ----------------------------------------------------------- softmax
+        regs_more<kRegsSoftmax>();
         const int i = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const uint32_t ts = tmem + i * 128 + lanes, to = tmem + 256 + i * 128 + lanes;
@@ -368,7 +459,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
         int ns = 0;  // score tiles so far
         bool ok = true;
         while (walk.next(s, p, a, x)) {
-            const int n = x.n[i];
+            const int n = i ? x.n[1] : x.n[0], ta = i ? x.a[1] : x.a[0], tb = i ? x.b[1] : x.b[0];
             const int r = x.row0 + i * kTileRows + row, tok = r / s.group;  // packed row and its token
             const int head = x.g * s.group + r - tok * s.group;
             const bool live = row < n;
@@ -379,7 +470,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             const int min_hi = a.prefix_run ? x.len - 1 : x.first + rf / s.group;
             const int max_lo = s.window > 0 && !a.prefix_run ? x.first + (rf + max(n, 1) - 1) / s.group - s.window + 1 : 0;
             float m = -INFINITY, l = 0.f;  // the reference maximum (raw scale) and the sum
-            const bool active = x.b[i] > x.a[i];
+            const bool active = tb > ta;
             if (active) {
                 // this row of Q, zeros past the item's rows
                 const uint16_t *src = a.r.q + (long long)(x.q0 + tok) * a.r.q_stride + (long long)head * HD;
@@ -392,36 +483,37 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 fence_proxy_async_smem();
                 mbar_arrive(&q_full[i]);
             }
-            for (int j = x.a[i]; j < x.b[i]; ++j) {
+            for (int j = ta; j < tb; ++j) {
                 if (ok) ok = paged_wait(&s_full[i], ns & 1, &abort_flag, status);
                 ok = __all_sync(0xffffffffu, ok);
                 if (ok) {
                     tc_fence_after_sync();
                     const int pos0 = j * kPagedUnitLarge;
                     const bool masked = pos0 < max_lo || pos0 + kPagedUnitLarge - 1 > min_hi;
-                    float mx = -INFINITY;
+                    uint32_t v[4][32];  // the row's 128 scores
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, v[q]);
+                    tmem_wait_ld();
+                    if (capped) {
+#pragma unroll
+                        for (int e = 0; e < 128; ++e)
+                            v[e >> 5][e & 31] =
+                                __float_as_uint(score_log2(__uint_as_float(v[e >> 5][e & 31]), 0.f, a.r.cap, c2));
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 128; ++e)
+                            if (pos0 + e > hi || pos0 + e < lo) v[e >> 5][e & 31] = 0xFF800000u;  // -inf
+                    }
+                    float mx4[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        uint32_t v[32];
-                        tmem_ld32(ts + 32 * q, v);
-                        tmem_wait_ld();
-                        if (capped) {
+                        mx4[q] = fmaxf(__uint_as_float(v[q][0]), __uint_as_float(v[q][1]));
 #pragma unroll
-                            for (int e = 0; e < 32; ++e)
-                                v[e] = __float_as_uint(score_log2(__uint_as_float(v[e]), 0.f, a.r.cap, c2));
-                        }
-                        if (masked) {
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) {
-                                const int at = pos0 + 32 * q + e;
-                                if (at > hi || at < lo) v[e] = 0xFF800000u;  // -inf
-                            }
-                        }
-                        if (capped || masked) tmem_st32(ts + 32 * q, v);
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) mx = fmaxf(mx, __uint_as_float(v[e]));
+                        for (int e = 2; e < 32; e += 2)
+                            mx4[q] = max3(mx4[q], __uint_as_float(v[q][e]), __uint_as_float(v[q][e + 1]));
                     }
-                    if (capped || masked) tmem_wait_st();
+                    const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3]));
                     bool grow = false;
                     float f = 1.f;
                     if (m == -INFINITY) {
@@ -433,19 +525,19 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                         l *= f;
                     }
                     // j > a: the products of the tiles before are in O
-                    if (__any_sync(0xffffffffu, grow) && j > x.a[i]) {
+                    if (__any_sync(0xffffffffu, grow) && j > ta) {
                         if (ok) ok = paged_wait(&o_done[i], (ns - 1) & 1, &abort_flag, status);
                         ok = __all_sync(0xffffffffu, ok);
                         if (ok) {
                             tc_fence_after_sync();
-#pragma unroll
-                            for (int q = 0; q < HD / 32; ++q) {
-                                uint32_t v[32];
-                                tmem_ld32(to + 32 * q, v);
+#pragma unroll 1
+                            for (int q = 0; q < HD / 16; ++q) {
+                                uint32_t y[16];
+                                tmem_ld16(to + 16 * q, y);
                                 tmem_wait_ld();
 #pragma unroll
-                                for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(__uint_as_float(v[e]) * f);
-                                tmem_st32(to + 32 * q, v);
+                                for (int e = 0; e < 16; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
+                                tmem_st16(to + 16 * q, y);
                             }
                             tmem_wait_st();
                         }
@@ -454,17 +546,15 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                     float l4[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
-                        uint32_t v[32], w[16];
-                        tmem_ld32(ts + 32 * q, v);
-                        tmem_wait_ld();
+                        uint32_t w[16];
 #pragma unroll
                         for (int e = 0; e < 32; e += 2) {
-                            const float x0 = exp2_approx(fmaf(__uint_as_float(v[e]), mult, -ref));
-                            const float x1 = exp2_approx(fmaf(__uint_as_float(v[e + 1]), mult, -ref));
+                            const float x0 = exp2_approx(fmaf(__uint_as_float(v[q][e]), mult, -ref));
+                            const float x1 = exp2_approx(fmaf(__uint_as_float(v[q][e + 1]), mult, -ref));
                             l4[(e >> 1) & 3] += x0 + x1;
                             w[e >> 1] = pack_bf16(x0, x1);
                         }
-                        tmem_st16(ts + 16 * q, w);  // over scores already read
+                        tmem_st16(ts + 16 * q, w);  // over the scores
                     }
                     l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
                     tmem_wait_st();
