@@ -96,6 +96,7 @@ m1moe_status make_shape(const m1moe_paged_cfg *c, int ctas, m1::PagedShape &s) {
     s.nh = c->num_heads;
     s.nkv = c->num_kv_heads;
     s.group = group;
+    s.by_group = m1::make_fastdiv(group);
     s.hd = c->head_dim;
     s.page_size = c->page_size;
     while ((1 << s.page_shift) < c->page_size) ++s.page_shift;

@@ -82,6 +82,7 @@ struct PagedPrefixView {
 
 struct PagedShape {
     int nh, nkv, group, hd;
+    FastDiv by_group;
     int page_size, page_shift, num_pages;
     int num_seqs, max_pages, total_q, max_q;
     int window, prefix;

@@ -162,7 +162,131 @@ __device__ __forceinline__ void regs_less() {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N));
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) { return fmaxf(fmaxf(a, b), c); }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Two fp32 values in one 64-bit register (packed arithmetic issues once for both).
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// 2^x for two values of x <= kRescaleLog2 on the FMA pipes: x = n + f with n
+// the nearest whole number (1.5 * 2^23 added and taken off again leaves it in
+// the sum's low bits) and |f| <= 1/2, 2^f by the degree-4 polynomial of least
+// largest relative error there (2.6e-6, found by Remez exchange; the weight
+// is rounded to bf16's 3.9e-3 next), n added to the exponent.  x is cut off
+// at -126, where the weight is as good as zero.
+__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x2) {
+    float a, b;
+    unpack2(x2, a, b);
+    const uint64_t x = pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
+    const uint64_t t = add2(x, pack2(12582912.f, 12582912.f));
+    const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), x);
+    uint64_t p = fma2(pack2(0.009570102207362652f, 0.009570102207362652f), f,
+                      pack2(0.05591785907745361f, 0.05591785907745361f));
+    p = fma2(p, f, pack2(0.240247443318367f, 0.240247443318367f));
+    p = fma2(p, f, pack2(0.6931217908859253f, 0.6931217908859253f));
+    p = fma2(p, f, pack2(0.9999992847442627f, 0.9999992847442627f));
+    float ta, tb, pa, pb;
+    unpack2(t, ta, tb);
+    unpack2(p, pa, pb);
+    return pack2(__uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23)),
+                 __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23)));
+}
+
+// 32 raw scores capped, in units of log2: cap tanh(x) log2 e with x = score *
+// scale / cap.  While |x| <= 1 throughout the warp, tanh(x) / x is a degree-5
+// polynomial in x^2 (least largest relative error, 5.9e-7, by Remez
+// exchange); beyond, tanh(x) = 1 - 2 / (1 + e^2x).
+__device__ __forceinline__ void cap_scores(uint32_t (&v)[32], float scale_log2, float cap) {
+    const float cs = scale_log2 / (cap * kLog2e);
+    float top = 0.f;
+#pragma unroll
+    for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(__uint_as_float(v[e])));
+    if (__all_sync(0xffffffffu, top * cs <= 1.f)) {
+        const uint64_t c2 = pack2(cs, cs), s2 = pack2(scale_log2, scale_log2);
+#pragma unroll
+        for (int e = 0; e < 32; e += 2) {
+            const uint64_t d = pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
+            const uint64_t x = mul2(d, c2), y = mul2(x, x);
+            uint64_t t = fma2(pack2(-0.003067060373723507f, -0.003067060373723507f), y,
+                              pack2(0.016743114218115807f, 0.016743114218115807f));
+            t = fma2(t, y, pack2(-0.051605675369501114f, -0.051605675369501114f));
+            t = fma2(t, y, pack2(0.13281433284282684f, 0.13281433284282684f));
+            t = fma2(t, y, pack2(-0.3332904279232025f, -0.3332904279232025f));
+            t = fma2(t, y, pack2(0.9999994039535522f, 0.9999994039535522f));
+            float a, b;
+            unpack2(mul2(mul2(d, s2), t), a, b);
+            v[e] = __float_as_uint(a);
+            v[e + 1] = __float_as_uint(b);
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+            v[e] = __float_as_uint(score_log2(__uint_as_float(v[e]), 0.f, cap, 2.f * cs * kLog2e));
+    }
+}
+
+// The weights of a row's 128 scores, over the scores in tensor memory as bf16;
+// returns their fp32 sum.  kPolyOf8 of every 8 pairs take the polynomial, the
+// others the special-function unit.
+template <int kPolyOf8>
+__device__ __forceinline__ float row_weights(const uint32_t (&v)[4][32], float mult, float ref, uint32_t ts) {
+    const uint64_t mult2 = pack2(mult, mult), ref2 = pack2(-ref, -ref);
+    uint64_t sum[2] = {0, 0};
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        uint32_t w[16];
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+            const uint64_t x = fma2(pack2(__uint_as_float(v[q][2 * e]), __uint_as_float(v[q][2 * e + 1])), mult2, ref2);
+            uint64_t y;
+            float a, b;
+            if ((e * kPolyOf8) % 8 + kPolyOf8 >= 8 && kPolyOf8 > 0) {
+                y = exp2_poly2(x);
+                unpack2(y, a, b);
+            } else {
+                unpack2(x, a, b);
+                a = exp2_approx(a);
+                b = exp2_approx(b);
+                y = pack2(a, b);
+            }
+            sum[e & 1] = add2(sum[e & 1], y);
+            w[e] = pack_bf16(a, b);
+        }
+        tmem_st16(ts + 16 * q, w);
+    }
+    float a, b;
+    unpack2(add2(sum[0], sum[1]), a, b);
+    return a + b;
+}
+#ifndef KPOLY
+#define KPOLY 0
+#endif
+constexpr int kPolyOf8 = KPOLY;
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -179,13 +303,12 @@ __device__ __forceinline__ bool paged_wait(uint64_t *bar, uint32_t parity, volat
     return false;
 }
 
-// One segment of a CTA's run: tiles [ja, jb) of an item, and per M-tile its
-// rows and the tiles [a, b) that any of them sees.
+// One segment of a CTA's run: tiles [ja, jb) of an item, for the rows of one
+// or two M-tiles.
 struct Rows256Segment {
-    int g, item, u0, u1, seg0, seg1;  // its units, the item's units
-    int seq, row0, nrows, q0, len, first;  // first: position of row 0's token
-    int ja, jb, lo;                   // lo: first position any row sees
-    int n[2], a[2], b[2];
+    int g, item, u0, u1, seg0, seg1;       // its units, the item's units
+    int seq, row0, nrows, q0, len, first;  // first: position of the sequence's first new token
+    int ja, jb, lo;                        // lo: first position any row sees
 };
 
 // The roles walk the same segments, each on its own.
@@ -224,23 +347,13 @@ struct Rows256Walk {
             x.q0 = p.cu_q[it.seq];
             x.len = p.kv_len[it.seq];
             x.first = x.len - (p.cu_q[it.seq + 1] - x.q0);
-            x.lo = s.window > 0 ? max(0, x.first + it.row0 / s.group - s.window + 1) : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            x.n[i] = min(kTileRows, max(0, it.nrows - i * kTileRows));
-            x.a[i] = x.b[i] = x.ja;
-            if (x.n[i] > 0) {
-                const int r = it.row0 + i * kTileRows;
-                const int hi0 = a.prefix_run ? x.len - 1 : x.first + r / s.group;
-                const int hi1 = a.prefix_run ? x.len - 1 : x.first + (r + x.n[i] - 1) / s.group;
-                const int lo = s.window > 0 && !a.prefix_run ? max(0, hi0 - s.window + 1) : 0;
-                x.a[i] = max(x.ja, lo / kPagedUnitLarge);
-                x.b[i] = max(x.a[i], min(x.jb, hi1 < 0 ? 0 : hi1 / kPagedUnitLarge + 1));
-            }
+            x.lo = s.window > 0 ? max(0, x.first + fdiv(it.row0, s.by_group) - s.window + 1) : 0;
         }
         u = x.u1;
         if (u == x.seg1 && ++item == items) item = 0, ++g;
+        // the next item's record, for the next call
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(p.items + item));
+        asm volatile("prefetch.global.L1 [%0];" ::"l"(p.unit_at + item + 1));
         return true;
     }
 };
@@ -252,7 +365,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                                                                       const __grid_constant__ CUtensorMap vmap) {
     using T = Rows256<HD>;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t kv_full[T::kStages], kv_empty[T::kStages], q_full[2], s_full[2], p_full[2], o_done[2], drain;
+    __shared__ uint64_t kv_full[T::kStages], kv_empty[T::kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2], drain;
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag, sm_last[2];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -265,7 +378,8 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             mbar_init(&kv_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
-            mbar_init(&q_full[i], kTileRows);
+            mbar_init(&q_full[i], kRows256Loaders);
+            mbar_init(&q_empty[i], 1);
             mbar_init(&s_full[i], 1);
             mbar_init(&p_full[i], kTileRows);
             mbar_init(&o_done[i], 1);
@@ -306,7 +420,36 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             ++tile;
             return st;
         };
+        int nq0 = 0, nq1 = 0;  // times each M-tile's Q was loaded
+        auto nq_of = [&](int i) { return i ? nq1 : nq0; };
         while (walk.next(s, p, a, x)) {
+            // the rows of Q, HD / 8 lanes a row, zeros past the item's rows,
+            // as soon as the last segment's scores are done with the buffers
+            const int tiles = x.nrows > kTileRows ? 2 : 1;
+            for (int i = 0; i < tiles; ++i) {
+                if (ok && nq_of(i) > 0) ok = paged_wait(&q_empty[i], (nq_of(i) - 1) & 1, &abort_flag, status);
+                ok = __all_sync(0xffffffffu, ok);
+                const uint32_t base = smem_addr(sq) + i * T::kTile + (c >> 3) * 16384;
+#pragma unroll 4
+                for (int k = 0; k < 128 / kRowsAtOnce; ++k) {
+                    const int r = r0 + k * kRowsAtOnce, pr = x.row0 + i * kTileRows + r;
+                    const bool in = i * kTileRows + r < x.nrows;
+                    const int pt = fdiv(pr, s.by_group);
+                    const long long src = in ? (long long)(x.q0 + pt) * a.r.q_stride +
+                                                   (long long)(x.g * s.group + pr - pt * s.group) * HD + c * 8
+                                             : 0;
+                    if (ok) cp_async16(base + sw128_offset(r, c & 7), a.r.q + src, in);
+                }
+            }
+            cp_async_commit();
+            ++nq0;
+            nq1 += tiles == 2;
+            bool q_sent = false;
+            auto send_q = [&]() {  // after a wait that covers the copies of Q
+                fence_proxy_async_smem();
+                for (int i = 0; i < tiles; ++i) mbar_arrive(&q_full[i]);
+                q_sent = true;
+            };
             for (int j = x.ja; j < x.jb; ++j) {
                 const int pos0 = j * kPagedUnitLarge;
                 // every warp looks up all of the tile's pages: lane b that of box b
@@ -333,6 +476,10 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                                             kv ? &vmap : &kmap, half * 64, row, &kv_full[st]);
                         }
                     }
+                    if (!q_sent) {
+                        cp_async_wait(0);
+                        send_q();
+                    }
                 } else {
                     int mine8 = -1;  // the page of positions 8 lane .. 8 lane + 7
                     if (lane < 16 && pos0 + 8 * lane < x.len && pos0 + 8 * lane + 7 >= x.lo)
@@ -354,6 +501,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                         cp_async_commit();
                     }
                     cp_async_wait(1);
+                    if (!q_sent) send_q();
                     fence_proxy_async_smem();
                     mbar_arrive(&kv_full[st[0]]);
                     cp_async_wait(0);
@@ -380,7 +528,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 tc_fence_after_sync();
             };
             auto wait_kv = [&](int n) { wait(&kv_full[n % T::kStages], n / T::kStages); };
-            auto qk = [&](int i, int n) {  // S_i = Q_i K^T with K in tile n
+            auto qk = [&](int i, int n, bool last) {  // S_i = Q_i K^T with K in tile n
                 const uint32_t off = uniform((n % T::kStages) * (T::kTile >> 4));
                 if (ok && elected) {
 #pragma unroll
@@ -389,6 +537,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                         umma_bf16_ss(tmem + i * 128, q_lo + i * (T::kTile >> 4) + step, k_lo + off + step, kIdQK, k > 0);
                     }
                     umma_commit(&s_full[i]);
+                    if (last) umma_commit(&q_empty[i]);  // the next segment's rows may come
                 }
                 __syncwarp();
             };
@@ -407,39 +556,46 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 if (ok && elected) umma_commit(&kv_empty[n % T::kStages]);
                 __syncwarp();
             };
-            while (walk.next(s, p, a, x)) {
-                const int t0 = tile;  // K of tile j is t0 + 2 (j - ja), V the next
+            // Tile after tile, across segments: S of the next tile (the next
+            // segment's first one, while this one's rows are still being
+            // finished) goes behind each P V.
+            bool more = walk.next(s, p, a, x);
+            int tiles = x.jb - x.ja, both = x.nrows > kTileRows;
+            if (more) {
+                wait_kv(0);
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (x.b[i] > x.a[i]) wait(&q_full[i], nq[i]++);
-                wait_kv(t0);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (x.a[i] <= x.ja && x.ja < x.b[i]) qk(i, t0);
-                release(t0);
-                for (int j = x.ja; j < x.jb; ++j) {
-                    const int tk = t0 + 2 * (j - x.ja), tv = tk + 1, tn = tk + 2;
-                    bool have_v = false, have_k = false;
+                    if (i == 0 || both) {
+                        wait(&q_full[i], nq[i]++);
+                        qk(i, 0, tiles == 1);
+                    }
+                release(0);
+            }
+            while (more) {
+                more = walk.next(s, p, a, x);
+                const int next_tiles = x.jb - x.ja, next_both = more && x.nrows > kTileRows;
+                for (int j = 0; j < tiles; ++j, tile += 2) {
+                    const bool ends = j + 1 == tiles;
+                    const bool follows = !ends || more;
+                    bool have_k = false;
+                    wait_kv(tile + 1);
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        if (x.a[i] <= j && j < x.b[i]) {
-                            if (!have_v) wait_kv(tv), have_v = true;
+                        if (i == 0 || both) {
                             wait(&p_full[i], np[i]++);
-                            pv(i, tv, j == x.a[i]);
+                            pv(i, tile + 1, j == 0);
                         }
-                        if (j + 1 < x.jb && x.a[i] <= j + 1 && j + 1 < x.b[i]) {
-                            if (!have_k) wait_kv(tn), have_k = true;
-                            qk(i, tn);
+                        if (follows && (i == 0 || (ends ? next_both : both))) {
+                            if (!have_k) wait_kv(tile + 2), have_k = true;
+                            if (ends) wait(&q_full[i], nq[i]++);
+                            qk(i, tile + 2, ends ? next_tiles == 1 : j + 2 == tiles);
                         }
                     }
-                    if (!have_v) wait_kv(tv);
-                    release(tv);
-                    if (j + 1 < x.jb) {
-                        if (!have_k) wait_kv(tn);
-                        release(tn);
-                    }
+                    release(tile + 1);
+                    if (follows) release(tile + 2);
                 }
-                tile = t0 + 2 * (x.jb - x.ja);
+                tiles = next_tiles;
+                both = next_both;
             }
             // every product has ended before tensor memory is given back
             if (elected) umma_commit(&drain);
@@ -455,56 +611,55 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
         const uint32_t ts = tmem + i * 128 + lanes, to = tmem + 256 + i * 128 + lanes;
         const bool capped = a.r.cap > 0.f;
         const float mult = capped ? 1.f : a.r.scale * kLog2e;
-        const float c2 = capped ? 2.f * a.r.scale / a.r.cap * kLog2e : 0.f;
         int ns = 0;  // score tiles so far
         bool ok = true;
         while (walk.next(s, p, a, x)) {
-            const int n = i ? x.n[1] : x.n[0], ta = i ? x.a[1] : x.a[0], tb = i ? x.b[1] : x.b[0];
-            const int r = x.row0 + i * kTileRows + row, tok = r / s.group;  // packed row and its token
+            const int n = min(kTileRows, x.nrows - i * kTileRows);  // rows of this M-tile
+            if (n <= 0) continue;
+            const int r = x.row0 + i * kTileRows + row, tok = fdiv(r, s.by_group);  // packed row and its token
             const int head = x.g * s.group + r - tok * s.group;
             const bool live = row < n;
             const int hi = a.prefix_run ? x.len - 1 : x.first + tok;
             const int lo = s.window > 0 && !a.prefix_run ? hi - s.window + 1 : 0;
             // limits that hold for the M-tile's every row
             const int rf = x.row0 + i * kTileRows;
-            const int min_hi = a.prefix_run ? x.len - 1 : x.first + rf / s.group;
-            const int max_lo = s.window > 0 && !a.prefix_run ? x.first + (rf + max(n, 1) - 1) / s.group - s.window + 1 : 0;
+            const int min_hi = a.prefix_run ? x.len - 1 : x.first + fdiv(rf, s.by_group);
+            const int max_lo = s.window > 0 && !a.prefix_run ? x.first + fdiv(rf + n - 1, s.by_group) - s.window + 1 : 0;
+            const int warp_hi = __shfl_sync(0xffffffffu, hi, 0), warp_lo = __shfl_sync(0xffffffffu, lo, 31);
             float m = -INFINITY, l = 0.f;  // the reference maximum (raw scale) and the sum
-            const bool active = tb > ta;
-            if (active) {
-                // this row of Q, zeros past the item's rows
-                const uint16_t *src = a.r.q + (long long)(x.q0 + tok) * a.r.q_stride + (long long)head * HD;
-                uint8_t *dst = sq + i * T::kTile;
-#pragma unroll
-                for (int c = 0; c < HD / 8; ++c) {
-                    const uint4 v = live ? *reinterpret_cast<const uint4 *>(src + 8 * c) : make_uint4(0, 0, 0, 0);
-                    *reinterpret_cast<uint4 *>(dst + (c >> 3) * 16384 + sw128_offset(row, c & 7)) = v;
-                }
-                fence_proxy_async_smem();
-                mbar_arrive(&q_full[i]);
-            }
-            for (int j = ta; j < tb; ++j) {
+            for (int j = x.ja; j < x.jb; ++j) {
                 if (ok) ok = paged_wait(&s_full[i], ns & 1, &abort_flag, status);
                 ok = __all_sync(0xffffffffu, ok);
                 if (ok) {
                     tc_fence_after_sync();
                     const int pos0 = j * kPagedUnitLarge;
                     const bool masked = pos0 < max_lo || pos0 + kPagedUnitLarge - 1 > min_hi;
+                    if (capped || masked) {
+                        // 32 scores at a time through tensor memory (rolled: the unrolled
+                        // code would not fit the instruction cache)
+#pragma unroll 1
+                        for (int q = 0; q < 4; ++q) {
+                            const int at = pos0 + 32 * q;
+                            // some row of this warp does not see all of the 32 positions
+                            const bool hides = at + 31 > warp_hi || at < warp_lo;
+                            if (!capped && !hides) continue;
+                            uint32_t y[32];
+                            tmem_ld32(ts + 32 * q, y);
+                            tmem_wait_ld();
+                            if (capped) cap_scores(y, a.r.scale * kLog2e, a.r.cap);
+                            if (hides) {
+#pragma unroll
+                                for (int e = 0; e < 32; ++e)
+                                    if (at + e > hi || at + e < lo) y[e] = 0xFF800000u;  // -inf
+                            }
+                            tmem_st32(ts + 32 * q, y);
+                        }
+                        tmem_wait_st();
+                    }
                     uint32_t v[4][32];  // the row's 128 scores
 #pragma unroll
                     for (int q = 0; q < 4; ++q) tmem_ld32(ts + 32 * q, v[q]);
                     tmem_wait_ld();
-                    if (capped) {
-#pragma unroll
-                        for (int e = 0; e < 128; ++e)
-                            v[e >> 5][e & 31] =
-                                __float_as_uint(score_log2(__uint_as_float(v[e >> 5][e & 31]), 0.f, a.r.cap, c2));
-                    }
-                    if (masked) {
-#pragma unroll
-                        for (int e = 0; e < 128; ++e)
-                            if (pos0 + e > hi || pos0 + e < lo) v[e >> 5][e & 31] = 0xFF800000u;  // -inf
-                    }
                     float mx4[4];
 #pragma unroll
                     for (int q = 0; q < 4; ++q) {
@@ -525,7 +680,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                         l *= f;
                     }
                     // j > a: the products of the tiles before are in O
-                    if (__any_sync(0xffffffffu, grow) && j > ta) {
+                    if (__any_sync(0xffffffffu, grow) && j > x.ja) {
                         if (ok) ok = paged_wait(&o_done[i], (ns - 1) & 1, &abort_flag, status);
                         ok = __all_sync(0xffffffffu, ok);
                         if (ok) {
@@ -543,20 +698,8 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                         }
                     }
                     const float ref = m == -INFINITY ? 0.f : m * mult;
-                    float l4[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        uint32_t w[16];
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
-                            const float x0 = exp2_approx(fmaf(__uint_as_float(v[q][e]), mult, -ref));
-                            const float x1 = exp2_approx(fmaf(__uint_as_float(v[q][e + 1]), mult, -ref));
-                            l4[(e >> 1) & 3] += x0 + x1;
-                            w[e >> 1] = pack_bf16(x0, x1);
-                        }
-                        tmem_st16(ts + 16 * q, w);  // over the scores
-                    }
-                    l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
+                    // hidden positions weigh exactly nothing: the special-function unit's 2^-inf
+                    l += masked ? row_weights<0>(v, mult, ref, ts) : row_weights<kPolyOf8>(v, mult, ref, ts);
                     tmem_wait_st();
                     tc_fence_before_sync();
                 }
@@ -564,21 +707,14 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 ++ns;
             }
             // ------------------------------------------------ the segment's end
-            if (active) {
-                if (ok) ok = paged_wait(&o_done[i], (ns - 1) & 1, &abort_flag, status);
-                ok = __all_sync(0xffffffffu, ok);
-                if (ok) tc_fence_after_sync();
-            }
-            const bool has_o = active && ok;
+            if (ok) ok = paged_wait(&o_done[i], (ns - 1) & 1, &abort_flag, status);
+            ok = __all_sync(0xffffffffu, ok);
+            if (ok) tc_fence_after_sync();
             const bool whole = x.u0 == x.seg0 && x.u1 == x.seg1;
             const long long token = x.q0 + tok;
-            auto write_row = [&](float inv, int q, const float (&o)[32]) {  // 32 columns of the row
-                if (a.prefix_run) {
-                    float *d = a.partial + (token * s.nh + head) * HD + 32 * q;
-#pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4 *>(d + e) = make_float4(o[e], o[e + 1], o[e + 2], o[e + 3]);
-                } else if (a.r.out_bf16) {
+            auto put = [&](float inv, int q, const float (&o)[32]) {  // 32 columns of this thread's row
+                if (!live) return;
+                if (!a.prefix_run && a.r.out_bf16) {
                     uint16_t *d = reinterpret_cast<uint16_t *>(a.r.out) + token * a.r.out_stride + (long long)head * HD + 32 * q;
 #pragma unroll
                     for (int e = 0; e < 32; e += 8)
@@ -586,10 +722,12 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                             make_uint4(pack_bf16(o[e] * inv, o[e + 1] * inv), pack_bf16(o[e + 2] * inv, o[e + 3] * inv),
                                        pack_bf16(o[e + 4] * inv, o[e + 5] * inv), pack_bf16(o[e + 6] * inv, o[e + 7] * inv));
                 } else {
-                    float *d = reinterpret_cast<float *>(a.r.out) + token * a.r.out_stride + (long long)head * HD + 32 * q;
+                    const float f = a.prefix_run ? 1.f : inv;
+                    float *d = a.prefix_run ? a.partial + (token * s.nh + head) * HD + 32 * q
+                                            : reinterpret_cast<float *>(a.r.out) + token * a.r.out_stride + (long long)head * HD + 32 * q;
 #pragma unroll
                     for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4 *>(d + e) = make_float4(o[e] * inv, o[e + 1] * inv, o[e + 2] * inv, o[e + 3] * inv);
+                        *reinterpret_cast<float4 *>(d + e) = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
                 }
             };
             // partials: [slot][M-tile][hd / 4][row] float4, so that a warp's rows are one run
@@ -600,38 +738,31 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             const int slot = 2 * blockIdx.x + (x.u0 == x.seg0 ? 1 : 0);
             const float ml_m = m == -INFINITY ? m : m * mult;  // log2 scale
             const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (n > 0) {
-#pragma unroll
-                for (int q = 0; q < HD / 32; ++q) {
-                    float o[32];
-                    if (has_o) {
-                        uint32_t v[32];
-                        tmem_ld32(to + 32 * q, v);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = __uint_as_float(v[e]);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
-                    }
-                    if (live) {
-                        if (whole) {
-                            write_row(inv, q, o);
-                        } else if (active) {
-                            float4 *d = part_at(slot) + 8 * q * kTileRows;
-#pragma unroll
-                            for (int e = 0; e < 8; ++e)
-                                d[e * kTileRows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                        }
-                    }
+#pragma unroll 1
+            for (int q = 0; q < HD / 32; ++q) {
+                uint32_t v[32];
+                float o[32];
+                if (ok) {
+                    tmem_ld32(to + 32 * q, v);
+                    tmem_wait_ld();
                 }
-                if (has_o) tc_fence_before_sync();
-                if (live) {
-                    if (!whole)
-                        *part_ml_at(slot) = make_float2(active ? ml_m : -INFINITY, l);
-                    else if (a.prefix_run)
-                        a.partial_ml[token * s.nh + head] = make_float2(ml_m, l);
+#pragma unroll
+                for (int e = 0; e < 32; ++e) o[e] = ok ? __uint_as_float(v[e]) : 0.f;
+                if (whole) {
+                    put(inv, q, o);
+                } else if (live) {
+                    float4 *d = part_at(slot) + 8 * q * kTileRows;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e)
+                        d[e * kTileRows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
+            }
+            if (ok) tc_fence_before_sync();
+            if (live) {
+                if (!whole)
+                    *part_ml_at(slot) = make_float2(ml_m, l);
+                else if (a.prefix_run)
+                    a.partial_ml[token * s.nh + head] = make_float2(ml_m, l);
             }
             if (!whole) {
                 // the last M-tile of the item to finish joins its partials, in position order
@@ -647,39 +778,37 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 named_sync(1 + i, kTileRows);
                 if (sm_last[i]) {
                     __threadfence();
-                    if (live) {
-                        auto slot_of = [&](int c) { return 2 * c + (c == first ? 1 : 0); };
-                        float mm = -INFINITY, ll = 0.f;
-                        for (int c = first; c <= last; ++c) {
-                            const float2 v = __ldcg(part_ml_at(slot_of(c)));
-                            const float mn = fmaxf(mm, v.x);
-                            if (mn != -INFINITY) ll = ll * exp2_approx(mm - mn) + v.y * exp2_approx(v.x - mn);
-                            mm = mn;
-                        }
-                        const float iv = ll == 0.f ? 0.f : 1.f / ll;
-#pragma unroll 1
-                        for (int q = 0; q < HD / 32; ++q) {
-                            float o[32];
-#pragma unroll
-                            for (int e = 0; e < 32; ++e) o[e] = 0.f;
-                            for (int c = first; c <= last; ++c) {
-                                const float2 v = __ldcg(part_ml_at(slot_of(c)));
-                                if (v.x == -INFINITY) continue;
-                                const float w = exp2_approx(v.x - mm);
-                                const float4 *d = part_at(slot_of(c)) + 8 * q * kTileRows;
-#pragma unroll
-                                for (int e = 0; e < 8; ++e) {
-                                    const float4 y = __ldcg(d + e * kTileRows);
-                                    o[4 * e] = fmaf(y.x, w, o[4 * e]);
-                                    o[4 * e + 1] = fmaf(y.y, w, o[4 * e + 1]);
-                                    o[4 * e + 2] = fmaf(y.z, w, o[4 * e + 2]);
-                                    o[4 * e + 3] = fmaf(y.w, w, o[4 * e + 3]);
-                                }
-                            }
-                            write_row(iv, q, o);
-                        }
-                        if (a.prefix_run) a.partial_ml[token * s.nh + head] = make_float2(mm, ll);
+                    auto slot_of = [&](int c) { return 2 * c + (c == first ? 1 : 0); };
+                    float mm = -INFINITY, ll = 0.f;
+                    for (int c = first; live && c <= last; ++c) {
+                        const float2 v = __ldcg(part_ml_at(slot_of(c)));
+                        const float mn = fmaxf(mm, v.x);
+                        if (mn != -INFINITY) ll = ll * exp2_approx(mm - mn) + v.y * exp2_approx(v.x - mn);
+                        mm = mn;
                     }
+                    const float iv = ll == 0.f ? 0.f : 1.f / ll;
+#pragma unroll 1
+                    for (int q = 0; q < HD / 32; ++q) {
+                        float o[32];
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                        for (int c = first; live && c <= last; ++c) {
+                            const float2 v = __ldcg(part_ml_at(slot_of(c)));
+                            if (v.x == -INFINITY) continue;
+                            const float w = exp2_approx(v.x - mm);
+                            const float4 *d = part_at(slot_of(c)) + 8 * q * kTileRows;
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) {
+                                const float4 y = __ldcg(d + e * kTileRows);
+                                o[4 * e] = fmaf(y.x, w, o[4 * e]);
+                                o[4 * e + 1] = fmaf(y.y, w, o[4 * e + 1]);
+                                o[4 * e + 2] = fmaf(y.z, w, o[4 * e + 2]);
+                                o[4 * e + 3] = fmaf(y.w, w, o[4 * e + 3]);
+                            }
+                        }
+                        put(iv, q, o);
+                    }
+                    if (live && a.prefix_run) a.partial_ml[token * s.nh + head] = make_float2(mm, ll);
                 }
             }
         }
