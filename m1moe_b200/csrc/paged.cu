@@ -225,6 +225,14 @@ m1moe_status launch_rows256(const m1::PagedShape &s, const m1::PagedPlanView &v,
     if (m1moe_status e = pool_map(s, r.v, &vmap)) return e;
     auto kern = m1::k_paged_rows256<HD>;
     constexpr int smem = m1::Rows256<HD>::kSmem;
+    // the register split of the warpgroups waits for ever if the block is
+    // launched with fewer registers than it hands out
+    static const int regs = [] {
+        cudaFuncAttributes at{};
+        return cudaFuncGetAttributes(&at, m1::k_paged_rows256<HD>) == cudaSuccess ? at.numRegs : 0;
+    }();
+    if (regs * m1::kRows256Threads < 128 * 2 * (m1::kRegsSoftmax + m1::kRegsOther))
+        return fail(M1MOE_ERR_CUDA, "k_paged_rows256 was built with %d registers", regs);
     P_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     return launch_pdl(kern, dim3(s.ctas), dim3(m1::kRows256Threads), (size_t)smem, st, "k_paged_rows256 launch", s, v, a,
                       kmap, vmap);

@@ -52,8 +52,9 @@ template <int HD>
 struct Rows256 {
     static constexpr int kHalves = HD / 64;                    // 128-byte columns of a tile
     static constexpr int kTile = 128 * HD * 2;                 // bytes of a Q M-tile, K tile or V tile
-    static constexpr int kStages = HD == 128 ? 5 : 8;
-    static constexpr int kSmem = 2 * kTile + kStages * kTile + 1024;
+    static constexpr int kStages = HD == 128 ? 4 : 8;
+    static constexpr int kStageOut = 8 * 1024;                  // 32 rows of 32 bytes a softmax warp, for the output
+    static constexpr int kSmem = (2 + kStages) * kTile + kStageOut + 1024;
 };
 
 struct Rows256Params {
@@ -193,30 +194,6 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
     return d;
 }
 
-// 2^x for two values of x <= kRescaleLog2 on the FMA pipes: x = n + f with n
-// the nearest whole number (1.5 * 2^23 added and taken off again leaves it in
-// the sum's low bits) and |f| <= 1/2, 2^f by the degree-4 polynomial of least
-// largest relative error there (2.6e-6, found by Remez exchange; the weight
-// is rounded to bf16's 3.9e-3 next), n added to the exponent.  x is cut off
-// at -126, where the weight is as good as zero.
-__device__ __forceinline__ uint64_t exp2_poly2(uint64_t x2) {
-    float a, b;
-    unpack2(x2, a, b);
-    const uint64_t x = pack2(fmaxf(a, -126.f), fmaxf(b, -126.f));
-    const uint64_t t = add2(x, pack2(12582912.f, 12582912.f));
-    const uint64_t f = fma2(add2(t, pack2(-12582912.f, -12582912.f)), pack2(-1.f, -1.f), x);
-    uint64_t p = fma2(pack2(0.009570102207362652f, 0.009570102207362652f), f,
-                      pack2(0.05591785907745361f, 0.05591785907745361f));
-    p = fma2(p, f, pack2(0.240247443318367f, 0.240247443318367f));
-    p = fma2(p, f, pack2(0.6931217908859253f, 0.6931217908859253f));
-    p = fma2(p, f, pack2(0.9999992847442627f, 0.9999992847442627f));
-    float ta, tb, pa, pb;
-    unpack2(t, ta, tb);
-    unpack2(p, pa, pb);
-    return pack2(__uint_as_float(__float_as_uint(pa) + (__float_as_uint(ta) << 23)),
-                 __uint_as_float(__float_as_uint(pb) + (__float_as_uint(tb) << 23)));
-}
-
 // 32 raw scores capped, in units of log2: cap tanh(x) log2 e with x = score *
 // scale / cap.  While |x| <= 1 throughout the warp, tanh(x) / x is a degree-5
 // polynomial in x^2 (least largest relative error, 5.9e-7, by Remez
@@ -251,42 +228,41 @@ __device__ __forceinline__ void cap_scores(uint32_t (&v)[32], float scale_log2, 
 }
 
 // The weights of a row's 128 scores, over the scores in tensor memory as bf16;
-// returns their fp32 sum.  kPolyOf8 of every 8 pairs take the polynomial, the
-// others the special-function unit.
-template <int kPolyOf8>
-__device__ __forceinline__ float row_weights(const uint32_t (&v)[4][32], float mult, float ref, uint32_t ts) {
+// returns their fp32 sum.  All scores are scaled first, then taken eight pairs
+// at a time, a batch's exponentials ahead of the last batch's sums and
+// conversions, so that the special-function unit always has work queued.
+__device__ __forceinline__ float row_weights(uint32_t (&v)[4][32], float mult, float ref, uint32_t ts) {
     const uint64_t mult2 = pack2(mult, mult), ref2 = pack2(-ref, -ref);
-    uint64_t sum[2] = {0, 0};
+    uint64_t sum[4] = {0, 0, 0, 0};
+    auto f = [&](int e) { return __uint_as_float(v[e >> 5][e & 31]); };
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-        uint32_t w[16];
+    for (int e = 0; e < 128; e += 2) {
+        float x0, x1;
+        unpack2(fma2(pack2(f(e), f(e + 1)), mult2, ref2), x0, x1);
+        v[e >> 5][e & 31] = __float_as_uint(x0);
+        v[e >> 5][(e & 31) + 1] = __float_as_uint(x1);
+    }
+    uint32_t w[16];
 #pragma unroll
-        for (int e = 0; e < 16; ++e) {
-            const uint64_t x = fma2(pack2(__uint_as_float(v[q][2 * e]), __uint_as_float(v[q][2 * e + 1])), mult2, ref2);
-            uint64_t y;
-            float a, b;
-            if ((e * kPolyOf8) % 8 + kPolyOf8 >= 8 && kPolyOf8 > 0) {
-                y = exp2_poly2(x);
-                unpack2(y, a, b);
-            } else {
-                unpack2(x, a, b);
-                a = exp2_approx(a);
-                b = exp2_approx(b);
-                y = pack2(a, b);
-            }
-            sum[e & 1] = add2(sum[e & 1], y);
-            w[e] = pack_bf16(a, b);
+    for (int b = 0; b <= 8; ++b) {
+        if (b < 8) {
+#pragma unroll
+            for (int e = 16 * b; e < 16 * b + 16; ++e) v[e >> 5][e & 31] = __float_as_uint(exp2_approx(f(e)));
         }
-        tmem_st16(ts + 16 * q, w);
+        if (b > 0) {
+            const int e0 = 16 * (b - 1);
+#pragma unroll
+            for (int e = e0; e < e0 + 16; e += 2) {
+                sum[(e >> 1) & 3] = add2(sum[(e >> 1) & 3], pack2(f(e), f(e + 1)));
+                w[(e & 31) >> 1] = pack_bf16(f(e), f(e + 1));
+            }
+            if ((b & 1) == 0) tmem_st16(ts + 8 * (b - 2), w);
+        }
     }
     float a, b;
-    unpack2(add2(sum[0], sum[1]), a, b);
+    unpack2(add2(add2(sum[0], sum[1]), add2(sum[2], sum[3])), a, b);
     return a + b;
 }
-#ifndef KPOLY
-#define KPOLY 0
-#endif
-constexpr int kPolyOf8 = KPOLY;
 
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -294,6 +270,7 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 // at once and the roles go through the rest of their motions without touching
 // tensor memory or issuing copies, so that every barrier still matches.
 __device__ __forceinline__ bool paged_wait(uint64_t *bar, uint32_t parity, volatile int *abort, int *status) {
+#pragma unroll 1
     for (uint32_t i = 0; i < kWaitLimit; ++i) {
         if (mbar_try_wait(bar, parity)) return true;
         if (*abort) return false;
@@ -370,6 +347,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
     __shared__ int abort_flag, sm_last[2];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sq = smem, *skv = smem + 2 * T::kTile;
+    uint8_t *sout = skv + T::kStages * T::kTile;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     int *status = p.status;
     if (threadIdx.x == 0) {
@@ -519,83 +497,81 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             const bool elected = elect_one();
             const uint32_t q_lo = umma_desc_lo(smem_addr(sq), 16), k_lo = umma_desc_lo(smem_addr(skv), 16);
             const uint32_t v_lo = umma_desc_lo(smem_addr(skv), 16384);
-            int tile = 0;
-            int nq[2] = {0, 0}, np[2] = {0, 0};
+            uint32_t phase = 0;  // bits 0, 1: next parity of q_full; 2, 3: of p_full
             bool ok = true;
-            auto wait = [&](uint64_t *bar, int n) {
-                if (ok) ok = paged_wait(bar, n & 1, &abort_flag, status);
+            auto wait = [&](uint64_t *bar, uint32_t parity) {
+                if (ok) ok = paged_wait(bar, parity & 1, &abort_flag, status);
                 ok = __all_sync(0xffffffffu, ok);
                 tc_fence_after_sync();
             };
             auto wait_kv = [&](int n) { wait(&kv_full[n % T::kStages], n / T::kStages); };
-            auto qk = [&](int i, int n, bool last) {  // S_i = Q_i K^T with K in tile n
-                const uint32_t off = uniform((n % T::kStages) * (T::kTile >> 4));
-                if (ok && elected) {
-#pragma unroll
-                    for (int k = 0; k < HD / 16; ++k) {
-                        const uint32_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                        umma_bf16_ss(tmem + i * 128, q_lo + i * (T::kTile >> 4) + step, k_lo + off + step, kIdQK, k > 0);
-                    }
-                    umma_commit(&s_full[i]);
-                    if (last) umma_commit(&q_empty[i]);  // the next segment's rows may come
-                }
-                __syncwarp();
-            };
-            auto pv = [&](int i, int n, bool first) {  // O_i += P_i V with V in tile n
-                const uint32_t off = uniform((n % T::kStages) * (T::kTile >> 4));
-                if (ok && elected) {
-#pragma unroll
-                    for (int k = 0; k < 8; ++k)
-                        umma_bf16_ts(tmem + 256 + i * 128, tmem + i * 128 + 8 * k, v_lo + off + k * (2048 >> 4), kIdPV,
-                                     !(first && k == 0));
-                    umma_commit(&o_done[i]);
-                }
-                __syncwarp();
-            };
             auto release = [&](int n) {
                 if (ok && elected) umma_commit(&kv_empty[n % T::kStages]);
                 __syncwarp();
             };
             // Tile after tile, across segments: S of the next tile (the next
             // segment's first one, while this one's rows are still being
-            // finished) goes behind each P V.
+            // finished) goes behind each P V.  The first turn has no P V.
+            // Loops stay rolled: the roles' code shares one instruction cache.
             bool more = walk.next(s, p, a, x);
-            int tiles = x.jb - x.ja, both = x.nrows > kTileRows;
-            if (more) {
-                wait_kv(0);
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    if (i == 0 || both) {
-                        wait(&q_full[i], nq[i]++);
-                        qk(i, 0, tiles == 1);
-                    }
-                release(0);
-            }
-            while (more) {
-                more = walk.next(s, p, a, x);
+            int tiles = 1, both = 0, j = 0, tile = -2;
+            bool begun = false;
+            while (more || j < tiles) {
+                const bool ends = j + 1 == tiles;
+                if (tile >= 0) wait_kv(tile + 1);
                 const int next_tiles = x.jb - x.ja, next_both = more && x.nrows > kTileRows;
-                for (int j = 0; j < tiles; ++j, tile += 2) {
-                    const bool ends = j + 1 == tiles;
-                    const bool follows = !ends || more;
-                    bool have_k = false;
-                    wait_kv(tile + 1);
+                const bool follows = !ends || more;
+                bool have_k = false;
+#pragma unroll 1
+                for (int i = 0; i < 2; ++i) {
+                    if (begun && (i == 0 || both)) {  // O_i += P_i V
+                        wait(&p_full[i], phase >> (2 + i));
+                        phase ^= 4u << i;
+                        const uint32_t off = uniform(((tile + 1) % T::kStages) * (T::kTile >> 4));
+                        const uint32_t d = uniform(tmem + 256 + i * 128), pa = uniform(tmem + i * 128);
+                        if (ok && elected) {
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        if (i == 0 || both) {
-                            wait(&p_full[i], np[i]++);
-                            pv(i, tile + 1, j == 0);
+                            for (int k = 0; k < 8; ++k)
+                                umma_bf16_ts(d, pa + 8 * k, v_lo + off + k * (2048 >> 4), kIdPV, !(j == 0 && k == 0));
+                            umma_commit(&o_done[i]);
                         }
-                        if (follows && (i == 0 || (ends ? next_both : both))) {
-                            if (!have_k) wait_kv(tile + 2), have_k = true;
-                            if (ends) wait(&q_full[i], nq[i]++);
-                            qk(i, tile + 2, ends ? next_tiles == 1 : j + 2 == tiles);
-                        }
+                        __syncwarp();
                     }
-                    release(tile + 1);
-                    if (follows) release(tile + 2);
+                    if (follows && (i == 0 || (ends ? next_both : both))) {  // S_i = Q_i K^T
+                        if (!have_k) wait_kv(tile + 2), have_k = true;
+                        if (ends) {
+                            wait(&q_full[i], phase >> i);
+                            phase ^= 1u << i;
+                        }
+                        const uint32_t off = uniform(((tile + 2) % T::kStages) * (T::kTile >> 4));
+                        const uint32_t d = uniform(tmem + i * 128), qa = uniform(q_lo + i * (T::kTile >> 4));
+                        if (ok && elected) {
+#pragma unroll
+                            for (int k = 0; k < HD / 16; ++k) {
+                                const uint32_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+                                umma_bf16_ss(d, qa + step, k_lo + off + step, kIdQK, k > 0);
+                            }
+                            umma_commit(&s_full[i]);
+                            // the segment's last scores: the next one's rows may come
+                            if (ends ? next_tiles == 1 : j + 2 == tiles) umma_commit(&q_empty[i]);
+                        }
+                        __syncwarp();
+                    }
                 }
-                tiles = next_tiles;
-                both = next_both;
+                if (tile >= 0) release(tile + 1);
+                if (follows) release(tile + 2);
+                tile += 2;
+                if (!ends) {
+                    ++j;
+                } else if (more) {
+                    tiles = next_tiles;
+                    both = next_both;
+                    j = 0;
+                    begun = true;
+                    more = walk.next(s, p, a, x);
+                } else {
+                    break;
+                }
             }
             // every product has ended before tensor memory is given back
             if (elected) umma_commit(&drain);
@@ -611,6 +587,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
         const uint32_t ts = tmem + i * 128 + lanes, to = tmem + 256 + i * 128 + lanes;
         const bool capped = a.r.cap > 0.f;
         const float mult = capped ? 1.f : a.r.scale * kLog2e;
+        uint8_t *stage = sout + warp * 1024;
         int ns = 0;  // score tiles so far
         bool ok = true;
         while (walk.next(s, p, a, x)) {
@@ -698,8 +675,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                         }
                     }
                     const float ref = m == -INFINITY ? 0.f : m * mult;
-                    // hidden positions weigh exactly nothing: the special-function unit's 2^-inf
-                    l += masked ? row_weights<0>(v, mult, ref, ts) : row_weights<kPolyOf8>(v, mult, ref, ts);
+                    l += row_weights(v, mult, ref, ts);
                     tmem_wait_st();
                     tc_fence_before_sync();
                 }
@@ -712,22 +688,41 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             if (ok) tc_fence_after_sync();
             const bool whole = x.u0 == x.seg0 && x.u1 == x.seg1;
             const long long token = x.q0 + tok;
-            auto put = [&](float inv, int q, const float (&o)[32]) {  // 32 columns of this thread's row
-                if (!live) return;
-                if (!a.prefix_run && a.r.out_bf16) {
-                    uint16_t *d = reinterpret_cast<uint16_t *>(a.r.out) + token * a.r.out_stride + (long long)head * HD + 32 * q;
+            const bool narrow = !a.prefix_run && a.r.out_bf16;  // bf16 rows; else f32
+            uint8_t *out_row = a.prefix_run ? reinterpret_cast<uint8_t *>(a.partial + (token * s.nh + head) * HD)
+                                            : reinterpret_cast<uint8_t *>(a.r.out) +
+                                                  (token * a.r.out_stride + (long long)head * HD) * (narrow ? 2 : 4);
+            const uint32_t live_rows = __ballot_sync(0xffffffffu, live);
+            // 32 bytes of each of the warp's rows, at byte `at` of the row: through
+            // shared memory, so that two lanes store a whole sector
+            auto store32 = [&](uint4 y0, uint4 y1, int at) {
+                const int sw = (lane >> 2) & 1;
+                *reinterpret_cast<uint4 *>(stage + lane * 32 + (sw << 4)) = y0;
+                *reinterpret_cast<uint4 *>(stage + lane * 32 + ((sw ^ 1) << 4)) = y1;
+                __syncwarp();
 #pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-                        *reinterpret_cast<uint4 *>(d + e) =
-                            make_uint4(pack_bf16(o[e] * inv, o[e + 1] * inv), pack_bf16(o[e + 2] * inv, o[e + 3] * inv),
-                                       pack_bf16(o[e + 4] * inv, o[e + 5] * inv), pack_bf16(o[e + 6] * inv, o[e + 7] * inv));
+                for (int k = 0; k < 2; ++k) {
+                    const int rr = 16 * k + (lane >> 1), c = lane & 1;
+                    const uint4 y = *reinterpret_cast<const uint4 *>(stage + rr * 32 + ((c ^ ((rr >> 2) & 1)) << 4));
+                    uint8_t *d = reinterpret_cast<uint8_t *>(
+                        __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(out_row), rr));
+                    if (live_rows >> rr & 1) *reinterpret_cast<uint4 *>(d + at + 16 * c) = y;
+                }
+                __syncwarp();
+            };
+            auto put = [&](float f, int col, const float (&o)[16]) {  // columns col .. col + 15 of this thread's row
+                if (narrow) {
+                    store32(make_uint4(pack_bf16(o[0] * f, o[1] * f), pack_bf16(o[2] * f, o[3] * f),
+                                       pack_bf16(o[4] * f, o[5] * f), pack_bf16(o[6] * f, o[7] * f)),
+                            make_uint4(pack_bf16(o[8] * f, o[9] * f), pack_bf16(o[10] * f, o[11] * f),
+                                       pack_bf16(o[12] * f, o[13] * f), pack_bf16(o[14] * f, o[15] * f)),
+                            2 * col);
                 } else {
-                    const float f = a.prefix_run ? 1.f : inv;
-                    float *d = a.prefix_run ? a.partial + (token * s.nh + head) * HD + 32 * q
-                                            : reinterpret_cast<float *>(a.r.out) + token * a.r.out_stride + (long long)head * HD + 32 * q;
+                    auto word = [&](int e) { return __float_as_uint(o[e] * f); };
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4)
-                        *reinterpret_cast<float4 *>(d + e) = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
+                    for (int e = 0; e < 16; e += 8)
+                        store32(make_uint4(word(e), word(e + 1), word(e + 2), word(e + 3)),
+                                make_uint4(word(e + 4), word(e + 5), word(e + 6), word(e + 7)), 4 * (col + e));
                 }
             };
             // partials: [slot][M-tile][hd / 4][row] float4, so that a warp's rows are one run
@@ -736,38 +731,33 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             };
             auto part_ml_at = [&](int slot) { return p.part_ml + ((size_t)slot * 2 + i) * kTileRows + row; };
             const int slot = 2 * blockIdx.x + (x.u0 == x.seg0 ? 1 : 0);
-            const float ml_m = m == -INFINITY ? m : m * mult;  // log2 scale
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-#pragma unroll 1
-            for (int q = 0; q < HD / 32; ++q) {
-                uint32_t v[32];
-                float o[32];
+            float mm = m == -INFINITY ? m : m * mult, ll = l;  // the row's maximum (log2 scale) and sum
+            const int per = p.header[kPhPer];
+            const int first = x.seg0 / per, last = (x.seg1 - 1) / per;
+            auto slot_of = [&](int c) { return 2 * c + (c == first ? 1 : 0); };
+            auto read_o = [&](int q, float (&o)[16]) {  // 16 columns of O
+                uint32_t v[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) v[e] = 0;
                 if (ok) {
-                    tmem_ld32(to + 32 * q, v);
+                    tmem_ld16(to + 16 * q, v);
                     tmem_wait_ld();
                 }
 #pragma unroll
-                for (int e = 0; e < 32; ++e) o[e] = ok ? __uint_as_float(v[e]) : 0.f;
-                if (whole) {
-                    put(inv, q, o);
-                } else if (live) {
-                    float4 *d = part_at(slot) + 8 * q * kTileRows;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e)
-                        d[e * kTileRows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                }
-            }
-            if (ok) tc_fence_before_sync();
-            if (live) {
-                if (!whole)
-                    *part_ml_at(slot) = make_float2(ml_m, l);
-                else if (a.prefix_run)
-                    a.partial_ml[token * s.nh + head] = make_float2(ml_m, l);
-            }
+                for (int e = 0; e < 16; ++e) o[e] = __uint_as_float(v[e]);
+            };
             if (!whole) {
-                // the last M-tile of the item to finish joins its partials, in position order
-                const int per = p.header[kPhPer];
-                const int first = x.seg0 / per, last = (x.seg1 - 1) / per;
+#pragma unroll 1
+                for (int q = 0; q < HD / 16; ++q) {
+                    float o[16];
+                    read_o(q, o);
+                    float4 *d = part_at(slot) + 4 * q * kTileRows;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        if (live) d[e * kTileRows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
+                }
+                if (live) *part_ml_at(slot) = make_float2(mm, ll);
+                // the last one of the item's CTAs joins its partials, in position order
                 __threadfence();
                 named_sync(1 + i, kTileRows);
                 if (row == 0) {
@@ -778,27 +768,34 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 named_sync(1 + i, kTileRows);
                 if (sm_last[i]) {
                     __threadfence();
-                    auto slot_of = [&](int c) { return 2 * c + (c == first ? 1 : 0); };
-                    float mm = -INFINITY, ll = 0.f;
+                    mm = -INFINITY, ll = 0.f;
+#pragma unroll 1
                     for (int c = first; live && c <= last; ++c) {
                         const float2 v = __ldcg(part_ml_at(slot_of(c)));
                         const float mn = fmaxf(mm, v.x);
                         if (mn != -INFINITY) ll = ll * exp2_approx(mm - mn) + v.y * exp2_approx(v.x - mn);
                         mm = mn;
                     }
-                    const float iv = ll == 0.f ? 0.f : 1.f / ll;
+                }
+            }
+            if (whole || sm_last[i]) {
+                const float f = a.prefix_run ? 1.f : ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll 1
-                    for (int q = 0; q < HD / 32; ++q) {
-                        float o[32];
+                for (int q = 0; q < HD / 16; ++q) {
+                    float o[16];
+                    if (whole) {
+                        read_o(q, o);
+                    } else {
 #pragma unroll
-                        for (int e = 0; e < 32; ++e) o[e] = 0.f;
+                        for (int e = 0; e < 16; ++e) o[e] = 0.f;
+#pragma unroll 1
                         for (int c = first; live && c <= last; ++c) {
                             const float2 v = __ldcg(part_ml_at(slot_of(c)));
                             if (v.x == -INFINITY) continue;
                             const float w = exp2_approx(v.x - mm);
-                            const float4 *d = part_at(slot_of(c)) + 8 * q * kTileRows;
+                            const float4 *d = part_at(slot_of(c)) + 4 * q * kTileRows;
 #pragma unroll
-                            for (int e = 0; e < 8; ++e) {
+                            for (int e = 0; e < 4; ++e) {
                                 const float4 y = __ldcg(d + e * kTileRows);
                                 o[4 * e] = fmaf(y.x, w, o[4 * e]);
                                 o[4 * e + 1] = fmaf(y.y, w, o[4 * e + 1]);
@@ -806,11 +803,13 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                                 o[4 * e + 3] = fmaf(y.w, w, o[4 * e + 3]);
                             }
                         }
-                        put(iv, q, o);
+                        __syncwarp();
                     }
-                    if (live && a.prefix_run) a.partial_ml[token * s.nh + head] = make_float2(mm, ll);
+                    put(f, 16 * q, o);
                 }
+                if (live && a.prefix_run) a.partial_ml[token * s.nh + head] = make_float2(mm, ll);
             }
+            if (ok) tc_fence_before_sync();
         }
     }
     tc_fence_before_sync();
