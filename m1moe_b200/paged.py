@@ -21,7 +21,29 @@ import math
 import torch
 
 from . import _lib
-from .expert_ffn import _stream, dtype_code
+from .expert_ffn import dtype_code
+
+_F32, _BF16 = torch.float32, torch.bfloat16
+_raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream() without its wrapper: 0.1 of 3 us
+
+
+def _fn(name: str):
+    """The entry point `name` with its status checked."""
+    f = None
+
+    def call(*args):
+        nonlocal f
+        if f is None:
+            f = getattr(_lib.lib(), name)
+        st = f(*args)
+        if st:
+            _lib.check(st, name)
+
+    return call
+
+
+_plan_call, _append_call = _fn("m1moe_cuda_paged_plan"), _fn("m1moe_cuda_paged_append")
+_attention_call, _status_call = _fn("m1moe_cuda_paged_attention"), _fn("m1moe_cuda_paged_status")
 
 
 class PagedKVCache:
@@ -50,6 +72,7 @@ class PagedKVCache:
         self.k, self.v = k, v
         self.num_layers, self.num_pages, self.num_kv_heads, self.page_size, self.head_dim = k.shape
         self.device = k.device
+        self._index = k.device.index
         self._layer_bytes = k[0].numel() * 2 if self.num_layers else 0
         self._k0, self._v0 = k.data_ptr(), v.data_ptr()
 
@@ -101,8 +124,10 @@ class PagedBatch:
                 raise ValueError(f"paged batch refused: {msg.decode() if msg else ''}")
             # torch's allocations are 512-byte aligned
             self.plan = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        self._home = torch.cuda.current_stream(dev).cuda_stream
+        self._home = _raw_stream(dev.index)
         self._plan, self._table = self.plan.data_ptr(), page_table.data_ptr()
+        self._q_shape = (cu[-1], num_heads, cache.head_dim)
+        self._qkv_shape = (cu[-1], (num_heads + 2 * cache.num_kv_heads) * cache.head_dim)
         self.update(stream=stream)
 
     def update(self, *, stream=None) -> None:
@@ -110,18 +135,18 @@ class PagedBatch:
         now (for a next step with the same new tokens per sequence; capturable)."""
         st = self._use(stream)
         with torch.cuda.device(self.cache.device):
-            _lib.call("m1moe_cuda_paged_plan", self._cfg, self.cu_q.data_ptr(), self.kv_lens.data_ptr(), self._table,
-                      self._plan, self.plan.numel(), st)
+            _plan_call(self._cfg, self.cu_q.data_ptr(), self.kv_lens.data_ptr(), self._table,
+                       self._plan, self.plan.numel(), st)
 
     def check(self, *, stream=None) -> None:
         """Wait for the stream and raise if a kernel found a length, page or position out of range."""
         with torch.cuda.device(self.cache.device):
-            _lib.call("m1moe_cuda_paged_status", self._plan, self._use(stream))
+            _status_call(self._plan, self._use(stream))
 
     def _use(self, stream) -> int:
-        st = _stream(stream)
+        st = _raw_stream(self.cache._index) if stream is None else stream.cuda_stream
         if st != self._home:  # keep the memory until this stream is done with it
-            s = stream if stream is not None else torch.cuda.current_stream()
+            s = stream if stream is not None else torch.cuda.current_stream(self.cache.device)
             for t in (self.plan, self.cu_q, self.kv_lens, self.page_table):
                 t.record_stream(s)
         return st
@@ -146,31 +171,36 @@ def paged_append(cache: PagedKVCache, layer: int, batch: PagedBatch, qkv: torch.
             with i + rot/2 or, with rope_pairs, 2i with 2i + 1
     q_norm, k_norm  bf16 [head dim] RMSNorm weights of each head, or None
     """
-    nh, hd = batch.num_heads, cache.head_dim
-    if qkv.dim() != 2 or qkv.shape[0] != batch.total_q or qkv.shape[1] != (nh + 2 * cache.num_kv_heads) * hd:
-        raise ValueError(f"qkv is {tuple(qkv.shape)}, expected ({batch.total_q}, {(nh + 2 * cache.num_kv_heads) * hd})")
-    if qkv.device != cache.device or qkv.stride(1) != 1:
+    if qkv.shape != batch._qkv_shape:
+        raise ValueError(f"qkv is {tuple(qkv.shape)}, expected {batch._qkv_shape}")
+    dev = cache.device
+    if qkv.device != dev or qkv.stride(1) != 1:
         raise ValueError("qkv: rows of contiguous elements on the cache's device")
-    if rope.device != cache.device or rope.dtype != torch.float32 or rope.dim() != 3 or rope.shape[2] != 2 or \
-            not rope.is_contiguous():
+    if rope.dim() != 3 or rope.dtype != _F32 or rope.shape[2] != 2 or rope.device != dev or not rope.is_contiguous():
         raise ValueError("rope: a contiguous float32 [positions][rot/2][2] tensor on the cache's device")
-    for w in (q_norm, k_norm):
-        if w is not None and (w.device != cache.device or w.dtype != torch.bfloat16 or w.shape != (hd,) or
-                              not w.is_contiguous()):
-            raise ValueError(f"norm weights: contiguous bfloat16 [{hd}] on the cache's device")
+    qn = kn = 0
+    if q_norm is not None:
+        qn = _norm_ptr(q_norm, cache)
+    if k_norm is not None:
+        kn = _norm_ptr(k_norm, cache)
     k, v = cache._ptrs(layer)
     st = batch._use(stream)
     if out is None:
-        out = _empty((batch.total_q, nh, hd), torch.bfloat16, cache.device, stream)
-    elif out.shape != (batch.total_q, nh, hd) or out.dtype != torch.bfloat16 or not out.is_contiguous() or \
-            out.device != cache.device:
-        raise ValueError(f"out: contiguous bfloat16 ({batch.total_q}, {nh}, {hd}) on the cache's device")
+        out = _empty(batch._q_shape, _BF16, dev, stream)
+    elif out.shape != batch._q_shape or out.dtype != _BF16 or not out.is_contiguous() or out.device != dev:
+        raise ValueError(f"out: contiguous bfloat16 {batch._q_shape} on the cache's device")
     if batch.total_q == 0:
         return out
-    _lib.call("m1moe_cuda_paged_append", batch._cfg, batch._plan, batch._table, qkv.data_ptr(), dtype_code(qkv.dtype),
-              qkv.stride(0), 0 if q_norm is None else q_norm.data_ptr(), 0 if k_norm is None else k_norm.data_ptr(),
-              eps, rope.data_ptr(), rope.shape[0], 2 * rope.shape[1], 1 if rope_pairs else 0, k, v, out.data_ptr(), st)
+    positions, pairs, _ = rope.shape
+    _append_call(batch._cfg, batch._plan, batch._table, qkv.data_ptr(), dtype_code(qkv.dtype), qkv.stride(0), qn, kn, eps,
+                 rope.data_ptr(), positions, 2 * pairs, 1 if rope_pairs else 0, k, v, out.data_ptr(), st)
     return out
+
+
+def _norm_ptr(w: torch.Tensor, cache: PagedKVCache) -> int:
+    if w.device != cache.device or w.dtype != _BF16 or w.shape != (cache.head_dim,) or not w.is_contiguous():
+        raise ValueError(f"norm weights: contiguous bfloat16 [{cache.head_dim}] on the cache's device")
+    return w.data_ptr()
 
 
 def paged_attention(cache: PagedKVCache, layer: int, batch: PagedBatch, q: torch.Tensor, *,
@@ -179,23 +209,31 @@ def paged_attention(cache: PagedKVCache, layer: int, batch: PagedBatch, q: torch
     """Attention of the batch's new tokens (q bf16 [total_q][heads][head dim], tokens may lie
     further apart) over their sequences; scores are scale * q.k (default 1/sqrt(head dim)), capped
     as softcap * tanh(score / softcap) if softcap > 0."""
-    nh, hd = batch.num_heads, cache.head_dim
-    for t, name in ((q, "q"), (out, "out")):
-        if t is not None and (t.shape != (batch.total_q, nh, hd) or t.device != cache.device or
-                              (t.numel() and (t.stride(2) != 1 or t.stride(1) != hd))):
-            raise ValueError(f"{name}: ({batch.total_q}, {nh}, {hd}) with contiguous heads on the cache's device")
-    if q.dtype != torch.bfloat16:
+    if q.dtype != _BF16:
         raise TypeError(f"q must be bfloat16, got {q.dtype}")
+    stride = _check_rows(q, "q", cache, batch)
     k, v = cache._ptrs(layer)
     st = batch._use(stream)
     if out is None:
-        out = _empty((batch.total_q, nh, hd), out_dtype, cache.device, stream)
+        out = _empty(batch._q_shape, out_dtype, cache.device, stream)
+        out_stride = batch._qkv_shape[1] - 2 * cache.num_kv_heads * cache.head_dim
+    else:
+        out_stride = _check_rows(out, "out", cache, batch)
     if batch.total_q == 0:
         return out
-    _lib.call("m1moe_cuda_paged_attention", batch._cfg, batch._plan, batch._table, q.data_ptr(), q.stride(0), k, v,
-              1.0 / math.sqrt(hd) if scale is None else scale, softcap, out.data_ptr(), dtype_code(out.dtype),
-              out.stride(0), st)
+    _attention_call(batch._cfg, batch._plan, batch._table, q.data_ptr(), stride, k, v,
+                    1.0 / math.sqrt(cache.head_dim) if scale is None else scale, softcap, out.data_ptr(),
+                    dtype_code(out.dtype), out_stride, st)
     return out
+
+
+def _check_rows(t: torch.Tensor, name: str, cache: PagedKVCache, batch: PagedBatch) -> int:
+    """The token stride of t [total_q][heads][head dim], heads contiguous."""
+    rows, inner, last = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if t.shape != batch._q_shape or t.device != cache.device or last != 1 or inner != cache.head_dim:
+        raise ValueError(f"{name}: {batch._q_shape} with contiguous heads on the cache's device")
+    # one token's stride may be anything; the C side wants at least its length
+    return rows if batch.total_q > 1 else batch.num_heads * cache.head_dim
 
 
 def rope_table(max_positions: int, rot_dim: int, *, theta: float = 10000.0, scaling: dict | None = None,

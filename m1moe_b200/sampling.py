@@ -8,9 +8,20 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib
-from .expert_ffn import _stream, dtype_code
-from .paged import _empty
+from .expert_ffn import dtype_code
+from .paged import _empty, _fn, _raw_stream
+
+_sample_call = _fn("m1moe_cuda_sample")
+_F32, _I32 = torch.float32, torch.int32
+
+
+def _setting(t, name: str, dtype: torch.dtype, rows: int, dev) -> tuple[int, float]:
+    """(pointer, 0) of a tensor [rows], or (0, value) of a number."""
+    if not isinstance(t, torch.Tensor):
+        return 0, t
+    if t.dtype != dtype or t.shape != (rows,) or t.device != dev or not t.is_contiguous():
+        raise ValueError(f"{name}: a contiguous {dtype} tensor [{rows}] on {dev}")
+    return t.data_ptr(), 0
 
 
 def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
@@ -23,26 +34,20 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, t
         raise ValueError("logits: a CUDA tensor [rows][vocab] of contiguous rows")
     rows, vocab = logits.shape
     dev = logits.device
-    args = []
-    for t, name, dtype in ((u, "u", torch.float32), (temperature, "temperature", torch.float32),
-                           (top_k, "top_k", torch.int32), (top_p, "top_p", torch.float32),
-                           (min_p, "min_p", torch.float32)):
-        if isinstance(t, torch.Tensor):
-            if t.device != dev or t.dtype != dtype or t.shape != (rows,) or not t.is_contiguous():
-                raise ValueError(f"{name}: a contiguous {dtype} tensor [{rows}] on {dev}")
-            args.append((t.data_ptr(), 0))
-        elif name == "u":
-            raise ValueError("u is a tensor of one uniform number per row")
-        else:
-            args.append((0, t))
-    st = _stream(stream)
+    if not isinstance(u, torch.Tensor):
+        raise ValueError("u is a tensor of one uniform number per row")
+    pu, _ = _setting(u, "u", _F32, rows, dev)
+    pt, vt = _setting(temperature, "temperature", _F32, rows, dev)
+    pk, vk = _setting(top_k, "top_k", _I32, rows, dev)
+    pp, vp = _setting(top_p, "top_p", _F32, rows, dev)
+    pm, vm = _setting(min_p, "min_p", _F32, rows, dev)
+    st = _raw_stream(dev.index) if stream is None else stream.cuda_stream
     if out is None:
-        out = _empty((rows,), torch.int32, dev, stream)
-    elif out.device != dev or out.dtype != torch.int32 or out.shape != (rows,) or not out.is_contiguous():
+        out = _empty((rows,), _I32, dev, stream)
+    elif out.device != dev or out.dtype != _I32 or out.shape != (rows,) or not out.is_contiguous():
         raise ValueError(f"out: a contiguous int32 tensor [{rows}] on {dev}")
-    (pu, _), (pt, vt), (pk, vk), (pp, vp), (pm, vm) = args
     # one row's stride may be anything; the C side wants at least the row's length
     stride = logits.stride(0) if rows > 1 else max(logits.stride(0), vocab)
-    _lib.call("m1moe_cuda_sample", logits.data_ptr(), dtype_code(logits.dtype), stride, rows, vocab, pu, pt, vt, pk,
-              vk, pp, vp, pm, vm, out.data_ptr(), st)
+    _sample_call(logits.data_ptr(), dtype_code(logits.dtype), stride, rows, vocab, pu, pt, vt, pk, vk, pp, vp, pm, vm,
+                 out.data_ptr(), st)
     return out
