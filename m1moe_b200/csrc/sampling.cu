@@ -2,6 +2,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstdlib>
 
 #include "m1moe_cuda.h"
 #include "sampling.cuh"
@@ -17,7 +18,7 @@ using m1abi::cuda_fail;
 using m1abi::fail;
 
 namespace {
-constexpr size_t kSliceCap = 200 * 1024;  // dynamic shared memory beside the histograms
+constexpr size_t kDynCap = 184 * 1024;  // dynamic shared memory beside the histograms
 }
 
 extern "C" {
@@ -50,21 +51,29 @@ m1moe_status m1moe_cuda_sample(const void *d_logits, int32_t dtype, int64_t row_
     p.top_p1 = top_p;
     p.min_p1 = min_p;
     p.tokens = d_tokens;
+    const size_t size = p.bf16 ? 2 : 4;
+    auto bytes_of = [&](int c) {  // a CTA's slice, 16 bytes of skew, and the own bins of a long one
+        const int slice = (vocab + c - 1) / c;
+        return ((size_t)slice * size + 16 + 15) / 16 * 16 +
+               (slice > m1::kSampleLong ? (size_t)m1::kSampleWide * m1::kSampleThreads * 8 : 0);
+    };
     // CTAs per row: enough for the slice to fit in shared memory, more while
     // SMs would be idle
     int c = 1;
-    while (c < m1::kSampleMaxCluster && ((size_t)((vocab + c - 1) / c) * 4 > kSliceCap || (long long)rows * c * 2 <= 148))
-        c *= 2;
+    while (c < m1::kSampleMaxCluster && (bytes_of(c) > kDynCap || (long long)rows * c * 2 <= 148)) c *= 2;
+    if (const char *e = getenv("SAMPLE_C")) c = atoi(e);
     if ((long long)rows * c > 0x7FFFFFFFLL) return fail(M1MOE_ERR_UNSUPPORTED, "%d rows are too many", rows);
     p.slice = (vocab + c - 1) / c;
-    const size_t bytes = (size_t)p.slice * 4;
-    p.in_smem = bytes <= kSliceCap;
-    cudaError_t e = cudaFuncSetAttribute(m1::k_sample, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSliceCap);
+    const bool in_smem = bytes_of(c) <= kDynCap;
+    const size_t bytes = in_smem ? bytes_of(c) : (size_t)m1::kSampleWide * m1::kSampleThreads * 8;
+    auto kern = p.bf16 ? (in_smem ? m1::k_sample<uint16_t, true> : m1::k_sample<uint16_t, false>)
+                       : (in_smem ? m1::k_sample<float, true> : m1::k_sample<float, false>);
+    cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kDynCap);
     if (e != cudaSuccess) return cuda_fail(e, "k_sample shared memory");
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)rows * c);
     cfg.blockDim = dim3(m1::kSampleThreads);
-    cfg.dynamicSmemBytes = p.in_smem ? bytes : 0;
+    cfg.dynamicSmemBytes = bytes;
     cfg.stream = reinterpret_cast<cudaStream_t>(stream);
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
@@ -75,7 +84,7 @@ m1moe_status m1moe_cuda_sample(const void *d_logits, int32_t dtype, int64_t row_
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 2;
-    e = cudaLaunchKernelEx(&cfg, m1::k_sample, p);
+    e = cudaLaunchKernelEx(&cfg, kern, p);
     if (e != cudaSuccess) return cuda_fail(e, "k_sample launch");
     m1abi::count_launch();
     return M1MOE_OK;
