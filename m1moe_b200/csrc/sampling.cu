@@ -2,7 +2,6 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
-#include <cstdlib>
 
 #include "m1moe_cuda.h"
 #include "sampling.cuh"
@@ -57,11 +56,14 @@ m1moe_status m1moe_cuda_sample(const void *d_logits, int32_t dtype, int64_t row_
         return ((size_t)slice * size + 16 + 15) / 16 * 16 +
                (slice > m1::kSampleLong ? (size_t)m1::kSampleWide * m1::kSampleThreads * 8 : 0);
     };
-    // CTAs per row: enough for the slice to fit in shared memory, more while
-    // SMs would be idle
+    // CTAs per row: enough for the slice to fit in shared memory, while most
+    // SMs would be idle, and for short slices where four make them so.  us for
+    // 1, 2, 4 and 8 CTAs a row: 192 rows of 32000 f32 95, 81, 73, 176; 256 of
+    // 50304 141, 128, 191, 234; one of 50304 35, 15, 12, 10; 48 of 150001 bf16
+    // 374, 216, 114, 132.
     int c = 1;
-    while (c < m1::kSampleMaxCluster && (bytes_of(c) > kDynCap || (long long)rows * c * 2 <= 148)) c *= 2;
-    if (const char *e = getenv("SAMPLE_C")) c = atoi(e);
+    while (c < m1::kSampleMaxCluster && (bytes_of(c) > kDynCap || (long long)rows * c * 2 <= 74)) c *= 2;
+    if (c < 4 && vocab > m1::kSampleLong) c = (vocab + 3) / 4 <= m1::kSampleLong ? 4 : 2;
     if ((long long)rows * c > 0x7FFFFFFFLL) return fail(M1MOE_ERR_UNSUPPORTED, "%d rows are too many", rows);
     p.slice = (vocab + c - 1) / c;
     const bool in_smem = bytes_of(c) <= kDynCap;

@@ -115,11 +115,16 @@ __device__ __forceinline__ void sample_scan(SampleShared &sm, uint32_t &n, unsig
     __syncthreads();
     if (lane == 31) sm.scan_n[warp] = n, sm.scan_w[warp] = w;
     __syncthreads();
-    uint32_t pn = 0;
-    unsigned long long pw = 0;
-    for (int i = 0; i < warp; ++i) pn += sm.scan_n[i], pw += sm.scan_w[i];
-    n += pn;
-    w += pw;
+    // every warp adds up the totals of those before it
+    uint32_t pn = lane < warp ? sm.scan_n[lane] : 0;
+    unsigned long long pw = lane < warp ? sm.scan_w[lane] : 0;
+#pragma unroll
+    for (int o = kSampleWarps / 2; o > 0; o >>= 1) {
+        pn += __shfl_xor_sync(0xffffffffu, pn, o);
+        pw += __shfl_xor_sync(0xffffffffu, pw, o);
+    }
+    n += __shfl_sync(0xffffffffu, pn, 0);
+    w += __shfl_sync(0xffffffffu, pw, 0);
 }
 
 // floor(2^36 e) of 0 <= e <= 1: the 24-bit significand shifted to its place.
@@ -150,6 +155,13 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleParams p)
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int C = (int)cluster.num_blocks(), rank = (int)cluster.block_rank();
     const int row = blockIdx.x / C;
+    auto row_sync = [&]() {  // of the row's CTAs
+        if (C > 1)
+            cluster.sync();
+        else
+            __syncthreads();
+    };
+    auto peer = [&](int c) { return C > 1 ? cluster.map_shared_rank(&sm, c) : &sm; };
     pdl_wait();
     const int i0 = min(p.vocab, rank * p.slice), n = min(p.vocab, i0 + p.slice) - i0;
     const T *src = reinterpret_cast<const T *>(p.logits) + (long long)row * p.stride + i0;
@@ -235,17 +247,18 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleParams p)
         sm.cta_top = best;
         sm.cta_arg = arg;
     }
-    cluster.sync();
+    row_sync();
     float top = -INFINITY;
     arg = 0x7FFFFFFF;
+#pragma unroll 1
     for (int c = 0; c < C; ++c) {
-        const SampleShared *o = cluster.map_shared_rank(&sm, c);
+        const SampleShared *o = peer(c);
         better(o->cta_top, o->cta_arg, top, arg);
     }
     const float temp = p.temperature ? p.temperature[row] : p.temperature1;
     if (top == -INFINITY || !(temp > 0.f)) {  // nothing to choose from; greedy
         if (rank == 0 && tid == 0) p.tokens[row] = top == -INFINITY ? -1 : arg;
-        cluster.sync();  // no CTA leaves while another reads its shared memory
+        row_sync();  // no CTA leaves while another reads its shared memory
         return;
     }
     const int k = p.top_k ? p.top_k[row] : p.top_k1;
@@ -276,11 +289,12 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleParams p)
         // clear the next round's buffer: it was last read two rounds ago, and
         // every CTA has passed the barrier of the last round since
         for (int q = 0; q < 3; ++q) sm.hist[(round + 1) % 3][q][tid] = 0;
-        cluster.sync();
+        row_sync();
         cnt = 0;
         wt = 0;
+#pragma unroll 1
         for (int c = 0; c < C; ++c) {
-            const uint32_t(*o)[kSampleBins] = cluster.map_shared_rank(&sm, c)->hist[b];
+            const uint32_t(*o)[kSampleBins] = peer(c)->hist[b];
             cnt += o[0][tid];
             if (weights) wt += (unsigned long long)o[1][tid] | ((unsigned long long)o[2][tid] << 32);
         }
@@ -479,10 +493,11 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleParams p)
         uint32_t none = 0;
         sample_scan(sm, none, w);
         if (tid == kSampleThreads - 1) sm.cta_w = w;
-        cluster.sync();
+        row_sync();
         w = 0;
-        for (int c = 0; c < C; ++c) w += cluster.map_shared_rank(&sm, c)->cta_w;
-        cluster.sync();  // (used again below)
+#pragma unroll 1
+        for (int c = 0; c < C; ++c) w += peer(c)->cta_w;
+        row_sync();  // (used again below)
         return w;
     };
     // The first bins of a long slice, by threads of their own: counts.
@@ -668,11 +683,12 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleParams p)
         sm.cta_w = a;
         sm.cta_n = b;
     }
-    cluster.sync();
+    row_sync();
     unsigned long long before = 0, all = 0;
     uint32_t n_before = 0, n_all = 0;
+#pragma unroll 1
     for (int c = 0; c < C; ++c) {
-        const SampleShared *o = cluster.map_shared_rank(&sm, c);
+        const SampleShared *o = peer(c);
         const unsigned long long cw = o->cta_w;
         const uint32_t cn = o->cta_n;
         // the cut's tokens are taken in index order
@@ -681,7 +697,7 @@ __global__ void __launch_bounds__(kSampleThreads) k_sample(const SampleParams p)
         all += cw + take * tie_w;
         n_all += cn;
     }
-    cluster.sync();  // every CTA has read the others' sums
+    row_sync();  // every CTA has read the others' sums
     const unsigned long long target = mul24(all, uf);
     // 4. the token: this warp's tokens hold the target, or another's do
     for (int i = 0; i < warp; ++i) {
