@@ -321,7 +321,6 @@ m1moe_status m1moe_cuda_paged_append(const m1moe_paged_cfg *cfg, const void *d_p
     if (s.total_q == 0) return M1MOE_OK;
     m1::AppendParams a{};
     a.qkv = d_qkv;
-    a.qkv_bf16 = bf;
     a.qkv_stride = qkv_stride;
     a.q_norm = d_q_norm;
     a.k_norm = d_k_norm;
@@ -334,13 +333,16 @@ m1moe_status m1moe_cuda_paged_append(const m1moe_paged_cfg *cfg, const void *d_p
     a.v = d_v_pages;
     a.q_out = d_q_out;
     a.table = d_page_table;
-    a.heads_per_group = 1;
-    a.groups = heads;
+    // one head a group of lanes while that leaves SMs idle, up to 4 (a token's
+    // place and angles are then looked up once for them)
     const int L = s.hd / 8;
-    const long long threads = (long long)s.total_q * a.groups * L;
-    if (threads > (1LL << 38)) return fail(M1MOE_ERR_UNSUPPORTED, "%d tokens are too many for one call", s.total_q);
-    const dim3 grid((unsigned)((threads + 255) / 256));
-    auto kern = s.hd == 128 ? m1::k_paged_append<128> : m1::k_paged_append<64>;
+    const long long lanes = (long long)s.total_q * heads * L;
+    if (lanes > (1LL << 38)) return fail(M1MOE_ERR_UNSUPPORTED, "%d tokens are too many for one call", s.total_q);
+    a.heads_per_group = (int)std::min<long long>(4, std::max<long long>(1, lanes / (s.ctas * 2048LL * 2)));
+    a.groups = (heads + a.heads_per_group - 1) / a.heads_per_group;
+    const dim3 grid((unsigned)(((long long)s.total_q * a.groups * L + 255) / 256));
+    auto kern = s.hd == 128 ? (bf ? m1::k_paged_append<128, true> : m1::k_paged_append<128, false>)
+                            : (bf ? m1::k_paged_append<64, true> : m1::k_paged_append<64, false>);
     return launch_pdl(kern, grid, dim3(256), 0, as_stream(stream), "k_paged_append launch", s, v, a);
 }
 

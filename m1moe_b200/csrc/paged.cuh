@@ -292,7 +292,6 @@ __global__ void __launch_bounds__(256) k_paged_tokens(const PagedShape s, const 
 // ----------------------------------------------------------------- append ----
 struct AppendParams {
     const void *qkv;
-    int qkv_bf16;
     long long qkv_stride;  // elements between tokens
     const uint16_t *q_norm, *k_norm;
     float eps;
@@ -305,41 +304,70 @@ struct AppendParams {
     int groups;            // groups per token
 };
 
-__device__ __forceinline__ void load8(const void *x, int bf16, long long at, float (&v)[8]) {
-    if (bf16) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4 *>(reinterpret_cast<const uint16_t *>(x) + at));
-        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            v[2 * i] = __uint_as_float(u[i] << 16);
-            v[2 * i + 1] = __uint_as_float(u[i] & 0xFFFF0000u);
-        }
-    } else {
-        const float4 *f = reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(x) + at);
-        const float4 a = __ldg(f), b = __ldg(f + 1);
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w;
-        v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-    }
-}
-
 __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<const uint32_t *>(&v);
 }
 
-__device__ __forceinline__ uint4 pack8(const float (&v)[8]) {
-    return make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
+// Two fp32 values in one 64-bit register (packed arithmetic issues once for both).
+__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(lo), "f"(hi));
+    return d;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float &lo, float &hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+// Four elements as two packed pairs.
+template <bool BF16>
+__device__ __forceinline__ void load4x(const void *x, long long at, uint64_t (&v)[2]) {
+    if constexpr (BF16) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2 *>(reinterpret_cast<const uint16_t *>(x) + at));
+        v[0] = pack2(__uint_as_float(w.x << 16), __uint_as_float(w.x & 0xFFFF0000u));
+        v[1] = pack2(__uint_as_float(w.y << 16), __uint_as_float(w.y & 0xFFFF0000u));
+    } else {
+        const float4 w = __ldg(reinterpret_cast<const float4 *>(reinterpret_cast<const float *>(x) + at));
+        v[0] = pack2(w.x, w.y);
+        v[1] = pack2(w.z, w.w);
+    }
+}
+__device__ __forceinline__ uint2 round4(const uint64_t (&v)[2]) {
+    float a, b, c, d;
+    unpack2(v[0], a, b);
+    unpack2(v[1], c, d);
+    return make_uint2(pack_bf16(a, b), pack_bf16(c, d));
 }
 
 // Append: y = rotate(x * rsqrt(mean(x^2) + eps) * w) of each new query and key
 // head, v as it is; q rows go out bf16, k and v rows into their pages.  A
-// group of HD / 8 lanes takes a head, 8 elements (16 bytes of bf16) a lane;
-// all sums in fp32, one rounding at the end.  The group keeps its token's
-// cosines and sines in registers over its heads.  A head half's partner
-// elements (i, i + rot/2) are rot/16 lanes away, adjacent pairs in the lane.
-template <int HD>
-__global__ void __launch_bounds__(256) k_paged_append(const PagedShape s, const PagedPlanView p,
-                                                      const AppendParams a) {
+// group of HD / 8 lanes takes a head, two runs of four elements a lane chosen
+// so that both elements of every rotated pair are the lane's: (i, i + rot/2)
+// from two runs rot/2 apart, or adjacent pairs from two neighbouring runs; the
+// lanes past the rotated part hold eight elements of the rest.  All sums in
+// fp32, one rounding at the end.  A group keeps its token's place and angles
+// over its heads and has the loads of kAppendAhead heads under way.  HBM
+// would bound it; what does is the instructions (about 80 a warp and two
+// heads), hence the packed arithmetic.
+constexpr int kAppendAhead = 2;
+template <int HD, bool BF16>
+__global__ void __launch_bounds__(256, 4) k_paged_append(const PagedShape s, const PagedPlanView p,
+                                                         const AppendParams a) {
     constexpr int L = HD / 8;
     const int gid = (blockIdx.x * 256 + threadIdx.x) / L, l = threadIdx.x % L;
     pdl_wait();
@@ -354,69 +382,103 @@ __global__ void __launch_bounds__(256) k_paged_append(const PagedShape s, const 
         pos = 0;
     }
     const int half = a.rot >> 1;
-    // this lane's elements 8l .. 8l+7 and the pairs they belong to
     const bool turns = 8 * l < a.rot;
-    const bool upper = !a.pairs && 8 * l >= half;  // the second half's elements
-    float2 cs[8];
+    const int at0 = turns && !a.pairs ? 4 * l : 8 * l, at1 = turns && !a.pairs ? 4 * l + half : 8 * l + 4;
+    uint64_t cs[2], sn[2];  // cosines and sines of this lane's four pairs
+    cs[0] = cs[1] = sn[0] = sn[1] = 0;
     if (turns) {
-        const int i0 = a.pairs ? 4 * l : (upper ? 8 * l - half : 8 * l);
-        const float4 *r = reinterpret_cast<const float4 *>(a.rope + (long long)pos * half + i0);
+        const float4 *r = reinterpret_cast<const float4 *>(a.rope + (long long)pos * half + 4 * l);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (a.pairs && i >= 2) break;
+        for (int i = 0; i < 2; ++i) {
             const float4 w = __ldg(r + i);
-            cs[2 * i] = make_float2(w.x, w.y);
-            cs[2 * i + 1] = make_float2(w.z, w.w);
+            cs[i] = pack2(w.x, w.z);
+            sn[i] = pack2(w.y, w.w);
         }
     }
     const int heads = s.nh + 2 * s.nkv;
     const int h0 = part * a.heads_per_group, h1 = min(heads, h0 + a.heads_per_group);
-    for (int h = h0; h < h1; ++h) {
-        float x[8];
-        load8(a.qkv, a.qkv_bf16, (long long)t * a.qkv_stride + (long long)h * HD + 8 * l, x);
-        const bool is_q = h < s.nh, is_v = h >= s.nh + s.nkv;
-        if (!is_v) {
-            const uint16_t *w = is_q ? a.q_norm : a.k_norm;
-            if (w) {
-                float ss = 0.f;
+    int row0 = -1;  // the token's pool row for KV head 0
+    if (in_seq && h1 > s.nh) row0 = paged_row(s, a.table, tok.x, 0, tok.y, p.status);
+    const long long src = (long long)t * a.qkv_stride;
+#pragma unroll 1
+    for (int kind = 0; kind < 3; ++kind) {  // queries, keys, values
+        const int from = kind == 0 ? 0 : s.nh + (kind - 1) * s.nkv;
+        const int b0 = max(h0, from), b1 = min(h1, kind == 0 ? s.nh : from + s.nkv);
+        if (b0 >= b1 || (kind > 0 && row0 < 0)) continue;
+        const uint16_t *w = kind == 0 ? a.q_norm : kind == 1 ? a.k_norm : nullptr;
+        uint64_t g0[2], g1[2];
+        if (w) load4x<true>(w, at0, g0), load4x<true>(w, at1, g1);
+        uint16_t *out = kind == 0 ? a.q_out + (long long)t * s.nh * HD
+                                  : (kind == 1 ? a.k : a.v) + (long long)row0 * HD;
+        const long long step = kind == 0 ? HD : (long long)s.page_size * HD;
+#pragma unroll 1
+        for (int hb = b0; hb < b1; hb += kAppendAhead) {
+            uint64_t x0[kAppendAhead][2], x1[kAppendAhead][2];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
-#pragma unroll
-                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
-                const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
-                float g[8];
-                load8(w, 1, 8 * l, g);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * r * g[i];
+            for (int j = 0; j < kAppendAhead; ++j) {
+                const long long at = src + (long long)min(hb + j, b1 - 1) * HD;
+                load4x<BF16>(a.qkv, at + at0, x0[j]);
+                load4x<BF16>(a.qkv, at + at1, x1[j]);
             }
-            if (a.pairs) {
-                if (turns) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float u = x[2 * i], v = x[2 * i + 1];
-                        x[2 * i] = u * cs[i].x - v * cs[i].y;
-                        x[2 * i + 1] = v * cs[i].x + u * cs[i].y;
+            for (int j = 0; j < kAppendAhead; ++j) {
+                if (hb + j >= b1) break;
+                uint64_t(&u)[2] = x0[j], (&v)[2] = x1[j];
+                if (w) {
+                    uint64_t ss2 = mul2(u[0], u[0]);
+                    ss2 = fma2(u[1], u[1], ss2);
+                    ss2 = fma2(v[0], v[0], ss2);
+                    ss2 = fma2(v[1], v[1], ss2);
+                    float sa, sb;
+                    unpack2(ss2, sa, sb);
+                    float ss = sa + sb;
+#pragma unroll
+                    for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(mask, ss, o);
+                    const float r = rsqrtf(ss * (1.0f / HD) + a.eps);
+                    const uint64_t r2 = pack2(r, r);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        u[i] = mul2(mul2(u[i], r2), g0[i]);
+                        v[i] = mul2(mul2(v[i], r2), g1[i]);
                     }
                 }
-            } else {
-                const int off = half / 8;
-                const int src = turns ? (upper ? l - off : l + off) : l;
+                if (kind < 2 && turns) {
+                    const uint64_t neg = pack2(-1.f, -1.f);
+                    if (a.pairs) {  // (u0 u1) (u2 u3) | (v0 v1) (v2 v3): each is a pair
+                        float p0[4], p1[4];
+                        unpack2(u[0], p0[0], p1[0]);
+                        unpack2(u[1], p0[1], p1[1]);
+                        unpack2(v[0], p0[2], p1[2]);
+                        unpack2(v[1], p0[3], p1[3]);
+                        float y0[4], y1[4];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const float o = __shfl_sync(mask, x[i], src, L);
-                    // first half a cos - b sin, second half b cos + a sin
-                    if (turns) x[i] = upper ? x[i] * cs[i].x + o * cs[i].y : x[i] * cs[i].x - o * cs[i].y;
+                        for (int i = 0; i < 2; ++i) {
+                            const uint64_t f = pack2(p0[2 * i], p0[2 * i + 1]), q = pack2(p1[2 * i], p1[2 * i + 1]);
+                            unpack2(fma2(f, cs[i], mul2(mul2(q, neg), sn[i])), y0[2 * i], y0[2 * i + 1]);
+                            unpack2(fma2(q, cs[i], mul2(f, sn[i])), y1[2 * i], y1[2 * i + 1]);
+                        }
+                        u[0] = pack2(y0[0], y1[0]);
+                        u[1] = pack2(y0[1], y1[1]);
+                        v[0] = pack2(y0[2], y1[2]);
+                        v[1] = pack2(y0[3], y1[3]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {  // first half a cos - b sin, second half b cos + a sin
+                            const uint64_t f = u[i], q = v[i];
+                            u[i] = fma2(f, cs[i], mul2(mul2(q, neg), sn[i]));
+                            v[i] = fma2(q, cs[i], mul2(f, sn[i]));
+                        }
+                    }
+                }
+                uint16_t *d = out + (hb + j - from) * step;
+                const uint2 y0 = round4(u), y1 = round4(v);
+                if (at1 == at0 + 4) {
+                    *reinterpret_cast<uint4 *>(d + at0) = make_uint4(y0.x, y0.y, y1.x, y1.y);
+                } else {
+                    *reinterpret_cast<uint2 *>(d + at0) = y0;
+                    *reinterpret_cast<uint2 *>(d + at1) = y1;
                 }
             }
-        }
-        const uint4 y = pack8(x);
-        if (is_q) {
-            *reinterpret_cast<uint4 *>(a.q_out + ((long long)t * s.nh + h) * HD + 8 * l) = y;
-        } else if (in_seq) {
-            const int g = is_v ? h - s.nh - s.nkv : h - s.nh;
-            const int row = paged_row(s, a.table, tok.x, g, tok.y, p.status);
-            uint16_t *pool = is_v ? a.v : a.k;
-            if (row >= 0) *reinterpret_cast<uint4 *>(pool + (long long)row * HD + 8 * l) = y;
         }
     }
 }
