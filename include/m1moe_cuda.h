@@ -544,6 +544,27 @@ M1MOE_API m1moe_status m1moe_cuda_paged_attention(const m1moe_paged_cfg *cfg, vo
  * M1MOE_ERR_DEVICE if a kernel of the batch raised a bit. */
 M1MOE_API m1moe_status m1moe_cuda_paged_status(void *d_plan, void *stream);
 
+/* One step of a whole model for a ragged batch over a paged cache: the new
+ * tokens d_tokens [total_q] of cfg's sequences (prompts, prompt chunks and
+ * single tokens together) through every layer -- embedding, input RMSNorm and
+ * q|k|v, m1moe_cuda_paged_append, m1moe_cuda_paged_attention, o projection and
+ * post-attention RMSNorm, the MoE block of `moe` -- then the final norm and LM
+ * head of each sequence's last new token: d_logits f32 [num_seqs][vocab] (a
+ * sequence without new tokens gets the logits of a zero state), for
+ * m1moe_cuda_sample.  The dense context gives weights and buffers; its own
+ * cache and position take no part.  d_k_pages and d_v_pages are
+ * [num_layers] pools one after another, d_rope as in m1moe_cuda_paged_append
+ * (the pairs i and i + rot_dim / 2).  Up to 8 tokens (and the MoE context's
+ * max_batch) take the decode kernels, more the prefill ones of
+ * m1moe_cuda_prefill_step.  The serving counterpart of InferenceEngine.forward
+ * (:124-156), which runs one token of one sequence.  Buffers for total_q
+ * tokens are allocated on the first call that needs them (synchronously). */
+M1MOE_API m1moe_status m1moe_cuda_paged_step(m1moe_dense_ctx *ctx, m1moe_cuda_ctx *moe,
+                                   const m1moe_paged_cfg *cfg, void *d_plan, const int32_t *d_page_table,
+                                   uint16_t *d_k_pages, uint16_t *d_v_pages, const float *d_rope,
+                                   int32_t rope_rows, int32_t rot_dim, const int32_t *d_tokens,
+                                   float *d_logits, void *stream);
+
 /* One token per row of logits [rows][vocab] (f32 or bf16, row_stride
  * elements apart; vocab at most 2^20) from one uniform number in [0, 1) per
  * row.  Settings per row (device arrays [rows]) or, where the array is NULL,

@@ -115,6 +115,8 @@ _SIGS = [
      [_vp, _vp, _vp, _vp, _i32, _i64, _vp, _vp, _f32, _vp, _i32, _i32, _i32, _vp, _vp, _vp, _vp]),
     ("m1moe_cuda_paged_attention", ctypes.c_int,
      [_vp, _vp, _vp, _vp, _i64, _vp, _vp, _f32, _f32, _vp, _i32, _i64, _vp]),
+    ("m1moe_cuda_paged_step", ctypes.c_int,
+     [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _i32, _i32, _vp, _vp, _vp]),
     ("m1moe_cuda_paged_status", ctypes.c_int, [_vp, _vp]),
     ("m1moe_cuda_sample", ctypes.c_int,
      [_vp, _i32, _i64, _i32, _i32, _vp, _vp, _f32, _vp, _i32, _vp, _f32, _vp, _f32, _vp, _vp]),

@@ -27,6 +27,9 @@ m1moe_status fail(m1moe_status st, const char *fmt, ...);
 m1moe_status cuda_fail(cudaError_t e, const char *what);
 void count_launch();
 m1moe_status moe_compatible(const m1moe_cuda_ctx *moe, int hidden, int layers, int batch, int device);
+int moe_max_batch(const m1moe_cuda_ctx *moe);
+m1moe_status paged_last_rows(const m1moe_paged_cfg *cfg, void *d_plan, const float *x, int h, float *out,
+                             cudaStream_t st);
 }  // namespace m1abi
 
 using m1abi::cuda_fail;
@@ -62,6 +65,12 @@ struct m1moe_dense_ctx {
     int pf_cap = 0;
     float *pf_res = nullptr, *pf_qkv = nullptr, *pf_hmid = nullptr;
     __nv_bfloat16 *pf_xn = nullptr, *pf_attn = nullptr;
+    // a step over a paged cache (m1moe_cuda_paged_step): the rotated queries of
+    // pg_cap tokens, the last rows of pg_seqs sequences and their bf16 form
+    int pg_cap = 0, pg_seqs = 0;
+    uint16_t *pg_q = nullptr;
+    float *pg_last = nullptr;
+    __nv_bfloat16 *pg_last_n = nullptr;
     cublasHandle_t blas = nullptr;
     // which tensors are loaded: [tensor][layer]
     std::vector<std::vector<uint8_t>> loaded;
@@ -141,7 +150,7 @@ void free_dense(m1moe_dense_ctx *c) {
                     (void *)c->attn_out, (void *)c->part, (void *)c->ss_acc, (void *)c->done,
                     (void *)c->keys, (void *)c->attn_cnt, (void *)c->pos, (void *)c->err,
                     (void *)c->pf_res, (void *)c->pf_qkv, (void *)c->pf_hmid, (void *)c->pf_xn,
-                    (void *)c->pf_attn})
+                    (void *)c->pf_attn, (void *)c->pg_q, (void *)c->pg_last, (void *)c->pg_last_n})
         cudaFree(q);
     if (c->blas) cublasDestroy(c->blas);
     delete c;
@@ -288,6 +297,25 @@ m1moe_status pf_dense_reserve(m1moe_dense_ctx *c, int T) {
     D_CK(cudaMalloc((void **)&c->pf_xn, (size_t)T * h * 2));
     D_CK(cudaMalloc((void **)&c->pf_attn, (size_t)T * c->qd * 2));
     c->pf_cap = T;
+    return M1MOE_OK;
+}
+
+// Buffers of a paged step: T tokens, B sequences.
+m1moe_status pg_reserve(m1moe_dense_ctx *c, int T, int B) {
+    if (m1moe_status st = pf_dense_reserve(c, T)) return st;
+    if (T <= c->pg_cap && B <= c->pg_seqs) return M1MOE_OK;
+    D_CK(cudaDeviceSynchronize());
+    const int t = std::max(T, c->pg_cap), b = std::max(B, c->pg_seqs);
+    for (void *q : {(void *)c->pg_q, (void *)c->pg_last, (void *)c->pg_last_n}) cudaFree(q);
+    c->pg_q = nullptr;
+    c->pg_last = nullptr;
+    c->pg_last_n = nullptr;
+    c->pg_cap = c->pg_seqs = 0;
+    D_CK(cudaMalloc((void **)&c->pg_q, (size_t)t * c->qd * 2));
+    D_CK(cudaMalloc((void **)&c->pg_last, (size_t)b * c->cfg.hidden_dim * 4));
+    D_CK(cudaMalloc((void **)&c->pg_last_n, (size_t)b * c->cfg.hidden_dim * 2));
+    c->pg_cap = t;
+    c->pg_seqs = b;
     return M1MOE_OK;
 }
 
@@ -707,6 +735,115 @@ m1moe_status m1moe_cuda_prefill_step(m1moe_dense_ctx *c, m1moe_cuda_ctx *moe, co
     lm.pos_add = T;
     lm.err = c->err;
     return gemv<m1::kEpiArgmax>(lm, c->num_sms, st);
+}
+
+m1moe_status m1moe_cuda_paged_step(m1moe_dense_ctx *c, m1moe_cuda_ctx *moe, const m1moe_paged_cfg *cfg, void *d_plan,
+                                   const int32_t *d_page_table, uint16_t *d_k_pages, uint16_t *d_v_pages,
+                                   const float *d_rope, int32_t rope_rows, int32_t rot_dim, const int32_t *d_tokens,
+                                   float *d_logits, void *stream) {
+    if (!c || !moe || !cfg || !d_plan || !d_page_table || !d_k_pages || !d_v_pages || !d_rope || !d_tokens || !d_logits)
+        return fail(M1MOE_ERR_INVALID_ARG, "NULL pointer");
+    const m1moe_dense_cfg &g = c->cfg;
+    if (cfg->num_heads != g.num_heads || cfg->num_kv_heads != g.num_kv_heads || cfg->head_dim != g.head_dim)
+        return fail(M1MOE_ERR_INVALID_ARG, "the batch's heads (%d, %d of %d) are not the model's (%d, %d of %d)",
+                    cfg->num_heads, cfg->num_kv_heads, cfg->head_dim, g.num_heads, g.num_kv_heads, g.head_dim);
+    const int T = cfg->total_q, B = cfg->num_seqs, h = g.hidden_dim;
+    if (T < 1) return fail(M1MOE_ERR_INVALID_ARG, "the batch has no new tokens");
+    if (m1moe_status st = check_loaded(c)) return st;
+    if (m1moe_status st = m1abi::moe_compatible(moe, h, g.num_layers, 1, g.device)) return st;
+    DevGuard dg(g.device);
+    if (m1moe_status st = pg_reserve(c, T, B)) return st;
+    cudaStream_t st = as_stream(stream);
+    const bool few = T <= std::min(m1::kDenseMaxTok, m1abi::moe_max_batch(moe));  // the decode kernels' batch
+    const size_t pool = (size_t)cfg->num_pages * g.num_kv_heads * cfg->page_size * c->hd;
+    if (m1moe_status s = launch_pdl(m1::k_embed, dim3(T), dim3(256), 0, st, "k_embed launch",
+                                    (const uint16_t *)c->embed, d_tokens, (int)g.vocab_size, h, c->pf_res, T, c->err))
+        return s;
+    for (int L = 0; L < g.num_layers; ++L) {
+        const uint16_t *wqkv = c->wqkv + (size_t)L * c->qkv_rows * h, *wo = c->wo + (size_t)L * h * c->qd;
+        const uint16_t *in_norm = c->in_norm + (size_t)L * h, *post_norm = c->post_norm + (size_t)L * h;
+        // 1. input RMSNorm and the q|k|v projections
+        if (few) {
+            m1::GemvParams q{};
+            q.w = wqkv;
+            q.rows = c->qkv_rows;
+            q.K = h;
+            q.x = c->pf_res;
+            q.norm_w = in_norm;
+            q.eps = g.rms_norm_eps;
+            q.y = c->pf_qkv;
+            q.ntok = T;
+            q.err = c->err;
+            if (m1moe_status s = gemv<m1::kEpiStore>(q, c->num_sms, st)) return s;
+        } else {
+            if (m1moe_status s = launch_pdl(m1::k_rmsnorm_bf16, dim3(T), dim3(256), 0, st, "k_rmsnorm_bf16 launch",
+                                            (const float *)c->pf_res, in_norm, (float)g.rms_norm_eps, c->pf_xn, h))
+                return s;
+            if (m1moe_status s = gemm_bf16(c, wqkv, c->pf_xn, c->pf_qkv, c->qkv_rows, h, T, false, st)) return s;
+        }
+        // 2. QK-norm, rotation and store of the new rows, then attention over the pages
+        uint16_t *kp = d_k_pages + (size_t)L * pool, *vp = d_v_pages + (size_t)L * pool;
+        if (m1moe_status s = m1moe_cuda_paged_append(
+                cfg, d_plan, d_page_table, c->pf_qkv, M1MOE_DTYPE_F32, c->qkv_rows,
+                g.qk_norm ? c->qn + (size_t)L * c->hd : nullptr, g.qk_norm ? c->kn + (size_t)L * c->hd : nullptr,
+                g.rms_norm_eps, d_rope, rope_rows, rot_dim, 0, kp, vp, c->pg_q, stream))
+            return s;
+        if (m1moe_status s = m1moe_cuda_paged_attention(cfg, d_plan, d_page_table, c->pg_q, c->qd, kp, vp,
+                                                        1.0f / sqrtf((float)c->hd), 0.f, c->pf_attn,
+                                                        M1MOE_DTYPE_BF16, c->qd, stream))
+            return s;
+        // 3. o projection added to the residual, post-attention RMSNorm, MoE block
+        if (few) {
+            m1::GemvParams o{};
+            o.w = wo;
+            o.rows = h;
+            o.K = c->qd;
+            o.x = c->pf_attn;
+            o.x_bf16 = 1;
+            o.eps = g.rms_norm_eps;
+            o.y = c->pf_res;
+            o.res = c->pf_res;
+            o.ntok = T;
+            o.post_w = post_norm;
+            o.post_out = c->pf_hmid;
+            o.ss_acc = c->ss_acc;
+            o.done = c->done;
+            o.err = c->err;
+            if (m1moe_status s = gemv<m1::kEpiPostNorm>(o, c->num_sms, st)) return s;
+            if (m1moe_status s = m1moe_cuda_moe_layer(moe, L, c->pf_hmid, M1MOE_DTYPE_F32, c->pf_res, M1MOE_DTYPE_F32,
+                                                      c->pf_res, M1MOE_DTYPE_F32, T, nullptr, nullptr, stream))
+                return s;
+        } else {
+            if (m1moe_status s = gemm_bf16(c, wo, c->pf_attn, c->pf_res, h, c->qd, T, true, st)) return s;
+            if (m1moe_status s = launch_pdl(m1::k_rmsnorm, dim3(T), dim3(256), 0, st, "k_rmsnorm launch",
+                                            (const void *)c->pf_res, 0, post_norm, (float)g.rms_norm_eps, c->pf_hmid, h))
+                return s;
+            if (m1moe_status s = m1moe_cuda_moe_prefill(moe, L, c->pf_hmid, M1MOE_DTYPE_F32, c->pf_res,
+                                                        M1MOE_DTYPE_F32, c->pf_res, M1MOE_DTYPE_F32, T, nullptr,
+                                                        nullptr, stream))
+                return s;
+        }
+    }
+    // 4. each sequence's last new token: final norm and LM head
+    if (m1moe_status s = m1abi::paged_last_rows(cfg, d_plan, c->pf_res, h, c->pg_last, st)) return s;
+    if (B <= m1::kDenseMaxTok) {
+        m1::GemvParams lm{};
+        lm.w = c->lm_head;
+        lm.rows = g.vocab_size;
+        lm.K = h;
+        lm.x = c->pg_last;
+        lm.norm_w = c->final_norm;
+        lm.eps = g.rms_norm_eps;
+        lm.y = d_logits;
+        lm.ntok = B;
+        lm.err = c->err;
+        return gemv<m1::kEpiStore>(lm, c->num_sms, st);
+    }
+    if (m1moe_status s = launch_pdl(m1::k_rmsnorm_bf16, dim3(B), dim3(256), 0, st, "k_rmsnorm_bf16 launch",
+                                    (const float *)c->pg_last, (const uint16_t *)c->final_norm, (float)g.rms_norm_eps,
+                                    c->pg_last_n, h))
+        return s;
+    return gemm_bf16(c, c->lm_head, c->pg_last_n, d_logits, g.vocab_size, h, B, false, st);
 }
 
 }  // extern "C"

@@ -57,6 +57,7 @@ m1moe_status cuda_fail(cudaError_t e, const char *what) {
 void count_launch() { g_launches.fetch_add(1, std::memory_order_relaxed); }
 
 m1moe_status moe_compatible(const m1moe_cuda_ctx *moe, int hidden, int layers, int batch, int device);
+int moe_max_batch(const m1moe_cuda_ctx *moe);
 
 }  // namespace m1abi
 
@@ -743,6 +744,8 @@ m1moe_status pf_gemm(m1moe_cuda_ctx *c, const m1::PrefillParams &p, const CUtens
 }
 
 }  // namespace
+
+int m1abi::moe_max_batch(const m1moe_cuda_ctx *c) { return c->cfg.max_batch; }
 
 m1moe_status m1abi::moe_compatible(const m1moe_cuda_ctx *c, int hidden, int layers, int batch,
                                    int device) {

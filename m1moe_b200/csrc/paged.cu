@@ -19,6 +19,8 @@ namespace m1abi {
 m1moe_status fail(m1moe_status st, const char *fmt, ...);
 m1moe_status cuda_fail(cudaError_t e, const char *what);
 void count_launch();
+m1moe_status paged_last_rows(const m1moe_paged_cfg *cfg, void *d_plan, const float *x, int h, float *out,
+                             cudaStream_t st);
 }  // namespace m1abi
 
 using m1abi::cuda_fail;
@@ -263,6 +265,14 @@ m1moe_status attention(const Plan &p, m1::RowsParams a, cudaStream_t st) {
 }
 
 }  // namespace
+
+// The last new token's row of each sequence (for dense.cu).
+m1moe_status m1abi::paged_last_rows(const m1moe_paged_cfg *cfg, void *d_plan, const float *x, int h, float *out,
+                                    cudaStream_t st) {
+    Plan p;
+    if (m1moe_status e = open_plan(cfg, d_plan, p)) return e;
+    return launch_pdl(m1::k_paged_last, dim3(p.s.num_seqs), dim3(256), 0, st, "k_paged_last launch", p.v, x, h, out);
+}
 
 extern "C" {
 

@@ -289,6 +289,14 @@ __global__ void __launch_bounds__(256) k_paged_tokens(const PagedShape s, const 
     p.tokens[t] = v;
 }
 
+// out[b] = x[last new token of sequence b] (f32 rows of h), zeros without one.
+__global__ void __launch_bounds__(256) k_paged_last(const PagedPlanView p, const float *x, int h, float *out) {
+    pdl_wait();
+    const int b = blockIdx.x, t = p.cu_q[b + 1] - 1;
+    const bool any = t >= p.cu_q[b];
+    for (int i = threadIdx.x; i < h; i += 256) out[(long long)b * h + i] = any ? x[(long long)t * h + i] : 0.f;
+}
+
 // ----------------------------------------------------------------- append ----
 struct AppendParams {
     const void *qkv;

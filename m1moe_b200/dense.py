@@ -154,6 +154,28 @@ class DenseModel:
                   _stream(stream))
         return next_tokens
 
+    def paged_step(self, moe, cache, batch, tokens: torch.Tensor, *, rope: torch.Tensor,
+                   logits: torch.Tensor | None = None, stream=None) -> torch.Tensor:
+        """One step of a ragged batch (paged.PagedBatch) over a paged cache: the new tokens
+        [total_q] (int32, CUDA) through every layer; returns f32 logits [sequences][vocab] of each
+        sequence's last new token, for sampling.sample.  rope: paged.rope_table."""
+        if tokens.shape != (batch.total_q,) or tokens.dtype != torch.int32:
+            raise ValueError(f"tokens: int32 [{batch.total_q}]")
+        if cache.num_layers != self.num_layers:
+            raise ValueError(f"the cache has {cache.num_layers} layers, the model {self.num_layers}")
+        if rope.dim() != 3 or rope.dtype != torch.float32 or rope.shape[2] != 2:
+            raise ValueError("rope: float32 [positions][rot/2][2]")
+        if logits is None:
+            logits = torch.empty((batch.num_seqs, self.vocab_size), dtype=torch.float32, device=tokens.device)
+        elif logits.shape != (batch.num_seqs, self.vocab_size) or logits.dtype != torch.float32:
+            raise ValueError(f"logits: float32 ({batch.num_seqs}, {self.vocab_size})")
+        _check_cuda(tokens, rope, logits)
+        k, v = cache._ptrs(0)
+        _lib.call("m1moe_cuda_paged_step", self._ctx, moe._ctx, batch._cfg, batch._plan, batch._table, k, v,
+                  rope.data_ptr(), rope.shape[0], 2 * rope.shape[1], tokens.data_ptr(), logits.data_ptr(),
+                  batch._use(stream))
+        return logits
+
 
 def _from_ptr(ptr: int, n: int, device: int) -> torch.Tensor:
     """A torch bf16 view of n elements of device memory that the library owns
