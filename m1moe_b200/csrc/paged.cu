@@ -115,10 +115,10 @@ m1moe_status make_shape(const m1moe_paged_cfg *c, int ctas, m1::PagedShape &s) {
     s.unit = small ? m1::kPagedUnitSmall : m1::kPagedUnitLarge;
     s.workers = small ? ctas * m1::kPagedWarps : ctas;
     s.min_per = small ? m1::kPagedWarps : 1;
-    s.prefix = small && c->window == 0 ? c->shared_prefix : 0;
+    s.prefix = small && c->window == 0 && c->total_q * group >= 40 ? c->shared_prefix : 0;
     const long long items = c->num_seqs + (long long)c->total_q * group / s.rows;
     const long long cap = (long long)c->max_pages_per_seq * c->page_size;
-    if (items * (cap / s.unit + 1) * c->num_kv_heads > 0x7FFFFFFFLL)
+    if (items * (cap / s.unit + 1 + m1::kPagedItemCost) * c->num_kv_heads > 0x7FFFFFFFLL)
         return fail(M1MOE_ERR_UNSUPPORTED, "the batch's work (%lld items of up to %lld positions) does not fit 31 bits",
                     items, cap);
     s.max_items = (int)items;

@@ -41,6 +41,10 @@ constexpr int kPagedRowsSmall = 16; // rows of an item there: one m16n8k16 tile
 constexpr int kPagedUnitSmall = 16; // positions of a unit there
 constexpr int kPagedRowsLarge = 256; // rows of an item of the 256-row kernel: two M-tiles of 128
 constexpr int kPagedUnitLarge = 128; // positions of a unit there: one K or V tile
+// Units that the split adds to each item of the 256-row kernel for what an
+// item costs besides its tiles (rows in and out, the pipeline's start and
+// end: about 9,500 cycles beside 4,300 for a unit).
+constexpr int kPagedItemCost = 2;
 
 // Words of the plan's header.
 enum PagedHeader {
@@ -222,7 +226,7 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
             if (s.window > 0) lo = max(lo, first - s.window + 1);
             it.unit0 = max(lo, 0) / s.unit;
             // at least one unit, so that an item whose rows see nothing is still written
-            n = max(1, (last + s.unit) / s.unit - it.unit0);
+            n = max(1, (last + s.unit) / s.unit - it.unit0) + (s.rows == kPagedRowsLarge ? kPagedItemCost : 0);
             p.items[i] = it;
         }
         int total;
@@ -257,7 +261,7 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
     // its positions (no items when it is not shared after all)
     const int rows = s.total_q * s.group;
     const int items2 = prefix ? (rows + kPagedRowsLarge - 1) / kPagedRowsLarge : 0;
-    const int n2 = (prefix + kPagedUnitLarge - 1) / kPagedUnitLarge, units2 = items2 * n2;
+    const int n2 = (prefix + kPagedUnitLarge - 1) / kPagedUnitLarge + kPagedItemCost, units2 = items2 * n2;
     for (int i = tid; i <= items2; i += 1024) {
         p2.unit_at[i] = i * n2;
         if (i < items2)

@@ -53,6 +53,7 @@ struct Rows256 {
     static constexpr int kHalves = HD / 64;                    // 128-byte columns of a tile
     static constexpr int kTile = 128 * HD * 2;                 // bytes of a Q M-tile, K tile or V tile
     static constexpr int kStages = HD == 128 ? 4 : 8;
+    static constexpr int kPairs = kStages / 2;  // V of a tile and K of the next are given back together
     static constexpr int kStageOut = 8 * 1024;                  // 32 rows of 32 bytes a softmax warp, for the output
     static constexpr int kSmem = (2 + kStages) * kTile + kStageOut + 1024;
 };
@@ -277,18 +278,26 @@ struct Rows256Walk {
     }
     __device__ __forceinline__ bool next(const PagedShape &s, const PagedPlanView &p, const Rows256Params &a,
                                          Rows256Segment &x) {
-        if (u >= end) return false;
-        const PagedItem it = p.items[item];
-        x.g = g;
-        x.item = item;
-        x.seg0 = g * units + p.unit_at[item];
-        x.seg1 = g * units + p.unit_at[item + 1];
-        x.u0 = u;
-        x.u1 = min(end, x.seg1);
+        PagedItem it;
+        for (;;) {
+            if (u >= end) return false;
+            it = p.items[item];
+            x.g = g;
+            x.item = item;
+            // (the item's first kPagedItemCost units stand for its overhead; a run
+            // that ends in them leaves the item to the next CTA)
+            x.seg0 = g * units + p.unit_at[item] + kPagedItemCost;
+            x.seg1 = g * units + p.unit_at[item + 1];
+            x.u0 = max(u, x.seg0);
+            x.u1 = min(end, x.seg1);
+            u = x.u1;
+            if (u == x.seg1 && ++item == items) item = 0, ++g;
+            if (x.u0 < x.u1) break;
+        }
         x.seq = it.seq;
         x.row0 = it.row0;
         x.nrows = it.nrows;
-        x.ja = it.unit0 + u - x.seg0;
+        x.ja = it.unit0 + x.u0 - x.seg0;
         x.jb = it.unit0 + x.u1 - x.seg0;
         if (a.prefix_run) {
             x.q0 = 0;
@@ -301,8 +310,6 @@ struct Rows256Walk {
             x.first = x.len - (p.cu_q[it.seq + 1] - x.q0);
             x.lo = s.window > 0 ? max(0, x.first + fdiv(it.row0, s.by_group) - s.window + 1) : 0;
         }
-        u = x.u1;
-        if (u == x.seg1 && ++item == items) item = 0, ++g;
         // the next item's record, for the next call
         asm volatile("prefetch.global.L1 [%0];" ::"l"(p.items + item));
         asm volatile("prefetch.global.L1 [%0];" ::"l"(p.unit_at + item + 1));
@@ -317,7 +324,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                                                                       const __grid_constant__ CUtensorMap vmap) {
     using T = Rows256<HD>;
     extern __shared__ uint8_t raw[];
-    __shared__ uint64_t kv_full[T::kStages], kv_empty[T::kStages], q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2], drain;
+    __shared__ uint64_t kv_full[T::kStages], kv_empty[T::kPairs], q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2], drain;
     __shared__ uint32_t tmem_base;
     __shared__ int abort_flag, sm_last[2];
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
@@ -328,7 +335,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
     if (threadIdx.x == 0) {
         for (int i = 0; i < T::kStages; ++i) {
             mbar_init(&kv_full[i], kRows256Loaders);
-            mbar_init(&kv_empty[i], 1);
+            if (i < T::kPairs) mbar_init(&kv_empty[i], 1);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&q_full[i], kRows256Loaders);
@@ -348,7 +355,13 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
     }
     __syncthreads();
     tc_fence_after_sync();
-    const uint32_t tmem = tmem_base;
+    // All 512 columns are this block's, so they start at address 0, which lets
+    // the products' operands be constants.
+    constexpr uint32_t tmem = 0;
+    if (threadIdx.x == 0 && tmem_base != 0) {
+        abort_flag = 1;
+        atomicOr(p.status, kPagedErrWait);
+    }
     pdl_wait();
     Rows256Walk walk;
     walk.start(s, p, blockIdx.x);
@@ -367,8 +380,10 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
         bool ok = true;
         auto claim = [&]() {  // the next tile's stage, free
             const int st = tile % T::kStages;
+            // its last tile, tile - kStages, went with pair (tile - kStages + 1) / 2
+            const int pair = (tile - T::kStages + 1) / 2;
             if (ok && tile >= T::kStages)
-                ok = paged_wait(&kv_empty[st], ((tile / T::kStages) - 1) & 1, &abort_flag, status);
+                ok = paged_wait(&kv_empty[pair % T::kPairs], (pair / T::kPairs) & 1, &abort_flag, status);
             ok = __all_sync(0xffffffffu, ok);
             ++tile;
             return st;
@@ -474,16 +489,11 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             const uint32_t v_lo = umma_desc_lo(smem_addr(skv), 16384);
             uint32_t phase = 0;  // bits 0, 1: next parity of q_full; 2, 3: of p_full
             bool ok = true;
+            // (only the elected lane's `ok` counts; the others keep it company)
             auto wait = [&](uint64_t *bar, uint32_t parity) {
                 if (ok) ok = paged_wait(bar, parity & 1, &abort_flag, status);
-                ok = __all_sync(0xffffffffu, ok);
-                tc_fence_after_sync();
             };
             auto wait_kv = [&](int n) { wait(&kv_full[n % T::kStages], n / T::kStages); };
-            auto release = [&](int n) {
-                if (ok && elected) umma_commit(&kv_empty[n % T::kStages]);
-                __syncwarp();
-            };
             // Tile after tile, across segments: S of the next tile (the next
             // segment's first one, while this one's rows are still being
             // finished) goes behind each P V.  The first turn has no P V.
@@ -493,48 +503,47 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             bool begun = false;
             while (more || j < tiles) {
                 const bool ends = j + 1 == tiles;
-                if (tile >= 0) wait_kv(tile + 1);
                 const int next_tiles = x.jb - x.ja, next_both = more && x.nrows > kTileRows;
                 const bool follows = !ends || more;
-                bool have_k = false;
-#pragma unroll 1
+                // both tiles first: nothing then stands between the weights and the products
+                if (tile >= 0) wait_kv(tile + 1);
+                if (follows) wait_kv(tile + 2);
+                const uint32_t v_off = uniform(((tile + 1) % T::kStages) * (T::kTile >> 4));
+                const uint32_t k_off = uniform(((tile + 2) % T::kStages) * (T::kTile >> 4));
+#pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     if (begun && (i == 0 || both)) {  // O_i += P_i V
                         wait(&p_full[i], phase >> (2 + i));
+                        tc_fence_after_sync();
                         phase ^= 4u << i;
-                        const uint32_t off = uniform(((tile + 1) % T::kStages) * (T::kTile >> 4));
-                        const uint32_t d = uniform(tmem + 256 + i * 128), pa = uniform(tmem + i * 128);
                         if (ok && elected) {
 #pragma unroll
                             for (int k = 0; k < 8; ++k)
-                                umma_bf16_ts(d, pa + 8 * k, v_lo + off + k * (2048 >> 4), kIdPV, !(j == 0 && k == 0));
-                            umma_commit(&o_done[i]);
+                                umma_bf16_ts(256 + i * 128, i * 128 + 8 * k, v_lo + v_off + k * (2048 >> 4), kIdPV,
+                                             !(j == 0 && k == 0));
+                            // (before that, the next scores' commit tells that O is up to date)
+                            if (ends) umma_commit(&o_done[i]);
                         }
-                        __syncwarp();
                     }
                     if (follows && (i == 0 || (ends ? next_both : both))) {  // S_i = Q_i K^T
-                        if (!have_k) wait_kv(tile + 2), have_k = true;
                         if (ends) {
                             wait(&q_full[i], phase >> i);
                             phase ^= 1u << i;
                         }
-                        const uint32_t off = uniform(((tile + 2) % T::kStages) * (T::kTile >> 4));
-                        const uint32_t d = uniform(tmem + i * 128), qa = uniform(q_lo + i * (T::kTile >> 4));
                         if (ok && elected) {
 #pragma unroll
                             for (int k = 0; k < HD / 16; ++k) {
                                 const uint32_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                                umma_bf16_ss(d, qa + step, k_lo + off + step, kIdQK, k > 0);
+                                umma_bf16_ss(i * 128, q_lo + i * (T::kTile >> 4) + step, k_lo + k_off + step, kIdQK, k > 0);
                             }
                             umma_commit(&s_full[i]);
                             // the segment's last scores: the next one's rows may come
                             if (ends ? next_tiles == 1 : j + 2 == tiles) umma_commit(&q_empty[i]);
                         }
-                        __syncwarp();
                     }
                 }
-                if (tile >= 0) release(tile + 1);
-                if (follows) release(tile + 2);
+                // V of this turn and K of the next are done with together
+                if (ok && elected) umma_commit(&kv_empty[(tile + 2) / 2 % T::kPairs]);
                 tile += 2;
                 if (!ends) {
                     ++j;
@@ -563,7 +572,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
         const bool capped = a.r.cap > 0.f;
         const float mult = capped ? 1.f : a.r.scale * kLog2e;
         uint8_t *stage = sout + warp * 1024;
-        int ns = 0;  // score tiles so far
+        int ns = 0, nseg = 0;  // score tiles, segments so far
         bool ok = true;
         while (walk.next(s, p, a, x)) {
             const int n = min(kTileRows, x.nrows - i * kTileRows);  // rows of this M-tile
@@ -633,10 +642,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                     }
                     // j > a: the products of the tiles before are in O
                     if (__any_sync(0xffffffffu, grow) && j > x.ja) {
-                        if (ok) ok = paged_wait(&o_done[i], (ns - 1) & 1, &abort_flag, status);
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (ok) {
-                            tc_fence_after_sync();
+                        {  // (these scores' products came after those of P V)
 #pragma unroll 1
                             for (int q = 0; q < HD / 16; ++q) {
                                 uint32_t y[16];
@@ -658,7 +664,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 ++ns;
             }
             // ------------------------------------------------ the segment's end
-            if (ok) ok = paged_wait(&o_done[i], (ns - 1) & 1, &abort_flag, status);
+            if (ok) ok = paged_wait(&o_done[i], nseg++ & 1, &abort_flag, status);
             ok = __all_sync(0xffffffffu, ok);
             if (ok) tc_fence_after_sync();
             const bool whole = x.u0 == x.seg0 && x.u1 == x.seg1;
@@ -744,9 +750,9 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 if (sm_last[i]) {
                     __threadfence();
                     mm = -INFINITY, ll = 0.f;
-#pragma unroll 1
-                    for (int c = first; live && c <= last; ++c) {
-                        const float2 v = __ldcg(part_ml_at(slot_of(c)));
+#pragma unroll 4
+                    for (int c = first; c <= last; ++c) {
+                        const float2 v = live ? __ldcg(part_ml_at(slot_of(c))) : make_float2(-INFINITY, 0.f);
                         const float mn = fmaxf(mm, v.x);
                         if (mn != -INFINITY) ll = ll * exp2_approx(mm - mn) + v.y * exp2_approx(v.x - mn);
                         mm = mn;
@@ -763,19 +769,32 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                     } else {
 #pragma unroll
                         for (int e = 0; e < 16; ++e) o[e] = 0.f;
+                        // four partials' loads under way together
 #pragma unroll 1
-                        for (int c = first; live && c <= last; ++c) {
-                            const float2 v = __ldcg(part_ml_at(slot_of(c)));
-                            if (v.x == -INFINITY) continue;
-                            const float w = exp2_approx(v.x - mm);
-                            const float4 *d = part_at(slot_of(c)) + 4 * q * kTileRows;
+                        for (int c0 = first; c0 <= last; c0 += 4) {
+                            float4 y[4][4];
+                            float w[4];
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
-                                const float4 y = __ldcg(d + e * kTileRows);
-                                o[4 * e] = fmaf(y.x, w, o[4 * e]);
-                                o[4 * e + 1] = fmaf(y.y, w, o[4 * e + 1]);
-                                o[4 * e + 2] = fmaf(y.z, w, o[4 * e + 2]);
-                                o[4 * e + 3] = fmaf(y.w, w, o[4 * e + 3]);
+                            for (int k = 0; k < 4; ++k) {
+                                const int c = min(c0 + k, last);
+                                w[k] = -INFINITY;
+                                if (live && c0 + k <= last) w[k] = __ldcg(part_ml_at(slot_of(c))).x;
+                                const float4 *d = part_at(slot_of(c)) + 4 * q * kTileRows;
+#pragma unroll
+                                for (int e = 0; e < 4; ++e)
+                                    y[k][e] = live ? __ldcg(d + e * kTileRows) : make_float4(0.f, 0.f, 0.f, 0.f);
+                            }
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) {
+                                if (w[k] == -INFINITY) continue;  // saw nothing (or is none)
+                                const float g = exp2_approx(w[k] - mm);
+#pragma unroll
+                                for (int e = 0; e < 4; ++e) {
+                                    o[4 * e] = fmaf(y[k][e].x, g, o[4 * e]);
+                                    o[4 * e + 1] = fmaf(y[k][e].y, g, o[4 * e + 1]);
+                                    o[4 * e + 2] = fmaf(y[k][e].z, g, o[4 * e + 2]);
+                                    o[4 * e + 3] = fmaf(y[k][e].w, g, o[4 * e + 3]);
+                                }
                             }
                         }
                         __syncwarp();
@@ -791,7 +810,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
     __syncthreads();
     if (warp == 12) {
         tc_fence_after_sync();
-        tmem_dealloc(tmem, 512);
+        tmem_dealloc(tmem_base, 512);
     }
 }
 
