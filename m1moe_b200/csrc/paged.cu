@@ -148,7 +148,7 @@ size_t plan_view(const m1::PagedShape &s, void *base, m1::PagedPlanView &v, m1::
     take(v.item_at, (size_t)(s.num_seqs + 1) * 4);
     take(v.unit_at, (size_t)(s.max_items + 1) * 4);
     take(v.start, (size_t)s.workers * 4);
-    take(v.count, (size_t)s.nkv * s.max_items * 4 * (large ? 2 : 1));
+    take(v.count, large ? 0 : (size_t)s.nkv * s.max_items * 4);
     take(v.part_ml, (size_t)2 * s.ctas * part_rows * 8);
     take(v.part, (size_t)2 * s.ctas * part_rows * s.hd * 4);
     v2 = v;
@@ -158,7 +158,6 @@ size_t plan_view(const m1::PagedShape &s, void *base, m1::PagedPlanView &v, m1::
     take(v2.items, items2 * sizeof(m1::PagedItem));
     take(v2.unit_at, (items2 + 1) * 4);
     take(v2.start, (size_t)s.ctas * 4);
-    take(v2.count, (size_t)s.nkv * items2 * 2 * 4);
     take(v2.part_ml, (size_t)2 * s.ctas * m1::kPagedRowsLarge * 8);
     take(v2.part, (size_t)2 * s.ctas * m1::kPagedRowsLarge * s.hd * 4);
     take(pre.ml, (size_t)s.total_q * s.nh * 8);
@@ -236,8 +235,11 @@ m1moe_status launch_rows256(const m1::PagedShape &s, const m1::PagedPlanView &v,
     if (regs * m1::kRows256Threads < 128 * 2 * (m1::kRegsSoftmax + m1::kRegsOther))
         return fail(M1MOE_ERR_CUDA, "k_paged_rows256 was built with %d registers", regs);
     P_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-    return launch_pdl(kern, dim3(s.ctas), dim3(m1::kRows256Threads), (size_t)smem, st, "k_paged_rows256 launch", s, v, a,
-                      kmap, vmap);
+    if (m1moe_status e = launch_pdl(kern, dim3(s.ctas), dim3(m1::kRows256Threads), (size_t)smem, st,
+                                    "k_paged_rows256 launch", s, v, a, kmap, vmap))
+        return e;
+    return launch_pdl(m1::k_paged_join<HD>, dim3(std::max(1, s.ctas - 1), 2, HD / 32), dim3(m1::kTileRows), 0, st,
+                      "k_paged_join launch", s, v, a);
 }
 
 template <int HD>

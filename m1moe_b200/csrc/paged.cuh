@@ -16,9 +16,11 @@
 // the number of position units its rows can see; the units of all KV heads'
 // items, concatenated, are cut into equal runs, one per CTA (and, for the
 // 16-row kernel, per warp), whatever the lengths are.  A run that starts or
-// ends inside an item leaves a partial (maximum, sum, weighted values); the
-// last CTA to finish an item merges its partials in position order, so the
-// result does not depend on which one that is.
+// ends inside an item leaves a partial (maximum, sum, weighted values); an
+// item's partials are merged in position order -- by the last CTA to finish
+// it (16 rows) or by a kernel that follows (256 rows: one CTA would read them
+// for longer than the launch takes) -- so the result does not depend on the
+// order of events.
 #pragma once
 
 #include <cuda_bf16.h>
@@ -72,7 +74,7 @@ struct PagedPlanView {
     int *item_at;        // [B + 1]: first item of each sequence
     int *unit_at;        // [max_items + 1]: units before each item
     int *start;          // [workers]: the item each worker starts in
-    int *count;          // [nkv * max_items] (two each, 256-row kernel): partials that have arrived
+    int *count;          // [nkv * max_items], 16-row kernel: partials that have arrived
     float *part;         // [2 * ctas][rows][hd] weighted values
     float2 *part_ml;     // [2 * ctas][rows] maximum and sum
 };
@@ -235,8 +237,7 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
         units += total;
     }
     if (tid == 0) p.unit_at[items] = units;
-    const int tiles = s.rows == kPagedRowsLarge ? 2 : 1;
-    for (int i = tid; i < items * s.nkv * tiles; i += 1024) p.count[i] = 0;
+    for (int i = tid; s.rows == kPagedRowsSmall && i < items * s.nkv; i += 1024) p.count[i] = 0;
     __syncthreads();
     const long long all = (long long)units * s.nkv;
     const int per = (int)max((long long)s.min_per, (all + s.ctas - 1) / s.ctas);
@@ -267,7 +268,6 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
         if (i < items2)
             p2.items[i] = PagedItem{lead, i * kPagedRowsLarge, min(kPagedRowsLarge, rows - i * kPagedRowsLarge), 0};
     }
-    for (int i = tid; i < items2 * s.nkv * 2; i += 1024) p2.count[i] = 0;
     const int all2 = units2 * s.nkv, per2 = max(1, (all2 + s.ctas - 1) / s.ctas);
     for (int c = tid; c < s.ctas; c += 1024) p2.start[c] = c * per2 < all2 ? (c * per2) % units2 / n2 : 0;
     if (tid == 0) {

@@ -326,7 +326,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
     extern __shared__ uint8_t raw[];
     __shared__ uint64_t kv_full[T::kStages], kv_empty[T::kPairs], q_full[2], q_empty[2], s_full[2], p_full[2], o_done[2], drain;
     __shared__ uint32_t tmem_base;
-    __shared__ int abort_flag, sm_last[2];
+    __shared__ int abort_flag;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
     uint8_t *sq = smem, *skv = smem + 2 * T::kTile;
     uint8_t *sout = skv + T::kStages * T::kTile;
@@ -712,10 +712,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             };
             auto part_ml_at = [&](int slot) { return p.part_ml + ((size_t)slot * 2 + i) * kTileRows + row; };
             const int slot = 2 * blockIdx.x + (x.u0 == x.seg0 ? 1 : 0);
-            float mm = m == -INFINITY ? m : m * mult, ll = l;  // the row's maximum (log2 scale) and sum
-            const int per = p.header[kPhPer];
-            const int first = x.seg0 / per, last = (x.seg1 - 1) / per;
-            auto slot_of = [&](int c) { return 2 * c + (c == first ? 1 : 0); };
+            const float mm = m == -INFINITY ? m : m * mult, ll = l;  // the row's maximum (log2 scale) and sum
             auto read_o = [&](int q, float (&o)[16]) {  // 16 columns of O
                 uint32_t v[16];
 #pragma unroll
@@ -727,81 +724,25 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
 #pragma unroll
                 for (int e = 0; e < 16; ++e) o[e] = __uint_as_float(v[e]);
             };
-            if (!whole) {
+            const float f = a.prefix_run ? 1.f : ll == 0.f ? 0.f : 1.f / ll;
 #pragma unroll 1
-                for (int q = 0; q < HD / 16; ++q) {
-                    float o[16];
-                    read_o(q, o);
+            for (int q = 0; q < HD / 16; ++q) {
+                float o[16];
+                read_o(q, o);
+                if (whole) {
+                    put(f, 16 * q, o);
+                } else if (live) {
                     float4 *d = part_at(slot) + 4 * q * kTileRows;
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
-                        if (live) d[e * kTileRows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-                }
-                if (live) *part_ml_at(slot) = make_float2(mm, ll);
-                // the last one of the item's CTAs joins its partials, in position order
-                __threadfence();
-                named_sync(1 + i, kTileRows);
-                if (row == 0) {
-                    int *cnt = p.count + ((size_t)x.g * walk.items + x.item) * 2 + i;
-                    sm_last[i] = atomicAdd(cnt, 1) == last - first;
-                    if (sm_last[i]) *cnt = 0;  // ready for the next call
-                }
-                named_sync(1 + i, kTileRows);
-                if (sm_last[i]) {
-                    __threadfence();
-                    mm = -INFINITY, ll = 0.f;
-#pragma unroll 4
-                    for (int c = first; c <= last; ++c) {
-                        const float2 v = live ? __ldcg(part_ml_at(slot_of(c))) : make_float2(-INFINITY, 0.f);
-                        const float mn = fmaxf(mm, v.x);
-                        if (mn != -INFINITY) ll = ll * exp2_approx(mm - mn) + v.y * exp2_approx(v.x - mn);
-                        mm = mn;
-                    }
+                        d[e * kTileRows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
             }
-            if (whole || sm_last[i]) {
-                const float f = a.prefix_run ? 1.f : ll == 0.f ? 0.f : 1.f / ll;
-#pragma unroll 1
-                for (int q = 0; q < HD / 16; ++q) {
-                    float o[16];
-                    if (whole) {
-                        read_o(q, o);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] = 0.f;
-                        // four partials' loads under way together
-#pragma unroll 1
-                        for (int c0 = first; c0 <= last; c0 += 4) {
-                            float4 y[4][4];
-                            float w[4];
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                const int c = min(c0 + k, last);
-                                w[k] = -INFINITY;
-                                if (live && c0 + k <= last) w[k] = __ldcg(part_ml_at(slot_of(c))).x;
-                                const float4 *d = part_at(slot_of(c)) + 4 * q * kTileRows;
-#pragma unroll
-                                for (int e = 0; e < 4; ++e)
-                                    y[k][e] = live ? __ldcg(d + e * kTileRows) : make_float4(0.f, 0.f, 0.f, 0.f);
-                            }
-#pragma unroll
-                            for (int k = 0; k < 4; ++k) {
-                                if (w[k] == -INFINITY) continue;  // saw nothing (or is none)
-                                const float g = exp2_approx(w[k] - mm);
-#pragma unroll
-                                for (int e = 0; e < 4; ++e) {
-                                    o[4 * e] = fmaf(y[k][e].x, g, o[4 * e]);
-                                    o[4 * e + 1] = fmaf(y[k][e].y, g, o[4 * e + 1]);
-                                    o[4 * e + 2] = fmaf(y[k][e].z, g, o[4 * e + 2]);
-                                    o[4 * e + 3] = fmaf(y[k][e].w, g, o[4 * e + 3]);
-                                }
-                            }
-                        }
-                        __syncwarp();
-                    }
-                    put(f, 16 * q, o);
-                }
-                if (live && a.prefix_run) a.partial_ml[token * s.nh + head] = make_float2(mm, ll);
+            if (live) {
+                if (!whole)
+                    *part_ml_at(slot) = make_float2(mm, ll);
+                else if (a.prefix_run)
+                    a.partial_ml[token * s.nh + head] = make_float2(mm, ll);
             }
             if (ok) tc_fence_before_sync();
         }
@@ -811,6 +752,70 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
     if (warp == 12) {
         tc_fence_after_sync();
         tmem_dealloc(tmem_base, 512);
+    }
+}
+
+// The items that the split cut: block (c, M-tile, 32 columns) joins, in
+// position order, the partials of the item that begins in CTA c's run and
+// does not end there (a run begins at most one such item).  A thread a row.
+template <int HD>
+__global__ void __launch_bounds__(kTileRows) k_paged_join(const PagedShape s, const PagedPlanView p,
+                                                          const Rows256Params a) {
+    pdl_wait();
+    const int c = blockIdx.x, i = blockIdx.y, col = 32 * blockIdx.z, row = threadIdx.x;
+    const int units = p.header[kPhUnits], per = p.header[kPhPer];
+    const int all = units * s.nkv, cut = (c + 1) * per;
+    if ((long long)(c + 1) * per >= all) return;
+    const int g = cut / units, item = p.start[c + 1];
+    const PagedItem it = p.items[item];
+    const int seg0 = g * units + p.unit_at[item] + kPagedItemCost, seg1 = g * units + p.unit_at[item + 1];
+    if (seg0 >= cut || seg0 / per != c) return;  // it begins later, or began before
+    const int last = (seg1 - 1) / per, n = min(kTileRows, it.nrows - i * kTileRows);
+    if (row >= n) return;
+    const size_t tile = (size_t)kTileRows * (HD / 4);
+    const float4 *part = reinterpret_cast<const float4 *>(p.part) + i * tile + (size_t)(col / 4) * kTileRows + row;
+    const float2 *ml = p.part_ml + (size_t)i * kTileRows + row;
+    auto slot_of = [&](int k) { return (size_t)(2 * k + (k == c ? 1 : 0)) * 2; };  // in M-tiles
+    float m = -INFINITY, l = 0.f, o[32];
+#pragma unroll
+    for (int e = 0; e < 32; ++e) o[e] = 0.f;
+#pragma unroll 2
+    for (int k = c; k <= last; ++k) {
+        const float2 v = ml[slot_of(k) * kTileRows];
+        const float4 *d = part + slot_of(k) * tile;
+        float4 y[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = d[e * kTileRows];
+        const float mn = fmaxf(m, v.x), f = mn == -INFINITY ? 0.f : exp2_approx(m - mn);
+        const float w = v.x == -INFINITY ? 0.f : exp2_approx(v.x - mn);
+        l = l * f + v.y * w;
+        m = mn;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            o[4 * e] = o[4 * e] * f + y[e].x * w;
+            o[4 * e + 1] = o[4 * e + 1] * f + y[e].y * w;
+            o[4 * e + 2] = o[4 * e + 2] * f + y[e].z * w;
+            o[4 * e + 3] = o[4 * e + 3] * f + y[e].w * w;
+        }
+    }
+    const int r = it.row0 + i * kTileRows + row, tok = fdiv(r, s.by_group), head = g * s.group + r - tok * s.group;
+    const long long token = (a.prefix_run ? 0 : p.cu_q[it.seq]) + tok;
+    if (!a.prefix_run && a.r.out_bf16) {
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        uint16_t *d = reinterpret_cast<uint16_t *>(a.r.out) + token * a.r.out_stride + (long long)head * HD + col;
+#pragma unroll
+        for (int e = 0; e < 32; e += 8)
+            *reinterpret_cast<uint4 *>(d + e) =
+                make_uint4(pack_bf16(o[e] * f, o[e + 1] * f), pack_bf16(o[e + 2] * f, o[e + 3] * f),
+                           pack_bf16(o[e + 4] * f, o[e + 5] * f), pack_bf16(o[e + 6] * f, o[e + 7] * f));
+    } else {
+        const float f = a.prefix_run ? 1.f : l == 0.f ? 0.f : 1.f / l;
+        float *d = a.prefix_run ? a.partial + (token * s.nh + head) * HD + col
+                                : reinterpret_cast<float *>(a.r.out) + token * a.r.out_stride + (long long)head * HD + col;
+#pragma unroll
+        for (int e = 0; e < 32; e += 4)
+            *reinterpret_cast<float4 *>(d + e) = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
+        if (a.prefix_run && col == 0) a.partial_ml[token * s.nh + head] = make_float2(m, l);
     }
 }
 
