@@ -33,6 +33,8 @@
 // there), sums are fp32.
 #pragma once
 
+#include <type_traits>
+
 #include "paged_rows16.cuh"
 #include "umma.cuh"
 
@@ -52,7 +54,7 @@ template <int HD>
 struct Rows256 {
     static constexpr int kHalves = HD / 64;                    // 128-byte columns of a tile
     static constexpr int kTile = 128 * HD * 2;                 // bytes of a Q M-tile, K tile or V tile
-    static constexpr int kStages = HD == 128 ? 4 : 8;
+    static constexpr int kStages = 4;  // the products' turns are written out for four
     static constexpr int kPairs = kStages / 2;  // V of a tile and K of the next are given back together
     static constexpr int kStageOut = 8 * 1024;                  // 32 rows of 32 bytes a softmax warp, for the output
     static constexpr int kSmem = (2 + kStages) * kTile + kStageOut + 1024;
@@ -493,39 +495,41 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             auto wait = [&](uint64_t *bar, uint32_t parity) {
                 if (ok) ok = paged_wait(bar, parity & 1, &abort_flag, status);
             };
-            auto wait_kv = [&](int n) { wait(&kv_full[n % T::kStages], n / T::kStages); };
             // Tile after tile, across segments: S of the next tile (the next
             // segment's first one, while this one's rows are still being
             // finished) goes behind each P V.  The first turn has no P V.
-            // Loops stay rolled: the roles' code shares one instruction cache.
             bool more = walk.next(s, p, a, x);
             int tiles = 1, both = 0, j = 0, tile = -2;
             bool begun = false;
-            while (more || j < tiles) {
-                const bool ends = j + 1 == tiles;
+            // One turn: O_i += P_i V of a tile, S_i = Q_i K^T of the next.  kPar: the
+            // turn's parity, which fixes the stages (tile is 4 n - 2 + 2 kPar), so
+            // that operands are constants: what the issuing warp computes between
+            // two products is what the tensor cores wait for.
+            auto turn = [&](auto kPar) {
+                constexpr int vs = (2 * kPar.value + 3) % 4, ks = 2 * kPar.value % 4;
+                static_assert(T::kStages == 4, "two tiles a turn, two parities");
+                const bool ends = j + 1 == tiles, follows = !ends || more;
                 const int next_tiles = x.jb - x.ja, next_both = more && x.nrows > kTileRows;
-                const bool follows = !ends || more;
+                const bool gives_q = ends ? next_tiles == 1 : j + 2 == tiles;
                 // both tiles first: nothing then stands between the weights and the products
-                if (tile >= 0) wait_kv(tile + 1);
-                if (follows) wait_kv(tile + 2);
-                const uint32_t v_off = uniform(((tile + 1) % T::kStages) * (T::kTile >> 4));
-                const uint32_t k_off = uniform(((tile + 2) % T::kStages) * (T::kTile >> 4));
+                if (begun) wait(&kv_full[vs], (tile + 1) / 4);
+                if (follows) wait(&kv_full[ks], (tile + 2) / 4);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (begun && (i == 0 || both)) {  // O_i += P_i V
+                    if (begun && (i == 0 || both)) {
                         wait(&p_full[i], phase >> (2 + i));
                         tc_fence_after_sync();
                         phase ^= 4u << i;
                         if (ok && elected) {
 #pragma unroll
                             for (int k = 0; k < 8; ++k)
-                                umma_bf16_ts(256 + i * 128, i * 128 + 8 * k, v_lo + v_off + k * (2048 >> 4), kIdPV,
-                                             !(j == 0 && k == 0));
+                                umma_bf16_ts(256 + i * 128, i * 128 + 8 * k, v_lo + ((vs * T::kTile + k * 2048) >> 4),
+                                             kIdPV, !(j == 0 && k == 0));
                             // (before that, the next scores' commit tells that O is up to date)
                             if (ends) umma_commit(&o_done[i]);
                         }
                     }
-                    if (follows && (i == 0 || (ends ? next_both : both))) {  // S_i = Q_i K^T
+                    if (follows && (i == 0 || (ends ? next_both : both))) {
                         if (ends) {
                             wait(&q_full[i], phase >> i);
                             phase ^= 1u << i;
@@ -533,28 +537,35 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                         if (ok && elected) {
 #pragma unroll
                             for (int k = 0; k < HD / 16; ++k) {
-                                const uint32_t step = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-                                umma_bf16_ss(i * 128, q_lo + i * (T::kTile >> 4) + step, k_lo + k_off + step, kIdQK, k > 0);
+                                const uint32_t step = (k >> 2) * 16384 + (k & 3) * 32;
+                                umma_bf16_ss(i * 128, q_lo + ((i * T::kTile + step) >> 4),
+                                             k_lo + ((ks * T::kTile + step) >> 4), kIdQK, k > 0);
                             }
                             umma_commit(&s_full[i]);
                             // the segment's last scores: the next one's rows may come
-                            if (ends ? next_tiles == 1 : j + 2 == tiles) umma_commit(&q_empty[i]);
+                            if (gives_q) umma_commit(&q_empty[i]);
                         }
                     }
                 }
                 // V of this turn and K of the next are done with together
-                if (ok && elected) umma_commit(&kv_empty[(tile + 2) / 2 % T::kPairs]);
+                if (ok && elected) umma_commit(&kv_empty[kPar.value]);
                 tile += 2;
                 if (!ends) {
                     ++j;
-                } else if (more) {
+                } else {
                     tiles = next_tiles;
                     both = next_both;
                     j = 0;
                     begun = true;
+                    if (!more) return false;
                     more = walk.next(s, p, a, x);
-                } else {
-                    break;
+                }
+                return true;
+            };
+            if (more) {
+                const std::integral_constant<int, 0> even;
+                const std::integral_constant<int, 1> odd;
+                while (turn(even) && turn(odd)) {
                 }
             }
             // every product has ended before tensor memory is given back
