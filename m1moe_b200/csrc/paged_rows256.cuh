@@ -505,18 +505,21 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             // turn's parity, which fixes the stages (tile is 4 n - 2 + 2 kPar), so
             // that operands are constants: what the issuing warp computes between
             // two products is what the tensor cores wait for.
-            auto turn = [&](auto kPar) {
+            auto turn_of = [&](auto kPar, auto kMiddle) {
                 constexpr int vs = (2 * kPar.value + 3) % 4, ks = 2 * kPar.value % 4;
                 static_assert(T::kStages == 4, "two tiles a turn, two parities");
-                const bool ends = j + 1 == tiles, follows = !ends || more;
+                // (most turns are amid an item's tiles, with both M-tiles at work)
+                constexpr bool mid = kMiddle.value;
+                const bool ends = !mid && j + 1 == tiles, follows = mid || !ends || more;
                 const int next_tiles = x.jb - x.ja, next_both = more && x.nrows > kTileRows;
-                const bool gives_q = ends ? next_tiles == 1 : j + 2 == tiles;
+                const bool gives_q = !mid && (ends ? next_tiles == 1 : j + 2 == tiles);
+                const bool works = mid || begun, two = mid || both;
                 // both tiles first: nothing then stands between the weights and the products
-                if (begun) wait(&kv_full[vs], (tile + 1) / 4);
+                if (works) wait(&kv_full[vs], (tile + 1) / 4);
                 if (follows) wait(&kv_full[ks], (tile + 2) / 4);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    if (begun && (i == 0 || both)) {
+                    if (works && (i == 0 || two)) {
                         wait(&p_full[i], phase >> (2 + i));
                         tc_fence_after_sync();
                         phase ^= 4u << i;
@@ -529,7 +532,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                             if (ends) umma_commit(&o_done[i]);
                         }
                     }
-                    if (follows && (i == 0 || (ends ? next_both : both))) {
+                    if (follows && (i == 0 || (ends ? next_both : two))) {
                         if (ends) {
                             wait(&q_full[i], phase >> i);
                             phase ^= 1u << i;
@@ -561,6 +564,10 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                     more = walk.next(s, p, a, x);
                 }
                 return true;
+            };
+            auto turn = [&](auto kPar) {
+                if (begun && both && j + 2 < tiles) return turn_of(kPar, std::true_type{});
+                return turn_of(kPar, std::false_type{});
             };
             if (more) {
                 const std::integral_constant<int, 0> even;
