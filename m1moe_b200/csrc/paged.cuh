@@ -59,9 +59,12 @@ enum PagedHeader {
 };
 
 // One item: rows row0 .. row0 + nrows - 1 of sequence `seq` (row = token
-// offset * group + head offset), position units [unit0, unit0 + units).
-struct PagedItem {
+// offset * group + head offset), seen from position unit0 * unit on; and of
+// the sequence the first of its nq new tokens and its length, so that one
+// load tells all (a worker's first copies wait for every load before them).
+struct __align__(16) PagedItem {
     int seq, row0, nrows, unit0;
+    int q0, nq, len, unused;
 };
 
 struct PagedPlanView {
@@ -221,6 +224,10 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
             PagedItem it;
             it.seq = b;
             it.row0 = r0;
+            it.q0 = q0;
+            it.nq = q1 - q0;
+            it.len = t;
+            it.unused = 0;
             it.nrows = min(s.rows, nrow - r0);
             const int first = t - (q1 - q0) + r0 / s.group;  // position of the first and the last row
             const int last = t - (q1 - q0) + (r0 + it.nrows - 1) / s.group;
@@ -266,7 +273,8 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
     for (int i = tid; i <= items2; i += 1024) {
         p2.unit_at[i] = i * n2;
         if (i < items2)
-            p2.items[i] = PagedItem{lead, i * kPagedRowsLarge, min(kPagedRowsLarge, rows - i * kPagedRowsLarge), 0};
+            p2.items[i] = PagedItem{lead, i * kPagedRowsLarge, min(kPagedRowsLarge, rows - i * kPagedRowsLarge), 0,
+                                    0, s.total_q, prefix, 0};
     }
     const int all2 = units2 * s.nkv, per2 = max(1, (all2 + s.ctas - 1) / s.ctas);
     for (int c = tid; c < s.ctas; c += 1024) p2.start[c] = c * per2 < all2 ? (c * per2) % units2 / n2 : 0;

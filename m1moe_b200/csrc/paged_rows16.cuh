@@ -227,6 +227,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
     float *front = reinterpret_cast<float *>(ring + a.stages * kUnit);
     const uint32_t ring_addr = smem_addr(ring);
     pdl_wait();
+    const int start = p.start[cta * kPagedWarps + warp];
     const int units = p.header[kPhUnits], items = p.header[kPhItems], per = p.header[kPhPer];
     const int prefix = p.header[kPhPrefix];
     int *status = p.status;
@@ -241,39 +242,34 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
     Rows16Left mine = {0, 0, 0, 0, 0, 0, 0};
     if (work) {
         cur.g = cur.u / units;
-        cur.item = p.start[cta * kPagedWarps + warp];
+        cur.item = start;
         cur.locate(p, units);
         UnitCursor ld = cur;  // the loader runs ahead
         PagedItem ld_item = p.items[ld.item];
-        int ld_len = p.kv_len[ld_item.seq], ld_lo = 0;
-        auto item_lo = [&](const PagedItem &it, int len) {  // first position any row of the item sees
+        auto item_lo = [&](const PagedItem &it) {  // first position any row of the item sees
             int lo = prefix;
-            if (s.window > 0) {
-                const int first = len - (p.cu_q[it.seq + 1] - p.cu_q[it.seq]) + it.row0 / s.group;
-                lo = max(lo, first - s.window + 1);
-            }
+            if (s.window > 0) lo = max(lo, it.len - it.nq + fdiv(it.row0, s.by_group) - s.window + 1);
             return lo;
         };
-        ld_lo = item_lo(ld_item, ld_len);
+        int ld_lo = item_lo(ld_item);
         int slot = 0;
         auto load_unit = [&]() {
             if (ld.u < ld.end) {
                 if (ld.u == ld.seg1) {
                     ld.next_item(p, units, items);
                     ld_item = p.items[ld.item];
-                    ld_len = p.kv_len[ld_item.seq];
-                    ld_lo = item_lo(ld_item, ld_len);
+                    ld_lo = item_lo(ld_item);
                 }
                 const int pos = (ld_item.unit0 + ld.u - ld.seg0) * kPagedUnitSmall;
                 // all 16 positions lie in one page (page sizes are multiples of 16)
                 int row = -1;
-                if (pos < ld_len) row = paged_row(s, a.table, ld_item.seq, ld.g, pos, status);
+                if (pos < ld_item.len) row = paged_row(s, a.table, ld_item.seq, ld.g, pos, status);
                 const long long at = (long long)max(row, 0) * HD;
                 const uint32_t dst = ring_addr + slot * kUnit;
 #pragma unroll
                 for (int i = 0; i < kPagedUnitSmall * CH / 32; ++i) {
                     const int r = (i * 32 + lane) / CH, c = (i * 32 + lane) % CH;
-                    const bool ok = row >= 0 && pos + r < ld_len && pos + r >= ld_lo;
+                    const bool ok = row >= 0 && pos + r < ld_item.len && pos + r >= ld_lo;
                     const uint32_t d = dst + r * kRow + ((c ^ (r & 7)) << 4);
                     const long long src = ok ? at + r * HD + c * 8 : 0;
                     cp_async16(d, a.k + src, ok);
@@ -294,14 +290,14 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
         PagedItem it;
         auto open_segment = [&]() {
             it = p.items[cur.item];
-            const int q0 = p.cu_q[it.seq], nq = p.cu_q[it.seq + 1] - q0, len = p.kv_len[it.seq];
+            const int q0 = it.q0, nq = it.nq, len = it.len;
             const uint16_t *qr[2];
             bool ok[2];
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int r = lane / 4 + 8 * h;
                 ok[h] = r < it.nrows;
-                const int row = it.row0 + (ok[h] ? r : 0), tok = row / s.group;
+                const int row = it.row0 + (ok[h] ? r : 0), tok = fdiv(row, s.by_group);
                 qr[h] = a.q + (long long)(q0 + tok) * a.q_stride + (long long)(cur.g * s.group + row - tok * s.group) * HD;
                 hi[h] = len - nq + tok;
                 lo[h] = prefix;
@@ -309,8 +305,8 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                 m[h] = -INFINITY;
                 l[h] = 0.f;
             }
-            min_hi = len - nq + it.row0 / s.group;
-            const int max_hi = len - nq + (it.row0 + it.nrows - 1) / s.group;
+            min_hi = len - nq + fdiv(it.row0, s.by_group);
+            const int max_hi = len - nq + fdiv(it.row0 + it.nrows - 1, s.by_group);
             max_lo = prefix;
             if (s.window > 0) max_lo = max(max_lo, max_hi - s.window + 1);
 #pragma unroll
@@ -348,13 +344,12 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
         };
         // the finished rows of an item, straight from the accumulators
         auto write_rows = [&]() {
-            const int q0 = p.cu_q[it.seq];
-            const int pre = p.kv_len[it.seq] > 0 ? prefix : 0;  // an idle slot has none
+            const int q0 = it.q0, pre = it.len > 0 ? prefix : 0;  // an idle slot has none
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int r = lane / 4 + 8 * h;
                 if (r >= it.nrows) continue;
-                const int row = it.row0 + r, tok = row / s.group;
+                const int row = it.row0 + r, tok = fdiv(row, s.by_group);
                 const int token = q0 + tok, head = cur.g * s.group + row - tok * s.group;
                 const long long pr = (long long)token * s.nh + head;
                 float c = 1.f, ci = 0.f, sum = l[h];
@@ -492,7 +487,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
     // Every warp takes every eighth row.
     auto join = [&](int w0, bool from_front, int n, bool closed, bool open_left, int g, int item) {
         const PagedItem it = p.items[item];
-        const int q0 = p.cu_q[it.seq], pre = p.kv_len[it.seq] > 0 ? prefix : 0;
+        const int q0 = it.q0, pre = it.len > 0 ? prefix : 0;
         const bool done = closed && !open_left;
         const int slot = 2 * cta + (open_left ? 0 : 1);
         for (int r = warp; r < it.nrows; r += kPagedWarps) {
@@ -507,7 +502,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                     load_vec<HD>(reinterpret_cast<const float *>(base) + r * HD + lane * E, oi);
                 },
                 m, l, o);
-            const int row = it.row0 + r, tok = row / s.group;
+            const int row = it.row0 + r, tok = fdiv(row, s.by_group);
             if (done) {
                 finish_row<HD>(s, a, pre, q0 + tok, g * s.group + row - tok * s.group, m, l, o);
             } else {
@@ -552,7 +547,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
         if (!sm_last) continue;
         __threadfence();
         const PagedItem it = p.items[item];
-        const int q0 = p.cu_q[it.seq], pre = p.kv_len[it.seq] > 0 ? prefix : 0;
+        const int q0 = it.q0, pre = it.len > 0 ? prefix : 0;
         for (int r = warp; r < it.nrows; r += kPagedWarps) {
             float m, l, o[E];
             merge_partials<HD>(
@@ -565,7 +560,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                     load_vec_cg<HD>(p.part + at * HD + lane * E, oi);
                 },
                 m, l, o);
-            const int row = it.row0 + r, tok = row / s.group;
+            const int row = it.row0 + r, tok = fdiv(row, s.by_group);
             finish_row<HD>(s, a, pre, q0 + tok, g * s.group + row - tok * s.group, m, l, o);
         }
     }

@@ -307,9 +307,9 @@ struct Rows256Walk {
             x.first = 0;
             x.lo = 0;
         } else {
-            x.q0 = p.cu_q[it.seq];
-            x.len = p.kv_len[it.seq];
-            x.first = x.len - (p.cu_q[it.seq + 1] - x.q0);
+            x.q0 = it.q0;
+            x.len = it.len;
+            x.first = it.len - it.nq;
             x.lo = s.window > 0 ? max(0, x.first + fdiv(it.row0, s.by_group) - s.window + 1) : 0;
         }
         // the next item's record, for the next call
@@ -817,7 +817,7 @@ __global__ void __launch_bounds__(kTileRows) k_paged_join(const PagedShape s, co
         }
     }
     const int r = it.row0 + i * kTileRows + row, tok = fdiv(r, s.by_group), head = g * s.group + r - tok * s.group;
-    const long long token = (a.prefix_run ? 0 : p.cu_q[it.seq]) + tok;
+    const long long token = it.q0 + tok;
     if (!a.prefix_run && a.r.out_bf16) {
         const float f = l == 0.f ? 0.f : 1.f / l;
         uint16_t *d = reinterpret_cast<uint16_t *>(a.r.out) + token * a.r.out_stride + (long long)head * HD + col;
