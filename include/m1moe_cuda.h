@@ -488,7 +488,8 @@ typedef struct m1moe_paged_cfg {
     int32_t max_q;             /* at least the most new tokens of one sequence   */
     int32_t window;            /* positions a token sees, itself included; 0: all */
     int32_t shared_prefix;     /* positions (whole pages) that all sequences may
-                                  share; a hint that changes no result           */
+                                  share; a hint that changes results by no more
+                                  than rounding                                  */
 } m1moe_paged_cfg;
 
 /* Bytes of the plan buffer of such a batch on the current device (0, with a

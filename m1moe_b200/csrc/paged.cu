@@ -109,16 +109,22 @@ m1moe_status make_shape(const m1moe_paged_cfg *c, int ctas, m1::PagedShape &s) {
     s.max_q = c->max_q;
     s.window = c->window;
     s.ctas = ctas;
-    // 16-row items while a sequence's rows fit one, 256-row ones beyond
+    // 16-row items while a sequence's rows fit one, 256-row ones beyond (64
+    // decode sequences: 113 us with 16 rows; a 8192-token prompt: 4226 us with
+    // 16 rows, 505 with 256)
     const bool small = (long long)group * c->max_q <= m1::kPagedRowsSmall;
     s.rows = small ? m1::kPagedRowsSmall : m1::kPagedRowsLarge;
     s.unit = small ? m1::kPagedUnitSmall : m1::kPagedUnitLarge;
     s.workers = small ? ctas * m1::kPagedWarps : ctas;
     s.min_per = small ? m1::kPagedWarps : 1;
-    s.prefix = small && c->window == 0 && c->total_q * group >= 40 ? c->shared_prefix : 0;
+    // A shared prefix pays from about 40 rows a KV head on: its pass is a
+    // 256-row one, however few it fills (16 rows over 1504 positions: 35 us
+    // with every sequence reading it, 73 shared; 800 rows over 16384: 1549 and
+    // 195).
+    s.prefix = small && c->window == 0 && (long long)c->total_q * group >= 40 ? c->shared_prefix : 0;
     const long long items = c->num_seqs + (long long)c->total_q * group / s.rows;
     const long long cap = (long long)c->max_pages_per_seq * c->page_size;
-    if (items * (cap / s.unit + 1 + m1::kPagedItemCost) * c->num_kv_heads > 0x7FFFFFFFLL)
+    if (items * (cap / s.unit + 1 + m1::kPagedItemCost) * c->num_kv_heads > 0x7FFF0000LL)
         return fail(M1MOE_ERR_UNSUPPORTED, "the batch's work (%lld items of up to %lld positions) does not fit 31 bits",
                     items, cap);
     s.max_items = (int)items;
@@ -192,15 +198,13 @@ using EncodeTiledFn = CUresult (*)(CUtensorMap *, CUtensorMapDataType, cuuint32_
 // A pool as rows of hd elements; a box is 64 columns of a page's rows (128 at
 // most), 128-byte swizzled.
 m1moe_status pool_map(const m1::PagedShape &s, const uint16_t *pool, CUtensorMap *map) {
-    static EncodeTiledFn encode = nullptr;  // one address for the process
-    if (!encode) {
+    static const EncodeTiledFn encode = []() -> EncodeTiledFn {  // one address for the process
         void *fn = nullptr;
         cudaDriverEntryPointQueryResult q{};
-        P_CK(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q));
-        if (!fn || q != cudaDriverEntryPointSuccess)
-            return fail(M1MOE_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
-        encode = reinterpret_cast<EncodeTiledFn>(fn);
-    }
+        const cudaError_t e = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &fn, cudaEnableDefault, &q);
+        return e == cudaSuccess && q == cudaDriverEntryPointSuccess ? reinterpret_cast<EncodeTiledFn>(fn) : nullptr;
+    }();
+    if (!encode) return fail(M1MOE_ERR_CUDA, "cuTensorMapEncodeTiled is not available");
     const cuuint64_t dims[2] = {(cuuint64_t)s.hd, (cuuint64_t)s.num_pages * s.nkv * s.page_size};
     const cuuint64_t strides[1] = {(cuuint64_t)s.hd * 2};
     const cuuint32_t box[2] = {64, (cuuint32_t)std::min(s.page_size, m1::kPagedUnitLarge)}, one[2] = {1, 1};

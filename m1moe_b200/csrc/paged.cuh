@@ -383,7 +383,10 @@ __device__ __forceinline__ uint2 round4(const uint64_t (&v)[2]) {
 // fp32, one rounding at the end.  A group keeps its token's place and angles
 // over its heads and has the loads of kAppendAhead heads under way.  HBM
 // would bound it; what does is the instructions (about 80 a warp and two
-// heads), hence the packed arithmetic.
+// heads), hence the packed arithmetic.  Measured: nine prompts, 13.9 thousand
+// tokens of 48 heads bf16 with norm, 91 us = 3.75 TB/s (57 % of the measured
+// copy rate; 141 us with a head per group of lanes and shuffled halves); 2000
+// tokens f32, 17 us = 4.4 TB/s; one token 3.3 us.
 constexpr int kAppendAhead = 2;
 template <int HD, bool BF16>
 __global__ void __launch_bounds__(256, 4) k_paged_append(const PagedShape s, const PagedPlanView p,

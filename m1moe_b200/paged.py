@@ -91,7 +91,8 @@ class PagedBatch:
     page_table  int32 CUDA [sequences][most pages]; unused entries are never read
     window      positions a token sees, itself included (0: all before it)
     shared_prefix  positions at the start, whole pages, that all page tables share: attention
-                   may then read them once for the batch; a hint that changes no result
+                   may then read them once for the batch; a hint that changes results by no
+                more than rounding
     """
 
     def __init__(self, cache: PagedKVCache, q_lens, kv_lens, page_table: torch.Tensor, *, num_heads: int,
