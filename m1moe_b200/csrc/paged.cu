@@ -117,17 +117,27 @@ m1moe_status make_shape(const m1moe_paged_cfg *c, int ctas, m1::PagedShape &s) {
     s.unit = small ? m1::kPagedUnitSmall : m1::kPagedUnitLarge;
     s.workers = small ? ctas * m1::kPagedWarps : ctas;
     s.min_per = small ? m1::kPagedWarps : 1;
-    // A shared prefix pays from about 40 rows a KV head on: its pass is a
-    // 256-row one, however few it fills (16 rows over 1504 positions: 35 us
-    // with every sequence reading it, 73 shared; 800 rows over 16384: 1549 and
-    // 195).
-    s.prefix = small && c->window == 0 && (long long)c->total_q * group >= 40 ? c->shared_prefix : 0;
     const long long items = c->num_seqs + (long long)c->total_q * group / s.rows;
     const long long cap = (long long)c->max_pages_per_seq * c->page_size;
     if (items * (cap / s.unit + 1 + m1::kPagedItemCost) * c->num_kv_heads > 0x7FFF0000LL)
         return fail(M1MOE_ERR_UNSUPPORTED, "the batch's work (%lld items of up to %lld positions) does not fit 31 bits",
                     items, cap);
     s.max_items = (int)items;
+    // A prefix is shared where reading it once saves 200 MB of reads: the extra
+    // pass and its partials cost what those take from L2 (us without and with
+    // it, n sequences over a prefix: 4 over 1504, 16/16 heads, 37 MB: 18 and 28;
+    // 16, 185 MB: 34.8 and 35.3; 32, 382 MB: 58.9 and 37.1; 24 over 2048, 32/8
+    // heads, 193 MB: 35.1 and 35.8; 8 over 8192, 235 MB: 42.5 and 40.7; 200 over
+    // 16384, 53 GB: 1549 and 195).
+    // Its pass takes 16-row items up to 128 rows a KV head, 256-row ones beyond
+    // (16-row and 256-row, 32/8 heads over 4096: 64 rows 39.7 and 45.4 us, 128
+    // rows 46.1 and 46.2, 256 rows 70.1 and 58.6).
+    // The plan keeps room for the pass whenever a prefix is named, so that its
+    // size does not jump as sequences join the batch.
+    s.prefix_room = small && c->window == 0 && c->num_seqs > 1 && c->shared_prefix > 0;
+    const long long saved = (long long)(c->num_seqs - 1) * c->shared_prefix * c->num_kv_heads * c->head_dim * 4;
+    s.prefix = s.prefix_room && saved >= 200000000LL ? c->shared_prefix : 0;
+    s.prefix_rows = (long long)c->total_q * group > 128 ? m1::kPagedRowsLarge : m1::kPagedRowsSmall;
     return M1MOE_OK;
 }
 
@@ -158,14 +168,16 @@ size_t plan_view(const m1::PagedShape &s, void *base, m1::PagedPlanView &v, m1::
     take(v.part_ml, (size_t)2 * s.ctas * part_rows * 8);
     take(v.part, (size_t)2 * s.ctas * part_rows * s.hd * 4);
     v2 = v;
-    if (s.prefix == 0) return at;
-    const size_t items2 = ((size_t)s.total_q * s.group + m1::kPagedRowsLarge - 1) / m1::kPagedRowsLarge;
+    if (!s.prefix_room) return at;
+    const size_t rows2 = s.prefix_rows, items2 = ((size_t)s.total_q * s.group + rows2 - 1) / rows2;
+    const bool small2 = s.prefix_rows == m1::kPagedRowsSmall;
     take(v2.header, m1::kPhWords * 4);
     take(v2.items, items2 * sizeof(m1::PagedItem));
     take(v2.unit_at, (items2 + 1) * 4);
-    take(v2.start, (size_t)s.ctas * 4);
-    take(v2.part_ml, (size_t)2 * s.ctas * m1::kPagedRowsLarge * 8);
-    take(v2.part, (size_t)2 * s.ctas * m1::kPagedRowsLarge * s.hd * 4);
+    take(v2.start, (size_t)s.ctas * 4 * (small2 ? m1::kPagedWarps : 1));
+    take(v2.count, small2 ? (size_t)s.nkv * items2 * 4 : 0);
+    take(v2.part_ml, (size_t)2 * s.ctas * rows2 * 8);
+    take(v2.part, (size_t)2 * s.ctas * rows2 * s.hd * 4);
     take(pre.ml, (size_t)s.total_q * s.nh * 8);
     take(pre.part, (size_t)s.total_q * s.nh * s.hd * 4);
     return at;
@@ -263,7 +275,13 @@ m1moe_status attention(const Plan &p, m1::RowsParams a, cudaStream_t st) {
     if (p.s.rows == m1::kPagedRowsLarge) return launch_rows256<HD>(p.s, p.v, a, nullptr, st);
     if (p.s.prefix > 0) {
         // one partial per row over the prefix, then the sequences' own parts
-        if (m1moe_status e = launch_rows256<HD>(p.s, p.v2, a, &p.pre, st)) return e;
+        m1::RowsParams b = a;
+        b.part_rows = m1::kPagedRowsSmall;
+        b.partial = p.pre.part;
+        b.partial_ml = p.pre.ml;
+        if (m1moe_status e = p.s.prefix_rows == m1::kPagedRowsLarge ? launch_rows256<HD>(p.s, p.v2, a, &p.pre, st)
+                                                                    : launch_rows16<HD>(p.s, p.v2, b, st))
+            return e;
         a.prefix_part = p.pre.part;
         a.prefix_ml = p.pre.ml;
     }

@@ -99,6 +99,8 @@ struct PagedShape {
     int ctas, workers;   // CTAs of the attention grid, and plan start entries
     int min_per;         // fewest units per CTA
     int max_items;
+    int prefix_room;     // the plan has room for the shared prefix's pass
+    int prefix_rows;     // item rows of the shared prefix's pass: 16 or 256
 };
 
 // Pool row of position p of sequence b and KV head g, or -1 (with the status
@@ -265,19 +267,28 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
         p.header[kPhPrefix] = prefix;
     }
     if (s.prefix == 0) return;
-    // the prefix's own split: all rows of the batch, 256 at a time, against
-    // its positions (no items when it is not shared after all)
-    const int rows = s.total_q * s.group;
-    const int items2 = prefix ? (rows + kPagedRowsLarge - 1) / kPagedRowsLarge : 0;
-    const int n2 = (prefix + kPagedUnitLarge - 1) / kPagedUnitLarge + kPagedItemCost, units2 = items2 * n2;
+    // the prefix's own split: all rows of the batch, 16 or 256 at a time,
+    // against its positions (no items when it is not shared after all)
+    const bool big = s.prefix_rows == kPagedRowsLarge;
+    const int rows = s.total_q * s.group, unit2 = big ? kPagedUnitLarge : kPagedUnitSmall;
+    const int items2 = prefix ? (rows + s.prefix_rows - 1) / s.prefix_rows : 0;
+    const int n2 = (prefix + unit2 - 1) / unit2 + (big ? kPagedItemCost : 0), units2 = items2 * n2;
     for (int i = tid; i <= items2; i += 1024) {
         p2.unit_at[i] = i * n2;
         if (i < items2)
-            p2.items[i] = PagedItem{lead, i * kPagedRowsLarge, min(kPagedRowsLarge, rows - i * kPagedRowsLarge), 0,
+            p2.items[i] = PagedItem{lead, i * s.prefix_rows, min(s.prefix_rows, rows - i * s.prefix_rows), 0,
                                     0, s.total_q, prefix, 0};
     }
-    const int all2 = units2 * s.nkv, per2 = max(1, (all2 + s.ctas - 1) / s.ctas);
-    for (int c = tid; c < s.ctas; c += 1024) p2.start[c] = c * per2 < all2 ? (c * per2) % units2 / n2 : 0;
+    for (int i = tid; !big && i < items2 * s.nkv; i += 1024) p2.count[i] = 0;
+    const int all2 = units2 * s.nkv, nw2 = big ? 1 : kPagedWarps;
+    const int per2 = max(big ? 1 : kPagedWarps, (all2 + s.ctas - 1) / s.ctas);
+    for (int w = tid; w < s.ctas * nw2; w += 1024) {
+        const int c = w / nw2;
+        const long long c0 = (long long)c * per2, c1 = min((long long)all2, c0 + per2);
+        const int pw = (int)((c1 - c0 + nw2 - 1) / nw2);
+        const long long u = c0 + (long long)(w - c * nw2) * pw;
+        p2.start[w] = u < c1 ? (int)(u % units2) / n2 : 0;
+    }
     if (tid == 0) {
         p2.header[kPhItems] = items2;
         p2.header[kPhUnits] = units2;

@@ -43,6 +43,8 @@ struct RowsParams {
     int part_rows;       // rows kept of a partial: group * max_q
     const float *prefix_part;  // [total_q][nh][hd] merged in when the header names a prefix
     const float2 *prefix_ml;   // [total_q][nh]
+    float *partial;            // not NULL: this launch is the prefix's pass -- all rows see all of it --
+    float2 *partial_ml;        // and leaves each row's values and (maximum, sum) here
 };
 
 constexpr float kLog2e = 1.4426950408889634f;
@@ -185,8 +187,13 @@ __device__ __forceinline__ void finish_row(const PagedShape &s, const RowsParams
                                            float m, float l, float (&o)[HD / 32]) {
     constexpr int E = HD / 32;
     const int lane = threadIdx.x & 31;
+    const long long r = (long long)token * s.nh + head;
+    if (a.partial) {
+        store_vec<HD>(a.partial + r * HD + lane * E, o);
+        if (lane == 0) a.partial_ml[r] = make_float2(m, l);
+        return;
+    }
     if (prefix > 0) {
-        const long long r = (long long)token * s.nh + head;
         const float2 ml = a.prefix_ml[r];
         float x[E];
         load_vec<HD>(a.prefix_part + r * HD + lane * E, x);
@@ -234,7 +241,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
     pdl_wait();
     const int start = p.start[cta * kPagedWarps + warp];
     const int units = p.header[kPhUnits], items = p.header[kPhItems], per = p.header[kPhPer];
-    const int prefix = p.header[kPhPrefix];
+    const int prefix = a.partial ? 0 : p.header[kPhPrefix];
     int *status = p.status;
     const int all = units * s.nkv;
     const int c0 = min(cta * per, all), c1 = min(all, c0 + per);
@@ -304,13 +311,13 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                 ok[h] = r < it.nrows;
                 const int row = it.row0 + (ok[h] ? r : 0), tok = fdiv(row, s.by_group);
                 qr[h] = a.q + (long long)(q0 + tok) * a.q_stride + (long long)(cur.g * s.group + row - tok * s.group) * HD;
-                hi[h] = len - nq + tok;
+                hi[h] = a.partial ? len - 1 : len - nq + tok;
                 lo[h] = prefix;
                 if (s.window > 0) lo[h] = max(lo[h], hi[h] - s.window + 1);
                 m[h] = -INFINITY;
                 l[h] = 0.f;
             }
-            min_hi = len - nq + fdiv(it.row0, s.by_group);
+            min_hi = a.partial ? len - 1 : len - nq + fdiv(it.row0, s.by_group);
             const int max_hi = len - nq + fdiv(it.row0 + it.nrows - 1, s.by_group);
             max_lo = prefix;
             if (s.window > 0) max_lo = max(max_lo, max_hi - s.window + 1);
@@ -365,7 +372,8 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                     ci = ml.x == -INFINITY ? 0.f : exp2_approx(ml.x - mn);
                     sum = sum * c + ml.y * ci;
                 }
-                const float inv = sum == 0.f ? 0.f : 1.f / sum;
+                const float inv = a.partial ? 1.f : sum == 0.f ? 0.f : 1.f / sum;
+                if (a.partial && (lane & 3) == 0) a.partial_ml[pr] = make_float2(m[h], sum);
                 const long long at = (long long)token * a.out_stride + (long long)head * HD;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
@@ -376,7 +384,9 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                         x0 += y.x * ci, x1 += y.y * ci;
                     }
                     x0 *= inv, x1 *= inv;
-                    if (a.out_bf16)
+                    if (a.partial)
+                        *reinterpret_cast<float2 *>(a.partial + pr * HD + col) = make_float2(x0, x1);
+                    else if (a.out_bf16)
                         *reinterpret_cast<uint32_t *>(reinterpret_cast<uint16_t *>(a.out) + at + col) = pack_bf16(x0, x1);
                     else
                         *reinterpret_cast<float2 *>(reinterpret_cast<float *>(a.out) + at + col) = make_float2(x0, x1);

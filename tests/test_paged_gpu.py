@@ -470,3 +470,45 @@ def test_a_prefix_that_cannot_be_shared_changes_nothing(why):
     batch.check()
     ref, mag = attention_ref(q, dense, q_lens, kv_lens, nkv, hd ** -0.5, window)
     check_attention(out, ref, mag)
+
+
+# A prefix is read once for the batch where that saves 200 MB of reads; the sizes
+# below are above that, in the 16-row form (up to 128 rows a KV head) and the 256-row one.
+@pytest.mark.parametrize("nh,nkv,hd,page,share,q_lens,kv_lens,cap", [
+    (16, 16, 128, 16, 1024, [1] * 27, [1025 + 5 * i for i in range(27)], 0.0),
+    (24, 8, 64, 32, 4064, [1, 2] * 13, [4066 + 9 * i for i in range(26)], 25.0),
+    (32, 8, 128, 64, 8192, [1] * 8, [0, 8193, 8400, 0, 8200, 9000, 8193, 8257], 0.0),  # idle slots
+    (16, 1, 128, 128, 57344, [1] * 8, [57345 + 40 * i for i in range(8)], 0.0),
+    (16, 1, 128, 128, 57344, [1] * 9, [57345 + 40 * i for i in range(9)], 0.0),
+])
+def test_shared_prefix_read_once(nh, nkv, hd, page, share, q_lens, kv_lens, cap):
+    assert (len(q_lens) - 1) * share * nkv * hd * 4 >= 200_000_000
+    cache, table, dense = make(nkv, hd, page, q_lens, kv_lens, seed=24, share=share)
+    g = torch.Generator(device="cuda").manual_seed(25)
+    q = (1.5 * torch.randn((sum(q_lens), nh, hd), generator=g, device="cuda")).bfloat16()
+    batch = PagedBatch(cache, q_lens, kv_lens, table, num_heads=nh, shared_prefix=share)
+    ref, mag = attention_ref(q, dense, q_lens, kv_lens, nkv, hd ** -0.5, 0, cap)
+    for dt in (torch.bfloat16, torch.float32):
+        out = paged_attention(cache, 0, batch, q, softcap=cap, out_dtype=dt)
+        batch.check()
+        check_attention(out, ref, mag)
+        assert torch.equal(out, paged_attention(cache, 0, batch, q, softcap=cap, out_dtype=dt))
+
+
+@pytest.mark.parametrize("why", ["tables differ", "a sequence ends inside it", "no sequence is live"])
+def test_a_long_prefix_that_cannot_be_shared_changes_nothing(why):
+    nh, nkv, hd, page, share = 32, 8, 128, 64, 8192
+    q_lens, kv_lens = [1] * 8, [8193 + 50 * i for i in range(8)]
+    if why == "a sequence ends inside it":
+        kv_lens[5] = 8192
+    cache, table, dense = make(nkv, hd, page, q_lens, kv_lens, seed=26, share=0 if why == "tables differ" else share)
+    q = torch.randn((sum(q_lens), nh, hd), device="cuda").bfloat16()
+    lens = [0] * 8 if why == "no sequence is live" else kv_lens
+    batch = PagedBatch(cache, q_lens, lens, table, num_heads=nh, shared_prefix=share)
+    out = paged_attention(cache, 0, batch, q)
+    batch.check()
+    if why == "no sequence is live":
+        assert not out.any()
+        return
+    ref, mag = attention_ref(q, dense, q_lens, kv_lens, nkv, hd ** -0.5, 0)
+    check_attention(out, ref, mag)
