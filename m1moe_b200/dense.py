@@ -159,6 +159,7 @@ class DenseModel:
         """One step of a ragged batch (paged.PagedBatch) over a paged cache: the new tokens
         [total_q] (int32, CUDA) through every layer; returns f32 logits [sequences][vocab] of each
         sequence's last new token, for sampling.sample.  rope: paged.rope_table."""
+        batch._made_for(cache)
         if tokens.shape != (batch.total_q,) or tokens.dtype != torch.int32:
             raise ValueError(f"tokens: int32 [{batch.total_q}]")
         if cache.num_layers != self.num_layers:

@@ -11,7 +11,8 @@ device memory and streams, every computation runs in libm1moe_cuda.so.
   paged_attention  causal attention over the pages (InferenceEngine.swift:349-399)
   rope_table       cosines and sines of every position, also scaled for long contexts
 
-A batch's calls use its plan's partial results and so belong on one stream, in order.
+A batch's calls use its plan's partial results and so belong on one stream, in order.  They take
+the cache that the batch was made for, or one with the same sizes on the same device.
 """
 from __future__ import annotations
 
@@ -81,6 +82,10 @@ class PagedKVCache:
             raise ValueError(f"layer {layer} out of range [0,{self.num_layers})")
         return self._k0 + layer * self._layer_bytes, self._v0 + layer * self._layer_bytes
 
+    def _sizes(self):
+        """What a batch's page ids and addresses are checked and formed by."""
+        return self.num_pages, self.num_kv_heads, self.page_size, self.head_dim, self.device
+
 
 class PagedBatch:
     """The sequences of one step.
@@ -139,6 +144,12 @@ class PagedBatch:
             _plan_call(self._cfg, self.cu_q.data_ptr(), self.kv_lens.data_ptr(), self._table,
                        self._plan, self.plan.numel(), st)
 
+    def _made_for(self, cache: PagedKVCache) -> None:
+        """Refuse a cache whose pools are not of the sizes that the plan goes by: the kernels would leave them."""
+        if cache is not self.cache and cache._sizes() != self.cache._sizes():
+            raise ValueError(f"the batch was made for a cache of (pages, kv heads, page size, head dim, device) "
+                             f"{self.cache._sizes()}, not {cache._sizes()}")
+
     def check(self, *, stream=None) -> None:
         """Wait for the stream and raise if a kernel found a length, page or position out of range."""
         with torch.cuda.device(self.cache.device):
@@ -172,6 +183,7 @@ def paged_append(cache: PagedKVCache, layer: int, batch: PagedBatch, qkv: torch.
             with i + rot/2 or, with rope_pairs, 2i with 2i + 1
     q_norm, k_norm  bf16 [head dim] RMSNorm weights of each head, or None
     """
+    batch._made_for(cache)
     if qkv.shape != batch._qkv_shape:
         raise ValueError(f"qkv is {tuple(qkv.shape)}, expected {batch._qkv_shape}")
     dev = cache.device
@@ -210,6 +222,7 @@ def paged_attention(cache: PagedKVCache, layer: int, batch: PagedBatch, q: torch
     """Attention of the batch's new tokens (q bf16 [total_q][heads][head dim], tokens may lie
     further apart) over their sequences; scores are scale * q.k (default 1/sqrt(head dim)), capped
     as softcap * tanh(score / softcap) if softcap > 0."""
+    batch._made_for(cache)
     if q.dtype != _BF16:
         raise TypeError(f"q must be bfloat16, got {q.dtype}")
     stride = _check_rows(q, "q", cache, batch)
