@@ -26,17 +26,23 @@ from .expert_ffn import dtype_code
 
 _F32, _BF16 = torch.float32, torch.bfloat16
 _raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream() without its wrapper: 0.1 of 3 us
+_current_device = torch._C._cuda_getDevice
 
 
 def _fn(name: str):
-    """The entry point `name` with its status checked."""
+    """The entry point `name`, called with device `index` current (a null stream is that of the
+    current device, whatever device the pointers are of) and its status checked."""
     f = None
 
-    def call(*args):
+    def call(index, *args):
         nonlocal f
         if f is None:
             f = getattr(_lib.lib(), name)
-        st = f(*args)
+        if index == _current_device():
+            st = f(*args)
+        else:
+            with torch.cuda.device(index):
+                st = f(*args)
         if st:
             _lib.check(st, name)
 
@@ -140,9 +146,8 @@ class PagedBatch:
         """Make the plan again from `cu_q`, `kv_lens` and `page_table` as they are on the device
         now (for a next step with the same new tokens per sequence; capturable)."""
         st = self._use(stream)
-        with torch.cuda.device(self.cache.device):
-            _plan_call(self._cfg, self.cu_q.data_ptr(), self.kv_lens.data_ptr(), self._table,
-                       self._plan, self.plan.numel(), st)
+        _plan_call(self.cache._index, self._cfg, self.cu_q.data_ptr(), self.kv_lens.data_ptr(), self._table,
+                   self._plan, self.plan.numel(), st)
 
     def _made_for(self, cache: PagedKVCache) -> None:
         """Refuse a cache whose pools are not of the sizes that the plan goes by: the kernels would leave them."""
@@ -152,8 +157,7 @@ class PagedBatch:
 
     def check(self, *, stream=None) -> None:
         """Wait for the stream and raise if a kernel found a length, page or position out of range."""
-        with torch.cuda.device(self.cache.device):
-            _status_call(self._plan, self._use(stream))
+        _status_call(self.cache._index, self._plan, self._use(stream))
 
     def _use(self, stream) -> int:
         st = _raw_stream(self.cache._index) if stream is None else stream.cuda_stream
@@ -205,8 +209,9 @@ def paged_append(cache: PagedKVCache, layer: int, batch: PagedBatch, qkv: torch.
     if batch.total_q == 0:
         return out
     positions, pairs, _ = rope.shape
-    _append_call(batch._cfg, batch._plan, batch._table, qkv.data_ptr(), dtype_code(qkv.dtype), qkv.stride(0), qn, kn, eps,
-                 rope.data_ptr(), positions, 2 * pairs, 1 if rope_pairs else 0, k, v, out.data_ptr(), st)
+    _append_call(cache._index, batch._cfg, batch._plan, batch._table, qkv.data_ptr(), dtype_code(qkv.dtype),
+                 qkv.stride(0), qn, kn, eps, rope.data_ptr(), positions, 2 * pairs, 1 if rope_pairs else 0, k, v,
+                 out.data_ptr(), st)
     return out
 
 
@@ -235,7 +240,7 @@ def paged_attention(cache: PagedKVCache, layer: int, batch: PagedBatch, q: torch
         out_stride = _check_rows(out, "out", cache, batch)
     if batch.total_q == 0:
         return out
-    _attention_call(batch._cfg, batch._plan, batch._table, q.data_ptr(), stride, k, v,
+    _attention_call(cache._index, batch._cfg, batch._plan, batch._table, q.data_ptr(), stride, k, v,
                     1.0 / math.sqrt(cache.head_dim) if scale is None else scale, softcap, out.data_ptr(),
                     dtype_code(out.dtype), out_stride, st)
     return out

@@ -48,6 +48,6 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, t
         raise ValueError(f"out: a contiguous int32 tensor [{rows}] on {dev}")
     # one row's stride may be anything; the C side wants at least the row's length
     stride = logits.stride(0) if rows > 1 else max(logits.stride(0), vocab)
-    _sample_call(logits.data_ptr(), dtype_code(logits.dtype), stride, rows, vocab, pu, pt, vt, pk, vk, pp, vp, pm, vm,
-                 out.data_ptr(), st)
+    _sample_call(dev.index, logits.data_ptr(), dtype_code(logits.dtype), stride, rows, vocab, pu, pt, vt, pk, vk, pp, vp,
+                 pm, vm, out.data_ptr(), st)
     return out

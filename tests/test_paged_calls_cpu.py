@@ -77,3 +77,74 @@ def test_a_cache_of_the_same_sizes_is_accepted(call, calls):
     call(batch.cache, batch)
     call(fake_cache(layers=7), batch)
     assert len(calls) == 2
+
+
+@pytest.fixture
+def devices(monkeypatch):
+    """Two devices, 0 the current one: the list of devices that the entry points ran on."""
+    state, ran = {"now": 0}, []
+
+    class Device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, state["now"] = state["now"], self.index
+
+        def __exit__(self, *exc):
+            state["now"] = self.before
+
+    class Lib:
+        def __getattr__(self, name):
+            return lambda *a: ran.append((name, state["now"])) or 0
+
+    monkeypatch.setattr(paged, "_current_device", lambda: state["now"])
+    monkeypatch.setattr(torch.cuda, "device", Device)
+    monkeypatch.setattr(_lib, "lib", Lib)
+    for name in ("plan", "append", "attention", "status"):
+        monkeypatch.setattr(paged, f"_{name}_call", paged._fn(f"m1moe_cuda_paged_{name}"))
+    return ran
+
+
+@pytest.mark.parametrize("index", [0, 1])
+def test_calls_run_on_the_caches_device(index, devices):
+    """Raw stream 0 is the default stream of whichever device is current: the call makes the tensors'
+    device current, and only then."""
+    batch = fake_batch(fake_cache())
+    batch.cache._index = index
+    batch.cu_q = batch.kv_lens = batch.plan = torch.zeros(1)
+    append(batch.cache, batch)
+    attend(batch.cache, batch)
+    batch.update()
+    batch.check()
+    assert devices == [(f"m1moe_cuda_paged_{x}", index) for x in ("append", "attention", "plan", "status")]
+    assert paged._current_device() == 0
+
+
+@pytest.mark.parametrize("index", [0, 1])
+def test_sampling_runs_on_the_logits_device(index, devices, monkeypatch):
+    from m1moe_b200 import sampling
+
+    class Logits:  # a CUDA tensor's face
+        is_cuda, dtype, shape = True, torch.float32, (2, 5)
+        device = torch.device("cuda", index)
+
+        def dim(self):
+            return 2
+
+        def numel(self):
+            return 10
+
+        def stride(self, i):
+            return (5, 1)[i]
+
+        def data_ptr(self):
+            return 64
+
+    monkeypatch.setattr(sampling, "_setting", lambda t, *a: (0, 0))
+    monkeypatch.setattr(sampling, "_raw_stream", lambda i: 0)
+    monkeypatch.setattr(sampling, "_empty", lambda *a: torch.zeros(2, dtype=torch.int32))
+    monkeypatch.setattr(sampling, "_sample_call", paged._fn("m1moe_cuda_sample"))
+    sampling.sample(Logits(), torch.zeros(2))
+    assert devices == [("m1moe_cuda_sample", index)]
+    assert paged._current_device() == 0
