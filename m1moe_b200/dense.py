@@ -160,6 +160,11 @@ class DenseModel:
         [total_q] (int32, CUDA) through every layer; returns f32 logits [sequences][vocab] of each
         sequence's last new token, for sampling.sample.  rope: paged.rope_table."""
         batch._made_for(cache)
+        dev = cache.device
+        if dev.index != self.device:
+            raise ValueError(f"the cache is on {dev}, the model on cuda:{self.device}")
+        if any(t.device != dev for t in (tokens, rope) + ((logits,) if logits is not None else ())):
+            raise ValueError(f"tokens, rope and logits belong on the cache's device {dev}")
         if tokens.shape != (batch.total_q,) or tokens.dtype != torch.int32:
             raise ValueError(f"tokens: int32 [{batch.total_q}]")
         if cache.num_layers != self.num_layers:
@@ -167,7 +172,7 @@ class DenseModel:
         if rope.dim() != 3 or rope.dtype != torch.float32 or rope.shape[2] != 2:
             raise ValueError("rope: float32 [positions][rot/2][2]")
         if logits is None:
-            logits = torch.empty((batch.num_seqs, self.vocab_size), dtype=torch.float32, device=tokens.device)
+            logits = torch.empty((batch.num_seqs, self.vocab_size), dtype=torch.float32, device=dev)
         elif logits.shape != (batch.num_seqs, self.vocab_size) or logits.dtype != torch.float32:
             raise ValueError(f"logits: float32 ({batch.num_seqs}, {self.vocab_size})")
         _check_cuda(tokens, rope, logits)

@@ -148,3 +148,30 @@ def test_sampling_runs_on_the_logits_device(index, devices, monkeypatch):
     sampling.sample(Logits(), torch.zeros(2))
     assert devices == [("m1moe_cuda_sample", index)]
     assert paged._current_device() == 0
+
+
+@pytest.mark.parametrize("on", ["cache", "tokens", "rope", "logits"])
+def test_a_whole_step_over_two_devices_is_refused(on, calls):
+    """The model's kernels run on its own device and would be given another one's pointers."""
+    from m1moe_b200.dense import DenseModel
+
+    class Face:  # a tensor's face
+        def __init__(self, shape, dtype, device):
+            self.shape, self.dtype, self.device, self.is_cuda = shape, dtype, torch.device("cuda", device), True
+
+        def dim(self):
+            return len(self.shape)
+
+        def is_contiguous(self):
+            return True
+
+    at = lambda name: 1 if on == name else 0
+    dm = DenseModel.__new__(DenseModel)
+    dm.num_layers, dm.vocab_size, dm.device = 2, 100, 0
+    cache = fake_cache(device=torch.device("cuda", at("cache")))
+    if on == "cache":  # all but the model
+        at = lambda name: 1
+    with pytest.raises(ValueError, match="device|model on"):
+        dm.paged_step(None, cache, fake_batch(cache), Face((3,), torch.int32, at("tokens")),
+                      rope=Face((64, HD // 2, 2), torch.float32, at("rope")),
+                      logits=Face((3, 100), torch.float32, at("logits")))
