@@ -228,7 +228,9 @@ M1MOE_API m1moe_status m1moe_cuda_moe_layer(m1moe_cuda_ctx *ctx, int32_t layer, 
  * the next m1moe_cuda_synchronize report M1MOE_ERR_DEVICE.  Needs group_size
  * 64 and intermediate_dim a multiple of 128.
  * Scratch for `tokens` is allocated on the first call that needs more
- * (synchronously, outside stream capture); out may alias x. */
+ * (synchronously; refused while the stream is being captured).  Scratch that a
+ * captured graph names is kept until the context is destroyed.  out may
+ * alias x. */
 M1MOE_API m1moe_status m1moe_cuda_moe_prefill(m1moe_cuda_ctx *ctx, int32_t layer, const void *d_x,
                                     int32_t x_dtype, const void *d_residual, int32_t res_dtype,
                                     void *d_out, int32_t out_dtype, int32_t tokens,
@@ -454,7 +456,9 @@ M1MOE_API m1moe_status m1moe_cuda_decode_step(m1moe_dense_ctx *ctx, m1moe_cuda_c
  * T.  The reference runs the prompt token by token through forward()
  * (bench/main.swift:139-141); this gives the same cache and next token
  * within the tolerance of its bf16/fp16 GEMM operands.  Buffers for T tokens
- * are allocated on the first call that needs them (synchronously). */
+ * are allocated on the first call that needs them (synchronously; refused
+ * while the stream is being captured) and kept while a captured graph may
+ * name them. */
 M1MOE_API m1moe_status m1moe_cuda_prefill_step(m1moe_dense_ctx *ctx, m1moe_cuda_ctx *moe,
                                      const int32_t *d_tokens, int32_t tokens,
                                      int32_t *d_next_token, float *d_logits, void *stream);
@@ -559,7 +563,10 @@ M1MOE_API m1moe_status m1moe_cuda_paged_status(void *d_plan, void *stream);
  * max_batch) take the decode kernels, more the prefill ones of
  * m1moe_cuda_prefill_step.  The serving counterpart of InferenceEngine.forward
  * (:124-156), which runs one token of one sequence.  Buffers for total_q
- * tokens are allocated on the first call that needs them (synchronously). */
+ * tokens are allocated on the first call that needs them (synchronously; a call
+ * that would have to while its stream is being captured is refused).  A
+ * captured step stays valid when later calls grow the buffers: those that a
+ * graph names are kept until the contexts are destroyed. */
 M1MOE_API m1moe_status m1moe_cuda_paged_step(m1moe_dense_ctx *ctx, m1moe_cuda_ctx *moe,
                                    const m1moe_paged_cfg *cfg, void *d_plan, const int32_t *d_page_table,
                                    uint16_t *d_k_pages, uint16_t *d_v_pages, const float *d_rope,

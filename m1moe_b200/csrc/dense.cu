@@ -19,6 +19,7 @@
 #include <vector>
 
 #include "m1moe_cuda.h"
+#include "scratch.cuh"
 #include "dense.cuh"
 
 // The error helpers and launch counter of m1moe_cuda.cu (one library).
@@ -63,6 +64,7 @@ struct m1moe_dense_ctx {
     // token-parallel prefill (m1moe_cuda_prefill_step): buffers for pf_cap
     // tokens (grown on demand) and the cuBLAS handle of its projections
     int pf_cap = 0;
+    m1::Scratch pf_scratch, pg_scratch;
     float *pf_res = nullptr, *pf_qkv = nullptr, *pf_hmid = nullptr;
     __nv_bfloat16 *pf_xn = nullptr, *pf_attn = nullptr;
     // a step over a paged cache (m1moe_cuda_paged_step): the rotated queries of
@@ -152,6 +154,8 @@ void free_dense(m1moe_dense_ctx *c) {
                     (void *)c->pf_res, (void *)c->pf_qkv, (void *)c->pf_hmid, (void *)c->pf_xn,
                     (void *)c->pf_attn, (void *)c->pg_q, (void *)c->pg_last, (void *)c->pg_last_n})
         cudaFree(q);
+    c->pf_scratch.release();
+    c->pg_scratch.release();
     if (c->blas) cublasDestroy(c->blas);
     delete c;
 }
@@ -276,17 +280,23 @@ m1moe_status check_loaded(m1moe_dense_ctx *c) {
     return M1MOE_OK;
 }
 
-// Buffers for T prefill tokens (grown, never shrunk; a synchronous reallocation).
-m1moe_status pf_dense_reserve(m1moe_dense_ctx *c, int T) {
+m1moe_status not_while_capturing(int T) {
+    return fail(M1MOE_ERR_INVALID_ARG, "%d tokens need larger buffers, which cannot be made while the stream is "
+                                       "captured: run a step of this size before", T);
+}
+
+// Buffers for T prefill tokens (grown, never shrunk; a synchronous reallocation
+// that leaves the buffers of captured graphs in place).
+m1moe_status pf_dense_reserve(m1moe_dense_ctx *c, int T, cudaStream_t st) {
+    const bool capturing = c->pf_scratch.capturing(st);
+    if (capturing && (!c->blas || T > c->pf_cap)) return not_while_capturing(T);
     if (!c->blas) {
         if (cublasCreate(&c->blas) != CUBLAS_STATUS_SUCCESS)
             return fail(M1MOE_ERR_CUDA, "cublasCreate failed");
     }
     if (T <= c->pf_cap) return M1MOE_OK;
     D_CK(cudaDeviceSynchronize());
-    for (void *q : {(void *)c->pf_res, (void *)c->pf_qkv, (void *)c->pf_hmid, (void *)c->pf_xn,
-                    (void *)c->pf_attn})
-        cudaFree(q);
+    c->pf_scratch.retire({c->pf_res, c->pf_qkv, c->pf_hmid, c->pf_xn, c->pf_attn});
     c->pf_res = c->pf_qkv = c->pf_hmid = nullptr;
     c->pf_xn = c->pf_attn = nullptr;
     c->pf_cap = 0;
@@ -301,12 +311,14 @@ m1moe_status pf_dense_reserve(m1moe_dense_ctx *c, int T) {
 }
 
 // Buffers of a paged step: T tokens, B sequences.
-m1moe_status pg_reserve(m1moe_dense_ctx *c, int T, int B) {
-    if (m1moe_status st = pf_dense_reserve(c, T)) return st;
+m1moe_status pg_reserve(m1moe_dense_ctx *c, int T, int B, cudaStream_t stream) {
+    if (m1moe_status st = pf_dense_reserve(c, T, stream)) return st;
+    const bool capturing = c->pg_scratch.capturing(stream);
     if (T <= c->pg_cap && B <= c->pg_seqs) return M1MOE_OK;
+    if (capturing) return not_while_capturing(T);
     D_CK(cudaDeviceSynchronize());
     const int t = std::max(T, c->pg_cap), b = std::max(B, c->pg_seqs);
-    for (void *q : {(void *)c->pg_q, (void *)c->pg_last, (void *)c->pg_last_n}) cudaFree(q);
+    c->pg_scratch.retire({c->pg_q, c->pg_last, c->pg_last_n});
     c->pg_q = nullptr;
     c->pg_last = nullptr;
     c->pg_last_n = nullptr;
@@ -666,7 +678,7 @@ m1moe_status m1moe_cuda_prefill_step(m1moe_dense_ctx *c, m1moe_cuda_ctx *moe, co
     if (m1moe_status st = check_loaded(c)) return st;
     if (m1moe_status st = m1abi::moe_compatible(moe, g.hidden_dim, g.num_layers, 1, g.device)) return st;
     DevGuard dg(g.device);
-    if (m1moe_status st = pf_dense_reserve(c, T)) return st;
+    if (m1moe_status st = pf_dense_reserve(c, T, as_stream(stream))) return st;
     D_CK(cudaFuncSetAttribute(m1::k_attn_prefill_tiled, cudaFuncAttributeMaxDynamicSharedMemorySize,
                               (int)m1::attn_prefill_smem()));
     cudaStream_t st = as_stream(stream);
@@ -752,7 +764,7 @@ m1moe_status m1moe_cuda_paged_step(m1moe_dense_ctx *c, m1moe_cuda_ctx *moe, cons
     if (m1moe_status st = check_loaded(c)) return st;
     if (m1moe_status st = m1abi::moe_compatible(moe, h, g.num_layers, 1, g.device)) return st;
     DevGuard dg(g.device);
-    if (m1moe_status st = pg_reserve(c, T, B)) return st;
+    if (m1moe_status st = pg_reserve(c, T, B, as_stream(stream))) return st;
     cudaStream_t st = as_stream(stream);
     const bool few = T <= std::min(m1::kDenseMaxTok, m1abi::moe_max_batch(moe));  // the decode kernels' batch
     const size_t pool = (size_t)cfg->num_pages * g.num_kv_heads * cfg->page_size * c->hd;

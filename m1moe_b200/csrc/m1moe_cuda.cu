@@ -25,6 +25,7 @@
 #include <vector>
 
 #include "m1moe_cuda.h"
+#include "scratch.cuh"
 #include "common.cuh"
 #include "host_io.cuh"
 #include "matvec4.cuh"
@@ -227,6 +228,7 @@ struct m1moe_cuda_ctx {
     // prefill (prefill.cuh): scratch for up to pf_cap tokens, grown on demand,
     // and the tensor maps of the table (made on first use)
     int pf_cap = 0, pf_nsplit = 0, pf_max_tiles = 0;
+    m1::Scratch pf_scratch;
     int *pf_idx = nullptr, *pf_tok_slot = nullptr, *pf_slot_tok = nullptr, *pf_ntiles = nullptr;
     float *pf_w = nullptr, *pf_ypart = nullptr;
     m1::PfTile *pf_tiles = nullptr;
@@ -290,6 +292,7 @@ void free_ctx(m1moe_cuda_ctx *c) {
                     (void *)c->pf_ntiles, (void *)c->pf_w, (void *)c->pf_ypart, (void *)c->pf_tiles,
                     (void *)c->pf_xg, (void *)c->pf_act})
         cudaFree(q);
+    c->pf_scratch.release();
     for (int r = 0; r < m1::kMaxRanks; ++r)
         if (c->ep_ipc[r]) cudaIpcCloseMemHandle(c->ep_peer[r]);
     cudaFree(c->ep_region);
@@ -695,9 +698,14 @@ m1moe_status pf_make_maps(m1moe_cuda_ctx *c) {
     return M1MOE_OK;
 }
 
-// Scratch for T tokens (grown, never shrunk; a synchronous reallocation).
-m1moe_status pf_reserve(m1moe_cuda_ctx *c, int T) {
+// Scratch for T tokens (grown, never shrunk; a synchronous reallocation that
+// leaves the buffers of captured graphs in place).
+m1moe_status pf_reserve(m1moe_cuda_ctx *c, int T, cudaStream_t stream) {
+    const bool capturing = c->pf_scratch.capturing(stream);
     if (T <= c->pf_cap) return M1MOE_OK;
+    if (capturing)
+        return fail(M1MOE_ERR_INVALID_ARG, "%d tokens need larger buffers, which cannot be made while the stream is "
+                                           "captured: run a prefill of this size before", T);
     const m1moe_cuda_cfg &g = c->cfg;
     const long long pairs = (long long)T * g.top_k;
     const int max_tiles = (int)std::min<long long>(c->ne, pairs) + (int)(pairs / m1::kPfTileTok) + 1;
@@ -708,10 +716,8 @@ m1moe_status pf_reserve(m1moe_cuda_ctx *c, int T) {
     int nsplit = (int)std::max<long long>(1, (4LL * c->num_sms + dn_units - 1) / dn_units);
     nsplit = std::min(nsplit, std::max(1, g.intermediate_dim / 64 / 8));
     M1_CK(cudaDeviceSynchronize());
-    for (void *q : {(void *)c->pf_idx, (void *)c->pf_tok_slot, (void *)c->pf_slot_tok,
-                    (void *)c->pf_ntiles, (void *)c->pf_w, (void *)c->pf_ypart, (void *)c->pf_tiles,
-                    (void *)c->pf_xg, (void *)c->pf_act})
-        cudaFree(q);
+    c->pf_scratch.retire({c->pf_idx, c->pf_tok_slot, c->pf_slot_tok, c->pf_ntiles, c->pf_w, c->pf_ypart, c->pf_tiles,
+                          c->pf_xg, c->pf_act});
     c->pf_idx = c->pf_tok_slot = c->pf_slot_tok = c->pf_ntiles = nullptr;
     c->pf_w = c->pf_ypart = nullptr;
     c->pf_tiles = nullptr;
@@ -1347,7 +1353,7 @@ m1moe_status m1moe_cuda_moe_prefill(m1moe_cuda_ctx *c, int32_t layer, const void
     if (!c->layer_loaded[layer]) return fail(M1MOE_ERR_NOT_LOADED, "experts of layer %d not loaded", layer);
     DeviceGuard dg(g.device);
     if (m1moe_status st = pf_make_maps(c)) return st;
-    if (m1moe_status st = pf_reserve(c, T)) return st;
+    if (m1moe_status st = pf_reserve(c, T, as_stream(stream))) return st;
     m1::PrefillParams p{};
     p.table = c->table + (size_t)layer * c->ne * c->tl.block;
     p.tl = c->tl;
