@@ -103,6 +103,13 @@ struct PagedShape {
     int prefix_rows;     // item rows of the shared prefix's pass: 16 or 256
 };
 
+// First position that a token at position p sees (window 0: all).  Tokens
+// before position 0 see nothing, and a window may be as large as an int:
+// p - window + 1 is formed only where it cannot pass 31 bits.
+__device__ __forceinline__ int first_seen(int p, int window) {
+    return window == 0 || p < window ? 0 : p - window + 1;
+}
+
 // Pool row of position p of sequence b and KV head g, or -1 (with the status
 // bit) if the page table names no page of the pool.
 __device__ __forceinline__ int paged_row(const PagedShape &s, const int *table, int b, int g, int p, int *status) {
@@ -233,9 +240,7 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
             it.nrows = min(s.rows, nrow - r0);
             const int first = t - (q1 - q0) + r0 / s.group;  // position of the first and the last row
             const int last = t - (q1 - q0) + (r0 + it.nrows - 1) / s.group;
-            int lo = prefix;
-            if (s.window > 0) lo = max(lo, first - s.window + 1);
-            it.unit0 = max(lo, 0) / s.unit;
+            it.unit0 = max(prefix, first_seen(first, s.window)) / s.unit;
             // at least one unit, so that an item whose rows see nothing is still written
             n = max(1, (last + s.unit) / s.unit - it.unit0) + (s.rows == kPagedRowsLarge ? kPagedItemCost : 0);
             p.items[i] = it;

@@ -259,9 +259,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
         UnitCursor ld = cur;  // the loader runs ahead
         PagedItem ld_item = p.items[ld.item];
         auto item_lo = [&](const PagedItem &it) {  // first position any row of the item sees
-            int lo = prefix;
-            if (s.window > 0) lo = max(lo, it.len - it.nq + fdiv(it.row0, s.by_group) - s.window + 1);
-            return lo;
+            return max(prefix, first_seen(it.len - it.nq + fdiv(it.row0, s.by_group), s.window));
         };
         int ld_lo = item_lo(ld_item);
         int slot = 0;
@@ -312,15 +310,13 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                 const int row = it.row0 + (ok[h] ? r : 0), tok = fdiv(row, s.by_group);
                 qr[h] = a.q + (long long)(q0 + tok) * a.q_stride + (long long)(cur.g * s.group + row - tok * s.group) * HD;
                 hi[h] = a.partial ? len - 1 : len - nq + tok;
-                lo[h] = prefix;
-                if (s.window > 0) lo[h] = max(lo[h], hi[h] - s.window + 1);
+                lo[h] = max(prefix, first_seen(hi[h], s.window));
                 m[h] = -INFINITY;
                 l[h] = 0.f;
             }
             min_hi = a.partial ? len - 1 : len - nq + fdiv(it.row0, s.by_group);
             const int max_hi = len - nq + fdiv(it.row0 + it.nrows - 1, s.by_group);
-            max_lo = prefix;
-            if (s.window > 0) max_lo = max(max_lo, max_hi - s.window + 1);
+            max_lo = max(prefix, first_seen(max_hi, s.window));
 #pragma unroll
             for (int k = 0; k < KS; ++k)
 #pragma unroll

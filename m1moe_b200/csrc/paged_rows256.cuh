@@ -322,7 +322,7 @@ struct Rows256Walk {
             x.q0 = it.q0;
             x.len = it.len;
             x.first = it.len - it.nq;
-            x.lo = s.window > 0 ? max(0, x.first + fdiv(it.row0, s.by_group) - s.window + 1) : 0;
+            x.lo = first_seen(x.first + fdiv(it.row0, s.by_group), s.window);
         }
         // the next item's record, for the next call
         asm volatile("prefetch.global.L1 [%0];" ::"l"(p.items + item));
@@ -611,11 +611,11 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             const int head = x.g * s.group + r - tok * s.group;
             const bool live = row < n;
             const int hi = a.prefix_run ? x.len - 1 : x.first + tok;
-            const int lo = s.window > 0 && !a.prefix_run ? hi - s.window + 1 : 0;
+            const int lo = a.prefix_run ? 0 : first_seen(hi, s.window);
             // limits that hold for the M-tile's every row
             const int rf = x.row0 + i * kTileRows;
             const int min_hi = a.prefix_run ? x.len - 1 : x.first + fdiv(rf, s.by_group);
-            const int max_lo = s.window > 0 && !a.prefix_run ? x.first + fdiv(rf + n - 1, s.by_group) - s.window + 1 : 0;
+            const int max_lo = a.prefix_run ? 0 : first_seen(x.first + fdiv(rf + n - 1, s.by_group), s.window);
             const int warp_hi = __shfl_sync(0xffffffffu, hi, 0), warp_lo = __shfl_sync(0xffffffffu, lo, 31);
             float m = -INFINITY, l = 0.f;  // the reference maximum (raw scale) and the sum
             for (int j = x.ja; j < x.jb; ++j) {
