@@ -89,7 +89,8 @@ m1moe_status make_shape(const m1moe_paged_cfg *c, int ctas, m1::PagedShape &s) {
     if (c->window < 0 || c->shared_prefix < 0 || c->shared_prefix % c->page_size)
         return fail(M1MOE_ERR_INVALID_ARG, "window %d must be >= 0, shared_prefix %d a multiple of the page size",
                     c->window, c->shared_prefix);
-    if ((long long)c->num_pages * c->num_kv_heads * c->page_size > 0x7FFFFFFFLL ||
+    // (each product of 32-bit sizes is compared before the next factor joins it)
+    if ((long long)c->num_pages * c->page_size > 0x7FFFFFFFLL / c->num_kv_heads ||
         (long long)c->max_pages_per_seq * c->page_size > 0x7FFFFF00LL)
         return fail(M1MOE_ERR_UNSUPPORTED, "the pool's rows and a sequence's positions must fit 31 bits");
     if (c->shared_prefix > (long long)c->max_pages_per_seq * c->page_size)
@@ -119,7 +120,7 @@ m1moe_status make_shape(const m1moe_paged_cfg *c, int ctas, m1::PagedShape &s) {
     s.min_per = small ? m1::kPagedWarps : 1;
     const long long items = c->num_seqs + (long long)c->total_q * group / s.rows;
     const long long cap = (long long)c->max_pages_per_seq * c->page_size;
-    if (items * (cap / s.unit + 1 + m1::kPagedItemCost) * c->num_kv_heads > 0x7FFF0000LL)
+    if (items * (cap / s.unit + 1 + m1::kPagedItemCost) > 0x7FFF0000LL / c->num_kv_heads)
         return fail(M1MOE_ERR_UNSUPPORTED, "the batch's work (%lld items of up to %lld positions) does not fit 31 bits",
                     items, cap);
     s.max_items = (int)items;
