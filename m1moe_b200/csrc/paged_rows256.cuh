@@ -56,6 +56,7 @@ constexpr int kTileRows = 128;              // an M-tile
 constexpr int kRows256Threads = 16 * 32;
 constexpr int kRows256Loaders = 128;
 constexpr float kRescaleLog2 = 8.f;
+constexpr uint32_t kDrainLimit = 1u << 16;  // polls, for copies that take microseconds
 // Registers a thread: the block is launched with 128 each (65,536 / 512); the
 // loader and product warpgroups give theirs up to the two softmax ones, which
 // hold a row of 128 scores: 2 * 200 + 2 * 56 = 4 * 128.
@@ -390,7 +391,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
         const int c = t % kChunks, r0 = t / kChunks;
         const uint32_t kv_addr = smem_addr(skv);
         const int box_shift = min(s.page_shift, 7), boxes = 128 >> box_shift;  // rows of a box, boxes along a tile
-        int tile = 0;  // K and V tiles so far, K first
+        int tile = 0, issued = 0;  // K and V tiles so far, K first; and those whose copies were issued
         bool ok = true;
         auto claim = [&]() {  // the next tile's stage, free
             const int st = tile % T::kStages;
@@ -400,6 +401,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 ok = paged_wait(&kv_empty[pair % T::kPairs], (pair / T::kPairs) & 1, &abort_flag, status);
             ok = __all_sync(0xffffffffu, ok);
             ++tile;
+            if (ok) issued = tile;
             return st;
         };
         int nq0 = 0, nq1 = 0;  // times each M-tile's Q was loaded
@@ -492,6 +494,12 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 }
             }
         }
+        // The last copies land before the CTA leaves: where a wait gave up, here
+        // or in another warp, no product may be waiting for them.
+        cp_async_wait(0);
+        for (int m = max(0, issued - T::kStages); m < issued; ++m)
+            for (uint32_t i = 0; i < kDrainLimit && !mbar_try_wait(&kv_full[m % T::kStages], (m / T::kStages) & 1); ++i) {
+            }
     } else if (warp >= 12) {
         // ---------------------------------------------------------- products
         // The whole warp follows the schedule; one elected lane issues.
