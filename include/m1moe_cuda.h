@@ -505,8 +505,10 @@ M1MOE_API size_t m1moe_cuda_paged_plan_bytes(const m1moe_paged_cfg *cfg);
  * place, the attention's work split over the SMs, and room for its partial
  * results.  Every layer's append and attention of the step read it; after a
  * change of cu_q, kv_len or the page table make it again.  d_plan is
- * 256-byte aligned.  Lengths that contradict cfg raise status bit 1 and the
- * batch is treated as empty. */
+ * 256-byte aligned, and the first 64 bytes of a new buffer are zero: status
+ * bits stay from plan to plan until m1moe_cuda_paged_status reports them.
+ * Lengths that contradict cfg raise status bit 1 and the batch is treated as
+ * empty. */
 M1MOE_API m1moe_status m1moe_cuda_paged_plan(const m1moe_paged_cfg *cfg, const int32_t *d_cu_q,
                                    const int32_t *d_kv_len, const int32_t *d_page_table, void *d_plan,
                                    size_t plan_bytes, void *stream);

@@ -265,7 +265,8 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
         p.start[w] = u < c1 ? upper_index(p.unit_at, items + 1, (int)(u % units)) : 0;
     }
     if (tid == 0) {
-        *p.status = sm_bad;
+        // (bits of earlier steps stay until they are reported)
+        if (sm_bad) atomicOr(p.status, sm_bad);
         p.header[kPhItems] = items;
         p.header[kPhUnits] = units;
         p.header[kPhPer] = per;

@@ -125,7 +125,6 @@ class PagedBatch:
         self.cache, self.page_table, self.kv_lens = cache, page_table, kv_lens
         self.num_seqs, self.total_q, self.max_q = len(q), cu[-1], max(q)
         self.num_heads = num_heads
-        self.cu_q = torch.tensor(cu, dtype=torch.int32, device=dev)
         self.cfg = _lib.PagedCfg(num_heads, cache.num_kv_heads, cache.head_dim, cache.page_size, cache.num_pages,
                                  len(q), page_table.shape[1], cu[-1], max(q), window, shared_prefix)
         self._cfg = ctypes.addressof(self.cfg)
@@ -134,9 +133,12 @@ class PagedBatch:
             if nbytes == 0:
                 msg = _lib.lib().m1moe_cuda_last_error()
                 raise ValueError(f"paged batch refused: {msg.decode() if msg else ''}")
-            # torch's allocations are 512-byte aligned
+        with torch.cuda.stream(stream):  # (None: the current one)
+            self.cu_q = torch.tensor(cu, dtype=torch.int32, device=dev)
+            # torch's allocations are 512-byte aligned; the plan's header starts without status bits
             self.plan = torch.empty(nbytes, dtype=torch.uint8, device=dev)
-        self._home = _raw_stream(dev.index)
+            self.plan[:64].zero_()
+        self._home = _raw_stream(dev.index) if stream is None else stream.cuda_stream
         self._plan, self._table = self.plan.data_ptr(), page_table.data_ptr()
         self._q_shape = (cu[-1], num_heads, cache.head_dim)
         self._qkv_shape = (cu[-1], (num_heads + 2 * cache.num_kv_heads) * cache.head_dim)
@@ -156,7 +158,8 @@ class PagedBatch:
                              f"{self.cache._sizes()}, not {cache._sizes()}")
 
     def check(self, *, stream=None) -> None:
-        """Wait for the stream and raise if a kernel found a length, page or position out of range."""
+        """Wait for the stream and raise if a kernel found a length, page or position out of range, in any
+        step since the last check."""
         _status_call(self.cache._index, self._plan, self._use(stream))
 
     def _use(self, stream) -> int:
