@@ -266,7 +266,7 @@ m1moe_status launch_rows16(const m1::PagedShape &s, const m1::PagedPlanView &v, 
     const int budget = (int)(kRows16SmemCap / m1::kPagedWarps);
     a.stages = std::min(4, (budget - part) / unit);
     const size_t smem = (size_t)m1::kPagedWarps * (a.stages * unit + part);
-    auto kern = m1::k_paged_rows16<HD>;
+    auto kern = a.cap > 0.f ? m1::k_paged_rows16<HD, true> : m1::k_paged_rows16<HD, false>;
     P_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRows16SmemCap));
     return launch_pdl(kern, dim3(s.ctas), dim3(m1::kPagedWarps * 32), smem, st, "k_paged_rows16 launch", s, v, a);
 }

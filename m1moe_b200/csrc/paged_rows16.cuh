@@ -55,14 +55,34 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-// The score in units of log2: cap * tanh(s / cap) * log2(e), or s * log2(e).
-// tanh(x) = 1 - 2 / (1 + e^2x): the absolute error stays near 1e-7.
-__device__ __forceinline__ float score_log2(float dot, float scale_log2, float cap, float two_over_cap_scaled) {
-    if (cap > 0.f) {
-        const float e = exp2_approx(dot * two_over_cap_scaled);
-        return cap * kLog2e * (1.f - __fdividef(2.f, 1.f + e));
-    }
-    return dot * scale_log2;
+// tanh(x) / x as a polynomial in y = x^2 for |x| <= 1, degree 5 (least largest
+// relative error, 5.9e-7, by Remez exchange).
+constexpr float kTanh0 = 0.9999994039535522f, kTanh1 = -0.3332904279232025f, kTanh2 = 0.13281433284282684f,
+                kTanh3 = -0.051605675369501114f, kTanh4 = 0.016743114218115807f, kTanh5 = -0.003067060373723507f;
+
+// A capped score in units of log2: cap * tanh(x) * log2(e) with x = score / cap
+// = dot * cs; `near` is its value where |x| <= 1: score * log2(e) * tanh(x) / x.
+// Beyond, tanh(x) = 1 - 2 / (1 + e^2x).  The error is relative to the score,
+// whatever the cap: 1e-7 of the second form is beside a value above 0.76.
+__device__ __forceinline__ float cap_far(float x, float cap) {
+    return cap * kLog2e * (1.f - __fdividef(2.f, 1.f + exp2_approx(x * (2.f * kLog2e))));
+}
+__device__ __forceinline__ float cap_score(float x, float near, float cap) {
+    const float far = cap_far(x, cap);
+    float r;  // (where the compiler branches here, most warps take both sides, element after element)
+    asm("{ .reg .pred p; setp.le.f32 p, %1, 0f3F800000; selp.f32 %0, %2, %3, p; }"
+        : "=f"(r)
+        : "f"(fabsf(x)), "f"(near), "f"(far));
+    return r;
+}
+__device__ __forceinline__ float cap_score(float dot, float scale_log2, float cap, float cs) {
+    const float x = dot * cs, y = x * x;
+    float t = fmaf(kTanh5, y, kTanh4);
+    t = fmaf(t, y, kTanh3);
+    t = fmaf(t, y, kTanh2);
+    t = fmaf(t, y, kTanh1);
+    t = fmaf(t, y, kTanh0);
+    return cap_score(x, dot * scale_log2 * t, cap);
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void *src, bool valid) {
@@ -224,7 +244,11 @@ struct Rows16Left {
     int open_right, open_left, g, item;
 };
 
-template <int HD>
+// kCap: scores are capped (a.cap > 0).  A kernel of its own each: what one step
+// of one short sequence takes is much the first fetch of its code (us in one
+// kernel for both, and in two: one uncapped token over 2048 positions 12.8 and
+// 12.3; 64 sequences to 16,000 114 and 112; 200 on a shared prefix 198 and 195).
+template <int HD, bool kCap>
 __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const PagedShape s, const PagedPlanView p,
                                                                       const RowsParams a) {
     constexpr int E = HD / 32, KS = HD / 16, NT = HD / 8, CH = HD / 8;  // CH: 16-byte chunks per row
@@ -296,7 +320,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
         float o[NT][4], m[2], l[2];
         int hi[2], lo[2];  // positions the lane's two rows see
         int min_hi = 0, max_lo = 0;
-        const float sl2 = a.scale * kLog2e, c2 = a.cap > 0.f ? 2.f * a.scale / a.cap * kLog2e : 0.f;
+        const float sl2 = a.scale * kLog2e, cs = kCap ? a.scale / a.cap : 0.f;
         PagedItem it;
         auto open_segment = [&]() {
             it = p.items[cur.item];
@@ -415,12 +439,23 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
             const int pos = (it.unit0 + cur.u - cur.seg0) * kPagedUnitSmall;
             float mx[2] = {m[0], m[1]};
             const bool whole = pos >= max_lo && pos + kPagedUnitSmall - 1 <= min_hi;
+            if constexpr (kCap) {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sc[t][j] = cap_score(sc[t][j], sl2, a.cap, cs);
+            } else {
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) sc[t][j] *= sl2;
+            }
 #pragma unroll
             for (int t = 0; t < 2; ++t)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int h = j >> 1;
-                    float x = score_log2(sc[t][j], sl2, a.cap, c2);
+                    float x = sc[t][j];
                     if (!whole) {
                         const int at = pos + 8 * t + 2 * (lane & 3) + (j & 1);
                         if (at > hi[h] || at < lo[h]) x = -INFINITY;

@@ -185,12 +185,14 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
-// 32 raw scores capped, in units of log2: cap tanh(x) log2 e with x = score *
-// scale / cap.  While |x| <= 1 throughout the warp, tanh(x) / x is a degree-5
-// polynomial in x^2 (least largest relative error, 5.9e-7, by Remez
-// exchange); beyond, tanh(x) = 1 - 2 / (1 + e^2x).
-__device__ __forceinline__ void cap_scores(uint32_t (&v)[32], float scale_log2, float cap) {
-    const float cs = scale_log2 / (cap * kLog2e);
+// 32 raw scores capped, in units of log2: by the polynomial, two at a time,
+// while |x| <= 1 throughout the warp, and score by score where not.  Up to a
+// cap of kFarCap the second form serves there for the small scores too: its
+// error, 1e-7 of the cap, is at most 4e-5 of a score's units, beside a weight's
+// rounding of 2^-9 (4096 tokens of 32/8 heads with scores mostly above the cap:
+// 328 us so, 374 with both forms of each).
+constexpr float kFarCap = 256.f;
+__device__ __forceinline__ void cap_scores(uint32_t (&v)[32], float scale_log2, float cap, float cs) {
     float top = 0.f;
 #pragma unroll
     for (int e = 0; e < 32; ++e) top = fmaxf(top, fabsf(__uint_as_float(v[e])));
@@ -200,21 +202,22 @@ __device__ __forceinline__ void cap_scores(uint32_t (&v)[32], float scale_log2, 
         for (int e = 0; e < 32; e += 2) {
             const uint64_t d = pack2(__uint_as_float(v[e]), __uint_as_float(v[e + 1]));
             const uint64_t x = mul2(d, c2), y = mul2(x, x);
-            uint64_t t = fma2(pack2(-0.003067060373723507f, -0.003067060373723507f), y,
-                              pack2(0.016743114218115807f, 0.016743114218115807f));
-            t = fma2(t, y, pack2(-0.051605675369501114f, -0.051605675369501114f));
-            t = fma2(t, y, pack2(0.13281433284282684f, 0.13281433284282684f));
-            t = fma2(t, y, pack2(-0.3332904279232025f, -0.3332904279232025f));
-            t = fma2(t, y, pack2(0.9999994039535522f, 0.9999994039535522f));
+            uint64_t t = fma2(pack2(kTanh5, kTanh5), y, pack2(kTanh4, kTanh4));
+            t = fma2(t, y, pack2(kTanh3, kTanh3));
+            t = fma2(t, y, pack2(kTanh2, kTanh2));
+            t = fma2(t, y, pack2(kTanh1, kTanh1));
+            t = fma2(t, y, pack2(kTanh0, kTanh0));
             float a, b;
             unpack2(mul2(mul2(d, s2), t), a, b);
             v[e] = __float_as_uint(a);
             v[e + 1] = __float_as_uint(b);
         }
+    } else if (cap <= kFarCap) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(cap_far(__uint_as_float(v[e]) * cs, cap));
     } else {
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-            v[e] = __float_as_uint(score_log2(__uint_as_float(v[e]), 0.f, cap, 2.f * cs * kLog2e));
+        for (int e = 0; e < 32; ++e) v[e] = __float_as_uint(cap_score(__uint_as_float(v[e]), scale_log2, cap, cs));
     }
 }
 
@@ -645,7 +648,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                             uint32_t y[32];
                             tmem_ld32(ts + 32 * q, y);
                             tmem_wait_ld();
-                            if (capped) cap_scores(y, a.r.scale * kLog2e, a.r.cap);
+                            if (capped) cap_scores(y, a.r.scale * kLog2e, a.r.cap, a.r.scale / a.r.cap);
                             if (hides) {
 #pragma unroll
                                 for (int e = 0; e < 32; ++e)

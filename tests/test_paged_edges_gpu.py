@@ -50,3 +50,20 @@ def test_a_new_batch_starts_without_status_bits():
             paged_attention(cache, 0, batch, q, **kw)
             batch.check(**kw)
             del batch
+
+
+@pytest.mark.parametrize("cap", [300.0, 1e4, 1e6, 1e8, 3e38])
+@pytest.mark.parametrize("hd,q_lens,kv_lens", [(128, [1, 1, 1], [1, 700, 33]), (64, [2, 1], [90, 64]),
+                                               (128, [70, 200], [300, 200]), (64, [130], [130])])
+def test_caps_far_above_the_scores(hd, q_lens, kv_lens, cap):
+    """cap tanh(s / cap) of scores between a ten-thousandth and a few times the cap: as the cap grows the
+    result is the uncapped one.  Errors of tanh are relative (6e-7 at most), so scores of up to about 20 are
+    off by about 1e-5, far inside the bar's 2^-11."""
+    nh, nkv = 16, 4
+    cache, table, dense = make(nkv, hd, 16, q_lens, kv_lens, seed=33)
+    q = (3 * torch.randn((sum(q_lens), nh, hd), device="cuda")).bfloat16()
+    batch = PagedBatch(cache, q_lens, kv_lens, table, num_heads=nh)
+    out = paged_attention(cache, 0, batch, q, softcap=cap, out_dtype=torch.float32)
+    batch.check()
+    ref, mag = attention_ref(q, dense, q_lens, kv_lens, nkv, 1 / math.sqrt(hd), 0, cap)
+    check_attention(out, ref, mag)
