@@ -536,8 +536,9 @@ M1MOE_API m1moe_status m1moe_cuda_paged_append(const m1moe_paged_cfg *cfg, const
  *   out = softmax(c(scale * q . k)) . v over positions max(0, p - window + 1) .. p,
  * c(s) = softcap * tanh(s / softcap), or s if softcap is 0.  d_q bf16, rows
  * q_stride elements apart, heads contiguous; d_out likewise (f32 or bf16).
- * fp32 scores, maxima, sums and accumulators; the weights enter the second
- * product as bf16.  The split over SMs depends on the lengths alone and
+ * A row's sums take the positions that it sees and no others, also where K or
+ * V of another one is infinite or NaN.  fp32 scores, maxima, sums and
+ * accumulators; the weights enter the second product as bf16.  The split over SMs depends on the lengths alone and
  * partials are merged in position order: the result is the same every time.
  * It uses the plan's partials, so calls on one plan must be ordered on one
  * stream.  Replaces encodeAttention (InferenceEngine.swift:349-399). */

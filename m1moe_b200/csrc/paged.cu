@@ -259,16 +259,24 @@ m1moe_status launch_rows256(const m1::PagedShape &s, const m1::PagedPlanView &v,
                       "k_paged_join launch", s, v, a);
 }
 
-template <int HD>
+template <int HD, bool kCap, bool kMany>
 m1moe_status launch_rows16(const m1::PagedShape &s, const m1::PagedPlanView &v, m1::RowsParams a, cudaStream_t st) {
     // the ring takes what the partials' rows leave, 2 to 4 stages a warp
     const int unit = m1::rows16_unit_bytes<HD>(), part = a.part_rows * HD * 4;
     const int budget = (int)(kRows16SmemCap / m1::kPagedWarps);
     a.stages = std::min(4, (budget - part) / unit);
     const size_t smem = (size_t)m1::kPagedWarps * (a.stages * unit + part);
-    auto kern = a.cap > 0.f ? m1::k_paged_rows16<HD, true> : m1::k_paged_rows16<HD, false>;
+    auto kern = m1::k_paged_rows16<HD, kCap, kMany>;
     P_CK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kRows16SmemCap));
     return launch_pdl(kern, dim3(s.ctas), dim3(m1::kPagedWarps * 32), smem, st, "k_paged_rows16 launch", s, v, a);
+}
+
+template <int HD>
+m1moe_status launch_rows16(const m1::PagedShape &s, const m1::PagedPlanView &v, const m1::RowsParams &a,
+                           cudaStream_t st) {
+    const bool many = s.max_q > 1 && !a.partial;  // (all rows see all of a shared prefix)
+    if (a.cap > 0.f) return many ? launch_rows16<HD, true, true>(s, v, a, st) : launch_rows16<HD, true, false>(s, v, a, st);
+    return many ? launch_rows16<HD, false, true>(s, v, a, st) : launch_rows16<HD, false, false>(s, v, a, st);
 }
 
 template <int HD>

@@ -55,6 +55,7 @@ enum PagedHeader {
     kPhUnits = 2,   // units per KV head
     kPhPer = 3,     // units per CTA
     kPhPrefix = 4,  // positions of the shared prefix in use (0: none)
+    kPhOdd = 5,     // a 256-row item's sums met an infinity or a NaN since the plan was made
     kPhWords = 16
 };
 
@@ -271,6 +272,7 @@ __global__ void __launch_bounds__(1024) k_paged_plan(const PagedShape s, const P
         p.header[kPhUnits] = units;
         p.header[kPhPer] = per;
         p.header[kPhPrefix] = prefix;
+        p.header[kPhOdd] = 0;
     }
     if (s.prefix == 0) return;
     // the prefix's own split: all rows of the batch, 16 or 256 at a time,

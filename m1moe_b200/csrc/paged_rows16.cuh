@@ -123,6 +123,164 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// Infinities and NaN in V.  A row's weight of a position that it does not see is
+// 0, and so is its product with that position's V -- unless V is infinite or NaN
+// there.  Where rows of one item see different positions and a row's sums have
+// come out infinite or NaN, they are taken again by what follows, one thread a
+// row and some columns, over the positions that the row sees and no others.
+// (Functions of their own, called after the loops that always run: within these
+// their calls cost 4 %, their code 2 to 7 %.)
+struct SeenRow {
+    const uint16_t *q, *k, *v;  // the row's query; the pools
+    const int *pages;           // the sequence's row of the page table
+    int nkv, g, page_shift, num_pages, p0, p1;
+    float scale_log2, cap, cs, ref;  // ref: the maximum that the row's weights are relative to
+};
+template <int N>
+struct Columns {
+    float x[N];
+};
+// The pool row of position p, or -1 (its K and V count as zeros; the copies have
+// reported the page).
+__device__ __forceinline__ long long seen_at(const SeenRow &r, int p) {
+    const int page = __ldg(r.pages + (p >> r.page_shift));
+    if ((unsigned)page >= (unsigned)r.num_pages) return -1;
+    return ((long long)page * r.nkv + r.g) << r.page_shift | (p & ((1 << r.page_shift) - 1));
+}
+// Its score in units of log2.
+template <int HD>
+__device__ __forceinline__ float seen_score(const SeenRow &r, long long row) {
+    const uint32_t *k = reinterpret_cast<const uint32_t *>(r.k + row * HD), *q = reinterpret_cast<const uint32_t *>(r.q);
+    float dot = 0.f;
+#pragma unroll 4
+    for (int d = 0; d < HD / 2; ++d) {
+        const uint32_t a = q[d], b = k[d];
+        dot = fmaf(__uint_as_float(a << 16), __uint_as_float(b << 16), dot);
+        dot = fmaf(__uint_as_float(a & 0xFFFF0000u), __uint_as_float(b & 0xFFFF0000u), dot);
+    }
+    return r.cap > 0.f ? cap_score(dot, r.scale_log2, r.cap, r.cs) : dot * r.scale_log2;
+}
+// N columns from `col` on.
+template <int HD, int N>
+__device__ __noinline__ Columns<N> sum_seen(const SeenRow r, int col) {
+    Columns<N> o;
+#pragma unroll
+    for (int e = 0; e < N; ++e) o.x[e] = 0.f;
+#pragma unroll 1
+    for (int p = r.p0; p <= r.p1; ++p) {
+        const long long row = seen_at(r, p);
+        if (row < 0) continue;
+        const uint32_t *v = reinterpret_cast<const uint32_t *>(r.v + row * HD + col);
+        const float w = __bfloat162float(__float2bfloat16_rn(exp2_approx(seen_score<HD>(r, row) - r.ref)));
+#pragma unroll
+        for (int e = 0; e < N; e += 2) {
+            const uint32_t b = v[e / 2];
+            o.x[e] = fmaf(w, __uint_as_float(b << 16), o.x[e]);
+            o.x[e + 1] = fmaf(w, __uint_as_float(b & 0xFFFF0000u), o.x[e + 1]);
+        }
+    }
+    return o;
+}
+// Row `row` of an item, from position `from` on; m: its largest score.
+template <int HD>
+__device__ __forceinline__ SeenRow seen_row(const PagedShape &s, const RowsParams &a, const PagedItem &it, int g, int row,
+                                            int from, float m) {
+    const int tok = fdiv(row, s.by_group);
+    SeenRow x;
+    x.q = a.q + (long long)(it.q0 + tok) * a.q_stride + (long long)(g * s.group + row - tok * s.group) * HD;
+    x.k = a.k, x.v = a.v;
+    x.pages = a.table + (size_t)it.seq * s.max_pages;
+    x.nkv = s.nkv, x.g = g, x.page_shift = s.page_shift, x.num_pages = s.num_pages;
+    x.p1 = it.len - it.nq + tok;
+    x.p0 = max(from, first_seen(x.p1, s.window));
+    x.scale_log2 = a.scale * kLog2e, x.cap = a.cap, x.cs = a.cap > 0.f ? a.scale / a.cap : 0.f;
+    x.ref = m == -INFINITY ? 0.f : m;
+    return x;
+}
+// Which of columns col .. col + n - 1 (n even, at most 64) of V at position p are infinite or NaN.
+__device__ __forceinline__ unsigned long long odd_columns(const SeenRow &r, int hd, int p, int col, int n) {
+    const long long row = seen_at(r, p);
+    if (row < 0) return 0;
+    const uint32_t *v = reinterpret_cast<const uint32_t *>(r.v + row * hd + col);
+    unsigned long long odd = 0;
+#pragma unroll 4
+    for (int e = 0; e < n; e += 2) {
+        const uint32_t b = v[e / 2];
+        odd |= (unsigned long long)(((b & 0x7F80u) == 0x7F80u ? 1 : 0) | ((b & 0x7F800000u) == 0x7F800000u ? 2 : 0)) << e;
+    }
+    return odd;
+}
+// Columns col .. col + n - 1 (n a multiple of 8, at most 64) of a row's result,
+// summed again where they are infinite or NaN and a position that came in with
+// the item's units, but that this row does not see, may be why.
+template <int HD>
+__device__ __noinline__ void mend_row(const PagedShape s, const RowsParams a, const PagedItem it, int g, int row, int col,
+                                      int n) {
+    const int tok = fdiv(row, s.by_group);
+    const long long at = (long long)(it.q0 + tok) * a.out_stride + (long long)(g * s.group + row - tok * s.group) * HD + col;
+    __nv_bfloat16 *narrow = reinterpret_cast<__nv_bfloat16 *>(a.out) + at;
+    float *wide = reinterpret_cast<float *>(a.out) + at;
+    unsigned long long odd = 0, why = 0;
+    for (int c = 0; c < n; ++c) {
+        const float y = a.out_bf16 ? __bfloat162float(narrow[c]) : wide[c];
+        odd |= (unsigned long long)(y * 0.f != 0.f) << c;
+    }
+    if (!odd) return;
+    SeenRow x = seen_row<HD>(s, a, it, g, row, 0, 0.f);
+    // (with such a value at its own position the result is none but these)
+    if (x.p1 >= 0) odd &= ~odd_columns(x, HD, x.p1, col, n);
+    const int p0 = it.len - it.nq + fdiv(it.row0, s.by_group), p1 = it.len - it.nq + fdiv(it.row0 + it.nrows - 1, s.by_group);
+    const int end = p1 < 0 ? 0 : min(it.len, (p1 / s.unit + 1) * s.unit);  // of the item's last unit
+    for (int p = first_seen(p0, s.window); p < x.p0; ++p) why |= odd_columns(x, HD, p, col, n);
+    for (int p = max(0, x.p1 + 1); p < end; ++p) why |= odd_columns(x, HD, p, col, n);
+    odd &= why;
+    if (!odd) return;
+    float m = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (int p = x.p0; p <= x.p1; ++p) {
+        const long long r = seen_at(x, p);
+        const float y = r < 0 ? 0.f : seen_score<HD>(x, r), top = fmaxf(m, y);
+        l = l * (m == -INFINITY ? 0.f : exp2_approx(m - top)) + (y == -INFINITY ? 0.f : exp2_approx(y - top));
+        m = top;
+    }
+    x.ref = m == -INFINITY ? 0.f : m;
+    const float f = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll 1
+    for (int c = 0; c < n; c += 8) {
+        if (!(odd >> c & 0xFF)) continue;
+        const Columns<8> y = sum_seen<HD, 8>(x, col + c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            if (!(odd >> (c + e) & 1)) continue;
+            if (a.out_bf16)
+                narrow[c + e] = __float2bfloat16_rn(y.x[e] * f);
+            else
+                wide[c + e] = y.x[e] * f;
+        }
+    }
+}
+// The rows of the items that lie whole in a warp's units [begin, end), half a
+// row a lane, and of the items that its CTA joined.
+template <int HD>
+__device__ __noinline__ void mend_finished(const PagedShape s, const PagedPlanView p, const RowsParams a, int begin, int end,
+                                           int item, const int2 *done, int done_n) {
+    const int units = p.header[kPhUnits], items = p.header[kPhItems], lane = threadIdx.x & 31;
+    for (int g = begin < end ? begin / units : 0; begin < end;) {
+        const int seg0 = g * units + p.unit_at[item], seg1 = g * units + p.unit_at[item + 1];
+        if (seg1 > end) break;
+        const PagedItem it = p.items[item];
+        if (seg0 >= begin && (lane & 15) < it.nrows)
+            mend_row<HD>(s, a, it, g, it.row0 + (lane & 15), (lane >> 4) * (HD / 2), HD / 2);
+        if (seg1 == end) break;
+        if (++item == items) item = 0, ++g;
+    }
+    for (int k = 0; k < done_n; ++k) {
+        const PagedItem it = p.items[done[k].y];
+        for (int r = threadIdx.x >> 5; r < it.nrows; r += kPagedWarps)
+            if (lane < HD / 8) mend_row<HD>(s, a, it, done[k].x, it.row0 + r, lane * 8, 8);
+    }
+}
+
 // A warp's place in the work: unit u of [u, end) lies in item `item` of KV
 // head g; [seg0, seg1) are that item's units.
 struct UnitCursor {
@@ -244,11 +402,13 @@ struct Rows16Left {
     int open_right, open_left, g, item;
 };
 
-// kCap: scores are capped (a.cap > 0).  A kernel of its own each: what one step
-// of one short sequence takes is much the first fetch of its code (us in one
-// kernel for both, and in two: one uncapped token over 2048 positions 12.8 and
-// 12.3; 64 sequences to 16,000 114 and 112; 200 on a shared prefix 198 and 195).
-template <int HD, bool kCap>
+// kCap: scores are capped (a.cap > 0).  kMany: rows of an item may see different
+// positions (several new tokens of a sequence).  A kernel of its own each: what
+// one step of one short sequence takes is much the first fetch of its code (us in
+// one kernel for both caps, and in two: one uncapped token over 2048 positions
+// 12.8 and 12.3; 64 sequences to 16,000 114 and 112; 200 on a shared prefix 198
+// and 195).
+template <int HD, bool kCap, bool kMany>
 __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const PagedShape s, const PagedPlanView p,
                                                                       const RowsParams a) {
     constexpr int E = HD / 32, KS = HD / 16, NT = HD / 8, CH = HD / 8;  // CH: 16-byte chunks per row
@@ -257,6 +417,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
     __shared__ Rows16Left left[kPagedWarps];
     __shared__ float2 ml_front[kPagedWarps][kPagedRowsSmall], ml_last[kPagedWarps][kPagedRowsSmall];
     __shared__ int sm_last;
+    __shared__ int2 done[kPagedWarps + 2];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, cta = blockIdx.x;
     const int warp_bytes = a.stages * kUnit + a.part_rows * HD * 4;
     uint8_t *ring = smem + (size_t)warp * warp_bytes;
@@ -276,6 +437,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
     const bool work = cur.u < cur.end;
     const int begin = cur.u;
     Rows16Left mine = {0, 0, 0, 0, 0, 0, 0};
+    [[maybe_unused]] float odd = 0.f;  // NaN once a finished row's sums were infinite or NaN
     if (work) {
         cur.g = cur.u / units;
         cur.item = start;
@@ -508,6 +670,12 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
             if (cur.u + 1 == cur.seg1) {
                 row_sums();
                 if (cur.seg0 >= begin) {
+                    if constexpr (kMany) {
+                        float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                        for (int n = 0; n < NT; ++n) z[n & 3] += (o[n][0] + o[n][1]) + (o[n][2] + o[n][3]);
+                        odd = fmaf((z[0] + z[1]) + (z[2] + z[3]), 0.f, odd);
+                    }
                     write_rows();  // the whole item was this warp's
                 } else {
                     store_partial(front, ml_front[warp]);
@@ -527,14 +695,29 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
     }
     if (lane == 0) left[warp] = mine;
     __syncthreads();
+    // The items that this CTA joins and finishes (one a warp at most, and two cut by its run's ends).
+    int done_n = 0;
+    auto note = [&](const float (&o)[E]) {
+        if constexpr (kMany) {
+#pragma unroll
+            for (int e = 0; e < E; ++e) odd = fmaf(o[e], 0.f, odd);
+        }
+    };
+    auto finished = [&](int g, int item) {
+        if constexpr (kMany) {
+            if (threadIdx.x == 0) done[done_n] = make_int2(g, item);
+            ++done_n;
+        }
+    };
     // The warps' unfinished segments, joined item by item in position order:
     // a group starts at a warp whose last segment begins its item (or at warp
     // 0, whatever it begins with) and runs on over the following warps.
     // Every warp takes every eighth row.
     auto join = [&](int w0, bool from_front, int n, bool closed, bool open_left, int g, int item) {
         const PagedItem it = p.items[item];
-        const int q0 = it.q0, pre = it.len > 0 ? prefix : 0;
-        const bool done = closed && !open_left;
+        const int pre = it.len > 0 ? prefix : 0;
+        const bool whole = closed && !open_left;
+        if (whole) finished(g, item);
         const int slot = 2 * cta + (open_left ? 0 : 1);
         for (int r = warp; r < it.nrows; r += kPagedWarps) {
             float m, l, o[E];
@@ -549,8 +732,9 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                 },
                 m, l, o);
             const int row = it.row0 + r, tok = fdiv(row, s.by_group);
-            if (done) {
-                finish_row<HD>(s, a, pre, q0 + tok, g * s.group + row - tok * s.group, m, l, o);
+            if (whole) {
+                note(o);
+                finish_row<HD>(s, a, pre, it.q0 + tok, g * s.group + row - tok * s.group, m, l, o);
             } else {
                 const size_t at = (size_t)slot * a.part_rows + r;
                 store_vec<HD>(p.part + at * HD + lane * E, o);
@@ -593,7 +777,7 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
         if (!sm_last) continue;
         __threadfence();
         const PagedItem it = p.items[item];
-        const int q0 = it.q0, pre = it.len > 0 ? prefix : 0;
+        const int pre = it.len > 0 ? prefix : 0;
         for (int r = warp; r < it.nrows; r += kPagedWarps) {
             float m, l, o[E];
             merge_partials<HD>(
@@ -607,8 +791,13 @@ __global__ void __launch_bounds__(kPagedWarps * 32, 1) k_paged_rows16(const Page
                 },
                 m, l, o);
             const int row = it.row0 + r, tok = fdiv(row, s.by_group);
-            finish_row<HD>(s, a, pre, q0 + tok, g * s.group + row - tok * s.group, m, l, o);
+            note(o);
+            finish_row<HD>(s, a, pre, it.q0 + tok, g * s.group + row - tok * s.group, m, l, o);
         }
+        finished(g, item);
+    }
+    if constexpr (kMany) {
+        if (__syncthreads_or(odd != odd)) mend_finished<HD>(s, p, a, work ? begin : 0, work ? cur.end : 0, start, done, done_n);
     }
 }
 

@@ -766,10 +766,17 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 for (int e = 0; e < 16; ++e) o[e] = __uint_as_float(v[e]);
             };
             const float f = a.prefix_run ? 1.f : ll == 0.f ? 0.f : 1.f / ll;
+            float odd = 0.f;  // NaN once an element of O is infinite or NaN
 #pragma unroll 1
             for (int q = 0; q < HD / 16; ++q) {
                 float o[16];
                 read_o(q, o);
+                uint64_t t[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) t[e] = add2(pack2(o[4 * e], o[4 * e + 1]), pack2(o[4 * e + 2], o[4 * e + 3]));
+                float ta, tb;
+                unpack2(add2(add2(t[0], t[1]), add2(t[2], t[3])), ta, tb);
+                odd = fmaf(ta + tb, 0.f, odd);
                 if (whole) {
                     put(f, 16 * q, o);
                 } else if (live) {
@@ -779,6 +786,10 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                         d[e * kTileRows] = make_float4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
                 }
             }
+            // A row's weight of a position that it does not see is 0, and so is its
+            // product with that position's V, unless V is infinite or NaN there:
+            // k_paged_join then sums such rows again.
+            if (odd != odd && live && !a.prefix_run) p.header[kPhOdd] = 1;
             if (live) {
                 if (!whole)
                     *part_ml_at(slot) = make_float2(mm, ll);
@@ -796,15 +807,29 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
     }
 }
 
+// Where k_paged_rows256 met infinities or NaN: the rows of the items that the
+// split did not cut whose results are such, again by the formula.  Blocks take
+// the items in turn.
+template <int HD>
+__device__ __noinline__ void mend_whole_items(const PagedShape s, const PagedPlanView p, const RowsParams a) {
+    const int i = blockIdx.y, col = 32 * blockIdx.z, row = threadIdx.x;
+    const int units = p.header[kPhUnits], items = p.header[kPhItems], per = p.header[kPhPer];
+    for (int k = blockIdx.x; k < items * s.nkv; k += gridDim.x) {
+        const int g = k / items, item = k - g * items;
+        const int seg0 = g * units + p.unit_at[item] + kPagedItemCost, seg1 = g * units + p.unit_at[item + 1];
+        const PagedItem it = p.items[item];
+        if (seg0 / per != (seg1 - 1) / per || i * kTileRows + row >= it.nrows) continue;
+        mend_row<HD>(s, a, it, g, it.row0 + i * kTileRows + row, col, 32);
+    }
+}
+
 // The items that the split cut: block (c, M-tile, 32 columns) joins, in
 // position order, the partials of the item that begins in CTA c's run and
 // does not end there (a run begins at most one such item).  A thread a row.
 template <int HD>
-__global__ void __launch_bounds__(kTileRows) k_paged_join(const PagedShape s, const PagedPlanView p,
-                                                          const Rows256Params a) {
-    pdl_wait();
+__device__ __forceinline__ void join_cut_item(const PagedShape &s, const PagedPlanView &p, const Rows256Params &a, int units,
+                                              int per, int odd) {
     const int c = blockIdx.x, i = blockIdx.y, col = 32 * blockIdx.z, row = threadIdx.x;
-    const int units = p.header[kPhUnits], per = p.header[kPhPer];
     const int all = units * s.nkv, cut = (c + 1) * per;
     if ((long long)(c + 1) * per >= all) return;
     const int g = cut / units, item = p.start[c + 1];
@@ -858,6 +883,15 @@ __global__ void __launch_bounds__(kTileRows) k_paged_join(const PagedShape s, co
             *reinterpret_cast<float4 *>(d + e) = make_float4(o[e] * f, o[e + 1] * f, o[e + 2] * f, o[e + 3] * f);
         if (a.prefix_run && col == 0) a.partial_ml[token * s.nh + head] = make_float2(m, l);
     }
+    if (odd) mend_row<HD>(s, a.r, it, g, r, col, 32);
+}
+template <int HD>
+__global__ void __launch_bounds__(kTileRows) k_paged_join(const PagedShape s, const PagedPlanView p,
+                                                          const Rows256Params a) {
+    pdl_wait();
+    const int units = p.header[kPhUnits], per = p.header[kPhPer], odd = a.prefix_run ? 0 : p.header[kPhOdd];
+    join_cut_item<HD>(s, p, a, units, per, odd);
+    if (odd) mend_whole_items<HD>(s, p, a.r);
 }
 
 }  // namespace m1

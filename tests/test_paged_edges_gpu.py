@@ -67,3 +67,54 @@ def test_caps_far_above_the_scores(hd, q_lens, kv_lens, cap):
     batch.check()
     ref, mag = attention_ref(q, dense, q_lens, kv_lens, nkv, 1 / math.sqrt(hd), 0, cap)
     check_attention(out, ref, mag)
+
+
+def attention_seen(q, dense, q_lens, kv_lens, nkv, scale, window):
+    """The formula in 64 bits, its sums over the positions a row sees and nothing else; and sum w |v|."""
+    ref = torch.zeros(q.shape, dtype=torch.float64, device="cuda")
+    mag, at, group = torch.zeros_like(ref), 0, q.shape[1] // nkv
+    for (k, v), a, t in zip(dense, q_lens, kv_lens):
+        for i in range(a):
+            hi = t - a + i
+            lo = max(0, hi - window + 1) if window else 0
+            ks, vs = k[lo:hi + 1].double(), v[lo:hi + 1].double()
+            x = q[at + i].double().view(nkv, group, -1)
+            w = torch.softmax(torch.einsum("hgd,thd->hgt", x, ks) * scale, -1)
+            ref[at + i] = torch.einsum("hgt,thd->hgd", w, vs).reshape(-1, q.shape[2])
+            mag[at + i] = torch.einsum("hgt,thd->hgd", w, vs.abs()).reshape(-1, q.shape[2])
+        at += a
+    return ref, mag
+
+
+@pytest.mark.parametrize("nh,nkv,hd,page,q_lens,kv_lens,window", [
+    (16, 4, 128, 16, [4, 1, 3], [30, 50, 3], 0),            # 16-row items
+    (8, 4, 64, 32, [8, 2], [100, 17], 3),
+    (16, 4, 128, 16, [60, 1, 200], [60, 300, 290], 0),      # 256-row items, whole tiles and edges
+    (16, 4, 128, 64, [300, 40], [700, 40], 50),
+    (4, 4, 64, 128, [270], [270], 0),
+    (32, 2, 128, 16, [70], [3000], 0),                      # an item cut over many runs
+])
+@pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
+def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(nh, nkv, hd, page, q_lens, kv_lens, window, value):
+    """A V element that is no finite number belongs to the sums of the rows that see its position; the
+    rows before it (and those whose window has passed it) are what they were."""
+    cache, table, dense = make(nkv, hd, page, q_lens, kv_lens, seed=34)
+    q = torch.randn((sum(q_lens), nh, hd), device="cuda").bfloat16()
+    dense = [(k.clone(), v.clone()) for k, v in dense]
+    for b, (a, t) in enumerate(zip(q_lens, kv_lens)):
+        # in the middle of the new tokens, at the last one, and (windowed: passed by some rows) before them
+        for pos, col in ((t - a + a // 2, 3), (t - 1, hd - 1), (max(0, t - a - 1), hd // 2)):
+            if pos == 0:
+                continue
+            dense[b][1][pos, nkv - 1, col] = value
+            cache.v[0][table[b, pos // page].long(), nkv - 1, pos % page, col] = value
+    batch = PagedBatch(cache, q_lens, kv_lens, table, num_heads=nh, window=window)
+    ref, mag = attention_seen(q, dense, q_lens, kv_lens, nkv, 1 / math.sqrt(hd), window)
+    finite = ref.isfinite()
+    assert finite.any() and not finite.all()
+    for dt in (torch.float32, torch.bfloat16):
+        out = paged_attention(cache, 0, batch, q, out_dtype=dt)
+        batch.check()
+        assert torch.equal(out.isfinite(), finite)
+        assert torch.equal(out[~finite].nan_to_num(7.0, 8.0, 9.0).double(), ref[~finite].nan_to_num(7.0, 8.0, 9.0))
+        check_attention(torch.where(finite, out, 0), torch.where(finite, ref, 0), torch.where(finite, mag, 0))
