@@ -285,9 +285,10 @@ def rope_table(max_positions: int, rot_dim: int, *, theta: float = 10000.0, scal
     elif kind == "yarn":
         n = float(scaling["original"])
         lo, hi = float(scaling.get("beta_slow", 1.0)), float(scaling.get("beta_fast", 32.0))
-        # linear in the pair's number between the numbers at which it turns hi and lo times
+        # linear in the pair's number between the numbers at which it turns hi and lo times, which may
+        # lie before the first pair or beyond the last
         at = lambda t: rot_dim * math.log(n / (2 * math.pi * t)) / (2 * math.log(theta))
-        a, b = max(math.floor(at(hi)), 0), min(math.ceil(at(lo)), rot_dim // 2 - 1)
+        a, b = math.floor(at(hi)), math.ceil(at(lo))
         ramp = ((i / 2 - a) / max(b - a, 1e-3)).clamp(0, 1)
         inv = inv * (1 - ramp) + inv / f * ramp
         gain = 0.1 * math.log(f) + 1.0
