@@ -27,9 +27,10 @@ def shared_prefix(prompts: list[list[int]], page_size: int) -> int:
 
 
 def generate(dense, moe, prompts: list[list[int]], *, max_new_tokens: int, rope: torch.Tensor | None = None,
-             rope_theta: float = 10000.0, page_size: int = 64, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+             rope_theta: float | None = None, page_size: int = 64, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
              generator: torch.Generator | None = None) -> torch.Tensor:
     """int32 tokens [prompts][max_new_tokens] (CUDA).  dense: DenseModel, moe: its MoEBlock;
+    rope: the rotation table, by default that of rope_theta, by default the model's own;
     the settings are sampling.sample's."""
     if not prompts or any(not p for p in prompts) or max_new_tokens < 1:
         raise ValueError("at least one prompt, none of them empty, and at least one new token")
@@ -49,7 +50,8 @@ def generate(dense, moe, prompts: list[list[int]], *, max_new_tokens: int, rope:
         at += x
     table = table.to(dev)
     if rope is None:
-        rope = rope_table(max(last), dense.head_dim, theta=rope_theta, device=dev)
+        theta = dense.cfg.rope_theta if rope_theta is None else rope_theta
+        rope = rope_table(max(last), dense.head_dim, theta=theta, device=dev)
     ints = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)
     if shared:
         one = PagedBatch(cache, [shared], [shared], table[:1].contiguous(), num_heads=dense.num_heads)
