@@ -78,4 +78,5 @@ def generate(dense, moe, prompts: list[list[int]], *, max_new_tokens: int, rope:
     if batch is not None:
         batch.check()
     dense.synchronize()
+    moe.synchronize()  # (each reports its own kernels' errors)
     return out.t().contiguous()

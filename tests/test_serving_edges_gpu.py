@@ -42,3 +42,14 @@ def test_generate_rotates_by_the_models_own_base(theta):
     assert [x[:1] for x in out] == again
     dm.close()
     blk.close()
+
+
+def test_generate_reports_the_moe_blocks_errors():
+    """Activations beyond the range of the prompt's tensor-core operands raise, as in MoEBlock.synchronize."""
+    dm, blk, _ = model(52, 2, 2, True)
+    huge = torch.full((256,), 1e7).bfloat16()
+    dm.load("post_norm", huge, 0)
+    with pytest.raises(M1MoECudaError):
+        generate(dm, blk, [list(range(30))], max_new_tokens=1, page_size=16, temperature=0.0)
+    dm.close()
+    blk.close()
