@@ -17,7 +17,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .expert_ffn import _check_cuda, _stream, dtype_code
+from .expert_ffn import _check_cuda, _empty, _stream, dtype_code
 
 _TENSORS = {"embed": _lib.W_EMBED, "final_norm": _lib.W_FINAL_NORM, "lm_head": _lib.W_LM_HEAD,
             "in_norm": _lib.W_INPUT_NORM, "post_norm": _lib.W_POST_NORM, "wq": _lib.W_Q,
@@ -114,8 +114,7 @@ class DenseModel:
                   stream=None) -> torch.Tensor:
         B = qkv.shape[0]
         if out is None:
-            out = torch.empty((B, self.num_heads * self.head_dim), dtype=torch.float32,
-                              device=qkv.device)
+            out = _empty((B, self.num_heads * self.head_dim), torch.float32, qkv.device, stream)
         _check_cuda(qkv, out)
         _lib.call("m1moe_cuda_dense_attention", self._ctx, layer, qkv.data_ptr(), B, out.data_ptr(),
                   _stream(stream))
@@ -123,8 +122,8 @@ class DenseModel:
 
     def lm_head(self, x: torch.Tensor, *, logits: bool = True, stream=None):
         B = x.shape[0]
-        tok = torch.empty((B,), dtype=torch.int32, device=x.device)
-        lg = torch.empty((B, self.vocab_size), dtype=torch.float32, device=x.device) if logits else None
+        tok = _empty((B,), torch.int32, x.device, stream)
+        lg = _empty((B, self.vocab_size), torch.float32, x.device, stream) if logits else None
         _check_cuda(x)
         _lib.call("m1moe_cuda_dense_lm_head", self._ctx, x.data_ptr(), B, tok.data_ptr(),
                   lg.data_ptr() if lg is not None else 0, _stream(stream))
@@ -135,7 +134,7 @@ class DenseModel:
         sequence slot 0 at the current position: returns the greedy next token
         [1] (and fills `logits` [vocab] if given); the position advances by T."""
         T = tokens.shape[0]
-        nxt = torch.empty((1,), dtype=torch.int32, device=tokens.device)
+        nxt = _empty((1,), torch.int32, tokens.device, stream)
         _check_cuda(tokens)
         _lib.call("m1moe_cuda_prefill_step", self._ctx, moe._ctx, tokens.data_ptr(), T, nxt.data_ptr(),
                   logits.data_ptr() if logits is not None else 0, _stream(stream))
@@ -147,7 +146,7 @@ class DenseModel:
         (and fills `logits` [B][vocab] if given); the position advances by one."""
         B = tokens.shape[0]
         if next_tokens is None:
-            next_tokens = torch.empty((B,), dtype=torch.int32, device=tokens.device)
+            next_tokens = _empty((B,), torch.int32, tokens.device, stream)
         _check_cuda(tokens, next_tokens)
         _lib.call("m1moe_cuda_decode_step", self._ctx, moe._ctx, tokens.data_ptr(), B,
                   next_tokens.data_ptr(), logits.data_ptr() if logits is not None else 0,
@@ -172,7 +171,7 @@ class DenseModel:
         if rope.dim() != 3 or rope.dtype != torch.float32 or rope.shape[2] != 2:
             raise ValueError("rope: float32 [positions][rot/2][2]")
         if logits is None:
-            logits = torch.empty((batch.num_seqs, self.vocab_size), dtype=torch.float32, device=dev)
+            logits = _empty((batch.num_seqs, self.vocab_size), torch.float32, dev, stream)
         elif logits.shape != (batch.num_seqs, self.vocab_size) or logits.dtype != torch.float32:
             raise ValueError(f"logits: float32 ({batch.num_seqs}, {self.vocab_size})")
         _check_cuda(tokens, rope, logits)
@@ -199,7 +198,7 @@ def gemv(w: torch.Tensor, x: torch.Tensor, *, norm_w: torch.Tensor | None = None
     B, K = x2.shape
     rows = w.shape[0]
     if out is None:
-        out = torch.empty((B, rows), dtype=torch.float32, device=x.device)
+        out = _empty((B, rows), torch.float32, x.device, stream)
     _check_cuda(w, x2, out)
     _lib.call("m1moe_cuda_dense_gemv", w.data_ptr(), rows, K, x2.data_ptr(), dtype_code(x2.dtype),
               norm_w.data_ptr() if norm_w is not None else 0, eps,
@@ -211,7 +210,7 @@ def rmsnorm(x: torch.Tensor, w: torch.Tensor, eps: float = 1e-5, *, out=None, st
     x2 = x.unsqueeze(0) if x.dim() == 1 else x
     B, D = x2.shape
     if out is None:
-        out = torch.empty((B, D), dtype=torch.float32, device=x.device)
+        out = _empty((B, D), torch.float32, x.device, stream)
     _check_cuda(x2, w, out)
     _lib.call("m1moe_cuda_dense_rmsnorm", x2.data_ptr(), dtype_code(x2.dtype), w.data_ptr(), eps,
               out.data_ptr(), D, B, _stream(stream))

@@ -29,6 +29,15 @@ def _stream(stream=None) -> int:
     return s.cuda_stream
 
 
+def _empty(shape, dtype, device, stream) -> torch.Tensor:
+    """Memory for a call's output, of the pool of the stream that the call runs on (the current
+    stream's pool may hold a block that work queued there still uses)."""
+    if stream is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    with torch.cuda.stream(stream):
+        return torch.empty(shape, dtype=dtype, device=device)
+
+
 def _check_cuda(*ts: torch.Tensor) -> None:
     for t in ts:
         if not t.is_cuda:
@@ -47,7 +56,7 @@ def matvec4(w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor, x: torc
     if x2.shape[-1] != in_dim:
         raise ValueError(f"x has {x2.shape[-1]} columns, W has {in_dim}")
     if out is None:
-        out = torch.empty((x2.shape[0], out_dim), dtype=out_dtype, device=w.device)
+        out = _empty((x2.shape[0], out_dim), out_dtype, w.device, stream)
     _check_cuda(w, scales, biases, x2, out)
     _lib.call("m1moe_cuda_matvec4", w.data_ptr(), scales.data_ptr(), biases.data_ptr(),
               x2.data_ptr(), dtype_code(x2.dtype), out.data_ptr(), dtype_code(out.dtype), out_dim,
@@ -63,7 +72,7 @@ def matvec4_strided(w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
     w/scales/biases are tensors whose data_ptr is the first matrix's W/S/B."""
     x2 = x.unsqueeze(0) if x.dim() == 1 else x
     if out is None:
-        out = torch.empty((num_mats, x2.shape[0], out_dim), dtype=out_dtype, device=x.device)
+        out = _empty((num_mats, x2.shape[0], out_dim), out_dtype, x.device, stream)
     _check_cuda(x2, out)
     _lib.call("m1moe_cuda_matvec4_strided", w.data_ptr(), scales.data_ptr(), biases.data_ptr(),
               mat_stride_bytes, num_mats, x2.data_ptr(), dtype_code(x2.dtype), out.data_ptr(),
@@ -74,7 +83,7 @@ def matvec4_strided(w: torch.Tensor, scales: torch.Tensor, biases: torch.Tensor,
 def unpack4(w: torch.Tensor, stream=None) -> torch.Tensor:
     """uint8 q[rows][cols] from packed uint32 W[rows][cols/8]."""
     rows, cols = w.shape[0], w.shape[1] * 8
-    q = torch.empty((rows, cols), dtype=torch.uint8, device=w.device)
+    q = _empty((rows, cols), torch.uint8, w.device, stream)
     _check_cuda(w, q)
     _lib.call("m1moe_cuda_unpack4", w.data_ptr(), q.data_ptr(), rows, cols, _stream(stream))
     return q

@@ -103,9 +103,9 @@ class EPFused:
                  out: torch.Tensor | None = None, idx: torch.Tensor | None = None,
                  w: torch.Tensor | None = None, stream=None) -> torch.Tensor:
         from . import _lib
-        from .expert_ffn import _stream, dtype_code
+        from .expert_ffn import _empty, _stream, dtype_code
         if out is None:
-            out = torch.empty((self.b, own.shape[-1]), dtype=torch.float32, device=own.device)
+            out = _empty((self.b, own.shape[-1]), torch.float32, own.device, stream)
         res_ptr, res_dt = (0, 0) if residual is None else (residual.data_ptr(), dtype_code(residual.dtype))
         _lib.call("m1moe_cuda_moe_layer_ep", self.blk._ctx, layer, own.data_ptr(), dtype_code(own.dtype),
                   res_ptr, res_dt, out.data_ptr(), dtype_code(out.dtype),

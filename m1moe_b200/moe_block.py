@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .expert_ffn import _check_cuda, _stream, dtype_code
+from .expert_ffn import _check_cuda, _empty, _stream, dtype_code
 from .spec import ModelSpec
 
 
@@ -101,9 +101,9 @@ class MoEBlock:
         """Top-K experts, their weights and the softmax scores for x [B][h]."""
         x2 = x.unsqueeze(0) if x.dim() == 1 else x
         B = x2.shape[0]
-        idx = torch.empty((B, self.top_k), dtype=torch.int32, device=x.device)
-        w = torch.empty((B, self.top_k), dtype=torch.float32, device=x.device)
-        scores = torch.empty((B, self.num_experts), dtype=torch.float32, device=x.device)
+        idx = _empty((B, self.top_k), torch.int32, x.device, stream)
+        w = _empty((B, self.top_k), torch.float32, x.device, stream)
+        scores = _empty((B, self.num_experts), torch.float32, x.device, stream)
         _check_cuda(x2)
         _lib.call("m1moe_cuda_router_topk", self._ctx, layer, x2.data_ptr(), dtype_code(x2.dtype),
                   B, idx.data_ptr(), w.data_ptr(), scores.data_ptr(), _stream(stream))
@@ -116,7 +116,7 @@ class MoEBlock:
         x2 = x.unsqueeze(0) if x.dim() == 1 else x
         B = x2.shape[0]
         if out is None:
-            out = torch.empty((B, self.hidden_dim), dtype=out_dtype, device=x.device)
+            out = _empty((B, self.hidden_dim), out_dtype, x.device, stream)
         _check_cuda(x2, out)
         res_ptr, res_dt = 0, 0
         if residual is not None:
@@ -125,8 +125,8 @@ class MoEBlock:
             res_ptr, res_dt = r2.data_ptr(), dtype_code(r2.dtype)
         idx = w = None
         if return_topk:
-            idx = torch.empty((B, self.top_k), dtype=torch.int32, device=x.device)
-            w = torch.empty((B, self.top_k), dtype=torch.float32, device=x.device)
+            idx = _empty((B, self.top_k), torch.int32, x.device, stream)
+            w = _empty((B, self.top_k), torch.float32, x.device, stream)
         _lib.call("m1moe_cuda_moe_layer", self._ctx, layer, x2.data_ptr(), dtype_code(x2.dtype),
                   res_ptr, res_dt, out.data_ptr(), dtype_code(out.dtype), B,
                   idx.data_ptr() if idx is not None else 0,
@@ -142,7 +142,7 @@ class MoEBlock:
         x2 = x.unsqueeze(0) if x.dim() == 1 else x
         T = x2.shape[0]
         if out is None:
-            out = torch.empty((T, self.hidden_dim), dtype=out_dtype, device=x.device)
+            out = _empty((T, self.hidden_dim), out_dtype, x.device, stream)
         _check_cuda(x2, out)
         res_ptr, res_dt = 0, 0
         if residual is not None:
@@ -151,8 +151,8 @@ class MoEBlock:
             res_ptr, res_dt = r2.data_ptr(), dtype_code(r2.dtype)
         idx = w = None
         if return_topk:
-            idx = torch.empty((T, self.top_k), dtype=torch.int32, device=x.device)
-            w = torch.empty((T, self.top_k), dtype=torch.float32, device=x.device)
+            idx = _empty((T, self.top_k), torch.int32, x.device, stream)
+            w = _empty((T, self.top_k), torch.float32, x.device, stream)
         _lib.call("m1moe_cuda_moe_prefill", self._ctx, layer, x2.data_ptr(), dtype_code(x2.dtype),
                   res_ptr, res_dt, out.data_ptr(), dtype_code(out.dtype), T,
                   idx.data_ptr() if idx is not None else 0,

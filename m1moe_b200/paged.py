@@ -22,7 +22,7 @@ import math
 import torch
 
 from . import _lib
-from .expert_ffn import dtype_code
+from .expert_ffn import _empty, dtype_code
 
 _F32, _BF16 = torch.float32, torch.bfloat16
 _raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream() without its wrapper: 0.1 of 3 us
@@ -169,14 +169,6 @@ class PagedBatch:
             for t in (self.plan, self.cu_q, self.kv_lens, self.page_table):
                 t.record_stream(s)
         return st
-
-
-def _empty(shape, dtype, device, stream):
-    """Output memory that belongs to the stream the kernel runs on."""
-    if stream is None:
-        return torch.empty(shape, dtype=dtype, device=device)
-    with torch.cuda.stream(stream):
-        return torch.empty(shape, dtype=dtype, device=device)
 
 
 def paged_append(cache: PagedKVCache, layer: int, batch: PagedBatch, qkv: torch.Tensor, *, rope: torch.Tensor,

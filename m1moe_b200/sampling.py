@@ -8,8 +8,8 @@ from __future__ import annotations
 
 import torch
 
-from .expert_ffn import dtype_code
-from .paged import _empty, _fn, _raw_stream
+from .expert_ffn import _empty, dtype_code
+from .paged import _fn, _raw_stream
 
 _sample_call = _fn("m1moe_cuda_sample")
 _F32, _I32 = torch.float32, torch.int32

@@ -53,3 +53,51 @@ def test_generate_reports_the_moe_blocks_errors():
         generate(dm, blk, [list(range(30))], max_new_tokens=1, page_size=16, temperature=0.0)
     dm.close()
     blk.close()
+
+
+def step_parts(dm, nkv, lens, nh, stream=None):
+    cache = PagedKVCache(num_layers=dm.num_layers, num_kv_heads=nkv, num_pages=sum(-(-n // 16) for n in lens), page_size=16)
+    table = torch.full((len(lens), max(-(-n // 16) for n in lens)), -1, dtype=torch.int32)
+    at = 0
+    for b, n in enumerate(lens):
+        x = -(-n // 16)
+        table[b, :x] = torch.arange(at, at + x, dtype=torch.int32)
+        at += x
+    return cache, table.cuda()
+
+
+def test_outputs_belong_to_the_stream_that_fills_them(monkeypatch):
+    """Memory for an output comes from the pool of the stream the call runs on: the current stream's
+    pool may hold a block that queued work still uses."""
+    dm, blk, _ = model(53, 2, 2, True)
+    cache, table = step_parts(dm, 2, [3, 4], 2)
+    s = torch.cuda.Stream()
+    toks = torch.arange(7, dtype=torch.int32, device="cuda")
+    rope = rope_table(16, 128)
+    batch = PagedBatch(cache, [3, 4], [3, 4], table, num_heads=2)
+    torch.cuda.synchronize()
+    made, empty = [], torch.empty
+
+    def record(*a, **kw):
+        made.append(torch.cuda.current_stream().cuda_stream)
+        return empty(*a, **kw)
+
+    monkeypatch.setattr(torch, "empty", record)
+    lg = dm.paged_step(blk, cache, batch, toks, rope=rope, stream=s)
+    assert made and set(made) == {s.cuda_stream}
+    made.clear()
+    dm.reset()
+    dm.prefill(blk, toks, stream=s)
+    dm.step(blk, toks[:1], stream=s)
+    dm.lm_head(torch.zeros((1, 256), device="cuda"), stream=s)
+    dm.attention(0, torch.zeros((1, 6 * 128), device="cuda"), stream=s)
+    x = torch.zeros((2, 256), device="cuda")
+    blk.forward(0, x, return_topk=True, stream=s)
+    blk.prefill(0, x, return_topk=True, stream=s)
+    blk.route(0, x, stream=s)
+    assert made and set(made) == {s.cuda_stream}
+    monkeypatch.undo()
+    s.synchronize()
+    assert lg.isfinite().all()
+    dm.close()
+    blk.close()
