@@ -17,7 +17,7 @@ import numpy as np
 import torch
 
 from . import _lib
-from .expert_ffn import _check_cuda, _empty, _stream, dtype_code
+from .expert_ffn import _check_cuda, _empty, _keep, _stream, dtype_code
 
 _TENSORS = {"embed": _lib.W_EMBED, "final_norm": _lib.W_FINAL_NORM, "lm_head": _lib.W_LM_HEAD,
             "in_norm": _lib.W_INPUT_NORM, "post_norm": _lib.W_POST_NORM, "wq": _lib.W_Q,
@@ -175,6 +175,7 @@ class DenseModel:
         elif logits.shape != (batch.num_seqs, self.vocab_size) or logits.dtype != torch.float32:
             raise ValueError(f"logits: float32 ({batch.num_seqs}, {self.vocab_size})")
         _check_cuda(tokens, rope, logits)
+        _keep(stream, tokens, rope, logits, cache.k, cache.v)
         k, v = cache._ptrs(0)
         _lib.call("m1moe_cuda_paged_step", self._ctx, moe._ctx, batch._cfg, batch._plan, batch._table, k, v,
                   rope.data_ptr(), rope.shape[0], 2 * rope.shape[1], tokens.data_ptr(), logits.data_ptr(),

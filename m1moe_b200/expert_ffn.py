@@ -38,6 +38,15 @@ def _empty(shape, dtype, device, stream) -> torch.Tensor:
         return torch.empty(shape, dtype=dtype, device=device)
 
 
+def _keep(stream, *tensors) -> None:
+    """What a call on `stream` uses stays allocated until the stream has run it, also where the caller
+    drops it before (None: the current stream, in whose order memory is given out anyway)."""
+    if stream is not None:
+        for t in tensors:
+            if isinstance(t, torch.Tensor):
+                t.record_stream(stream)
+
+
 def _check_cuda(*ts: torch.Tensor) -> None:
     for t in ts:
         if not t.is_cuda:

@@ -22,7 +22,7 @@ import math
 import torch
 
 from . import _lib
-from .expert_ffn import _empty, dtype_code
+from .expert_ffn import _empty, _keep, dtype_code
 
 _F32, _BF16 = torch.float32, torch.bfloat16
 _raw_stream = torch._C._cuda_getCurrentRawStream  # torch.cuda.current_stream() without its wrapper: 0.1 of 3 us
@@ -139,6 +139,7 @@ class PagedBatch:
             self.plan = torch.empty(nbytes, dtype=torch.uint8, device=dev)
             self.plan[:64].zero_()
         self._home = _raw_stream(dev.index) if stream is None else stream.cuda_stream
+        _keep(stream if stream is not None else torch.cuda.current_stream(dev), kv_lens, page_table)
         self._plan, self._table = self.plan.data_ptr(), page_table.data_ptr()
         self._q_shape = (cu[-1], num_heads, cache.head_dim)
         self._qkv_shape = (cu[-1], (num_heads + 2 * cache.num_kv_heads) * cache.head_dim)
@@ -203,6 +204,7 @@ def paged_append(cache: PagedKVCache, layer: int, batch: PagedBatch, qkv: torch.
         raise ValueError(f"out: contiguous bfloat16 {batch._q_shape} on the cache's device")
     if batch.total_q == 0:
         return out
+    _keep(stream, qkv, rope, q_norm, k_norm, out, cache.k, cache.v)
     positions, pairs, _ = rope.shape
     _append_call(cache._index, batch._cfg, batch._plan, batch._table, qkv.data_ptr(), dtype_code(qkv.dtype),
                  qkv.stride(0), qn, kn, eps, rope.data_ptr(), positions, 2 * pairs, 1 if rope_pairs else 0, k, v,
@@ -235,6 +237,7 @@ def paged_attention(cache: PagedKVCache, layer: int, batch: PagedBatch, q: torch
         out_stride = _check_rows(out, "out", cache, batch)
     if batch.total_q == 0:
         return out
+    _keep(stream, q, out, cache.k, cache.v)
     _attention_call(cache._index, batch._cfg, batch._plan, batch._table, q.data_ptr(), stride, k, v,
                     1.0 / math.sqrt(cache.head_dim) if scale is None else scale, softcap, out.data_ptr(),
                     dtype_code(out.dtype), out_stride, st)

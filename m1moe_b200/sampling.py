@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import torch
 
-from .expert_ffn import _empty, dtype_code
+from .expert_ffn import _empty, _keep, dtype_code
 from .paged import _fn, _raw_stream
 
 _sample_call = _fn("m1moe_cuda_sample")
@@ -46,6 +46,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, t
         out = _empty((rows,), _I32, dev, stream)
     elif out.device != dev or out.dtype != _I32 or out.shape != (rows,) or not out.is_contiguous():
         raise ValueError(f"out: a contiguous int32 tensor [{rows}] on {dev}")
+    _keep(stream, logits, u, temperature, top_k, top_p, min_p, out)
     # one row's stride may be anything; the C side wants at least the row's length
     stride = logits.stride(0) if rows > 1 else max(logits.stride(0), vocab)
     _sample_call(dev.index, logits.data_ptr(), dtype_code(logits.dtype), stride, rows, vocab, pu, pt, vt, pk, vk, pp, vp,
