@@ -206,9 +206,10 @@ def paged_append(cache: PagedKVCache, layer: int, batch: PagedBatch, qkv: torch.
         return out
     _keep(stream, qkv, rope, q_norm, k_norm, out, cache.k, cache.v)
     positions, pairs, _ = rope.shape
-    _append_call(cache._index, batch._cfg, batch._plan, batch._table, qkv.data_ptr(), dtype_code(qkv.dtype),
-                 qkv.stride(0), qn, kn, eps, rope.data_ptr(), positions, 2 * pairs, 1 if rope_pairs else 0, k, v,
-                 out.data_ptr(), st)
+    # one token's stride may be anything; the C side wants at least its length
+    stride = qkv.stride(0) if batch.total_q > 1 else batch._qkv_shape[1]
+    _append_call(cache._index, batch._cfg, batch._plan, batch._table, qkv.data_ptr(), dtype_code(qkv.dtype), stride,
+                 qn, kn, eps, rope.data_ptr(), positions, 2 * pairs, 1 if rope_pairs else 0, k, v, out.data_ptr(), st)
     return out
 
 
@@ -247,6 +248,8 @@ def paged_attention(cache: PagedKVCache, layer: int, batch: PagedBatch, q: torch
 def _check_rows(t: torch.Tensor, name: str, cache: PagedKVCache, batch: PagedBatch) -> int:
     """The token stride of t [total_q][heads][head dim], heads contiguous."""
     rows, inner, last = t.stride() if t.dim() == 3 else (0, 0, 0)
+    if inner != cache.head_dim and batch.num_heads == 1:
+        inner = cache.head_dim  # (one head's stride may be anything)
     if t.shape != batch._q_shape or t.device != cache.device or last != 1 or inner != cache.head_dim:
         raise ValueError(f"{name}: {batch._q_shape} with contiguous heads on the cache's device")
     # one token's stride may be anything; the C side wants at least its length

@@ -118,3 +118,23 @@ def test_values_that_are_not_finite_reach_only_the_rows_that_see_them(nh, nkv, h
         assert torch.equal(out.isfinite(), finite)
         assert torch.equal(out[~finite].nan_to_num(7.0, 8.0, 9.0).double(), ref[~finite].nan_to_num(7.0, 8.0, 9.0))
         check_attention(torch.where(finite, out, 0), torch.where(finite, ref, 0), torch.where(finite, mag, 0))
+
+
+def test_one_token_may_have_any_row_stride():
+    """A dimension of one row has no stride: what the tensor says of it is not looked at."""
+    nh, nkv, hd, page = 4, 2, 128, 16
+    cache, table, _ = make(nkv, hd, page, [1], [20], seed=35)
+    rope = rope_table(32, hd)
+    batch = PagedBatch(cache, [1], [20], table, num_heads=nh)
+    qkv = torch.randn((1, (nh + 2 * nkv) * hd), device="cuda").bfloat16()
+    ref = paged_append(cache, 0, batch, qkv, rope=rope)
+    odd = qkv.view(-1, 1).t()
+    assert odd.stride() == (1, 1)
+    assert torch.equal(paged_append(cache, 0, batch, odd, rope=rope), ref)
+    # one head: the stride between heads is not looked at either
+    cache, table, dense = make(1, hd, page, [2], [20], seed=36)
+    batch = PagedBatch(cache, [2], [20], table, num_heads=1)
+    q = torch.randn((1, 2, hd), device="cuda").bfloat16().transpose(0, 1)
+    assert q.stride() == (hd, 2 * hd, 1)
+    out = paged_attention(cache, 0, batch, q)
+    assert torch.equal(out, paged_attention(cache, 0, batch, q.contiguous()))
