@@ -138,3 +138,31 @@ def test_one_token_may_have_any_row_stride():
     assert q.stride() == (hd, 2 * hd, 1)
     out = paged_attention(cache, 0, batch, q)
     assert torch.equal(out, paged_attention(cache, 0, batch, q.contiguous()))
+
+
+@pytest.mark.parametrize("nh,nkv,hd,page,q_lens,kv_lens,window,cap", [
+    (16, 4, 128, 16, [4, 1, 3], [30, 50, 3], 0, 0.0), (8, 4, 64, 32, [8, 2], [100, 17], 3, 20.0),
+    (16, 4, 128, 16, [60, 1, 200], [60, 300, 290], 0, 30.0), (16, 4, 128, 64, [300, 40], [700, 40], 50, 0.0)])
+def test_keys_that_are_not_finite_reach_only_the_rows_that_see_them(nh, nkv, hd, page, q_lens, kv_lens, window, cap):
+    """A NaN key makes the rows that see it NaN, throughout their head, and no others."""
+    cache, table, dense = make(nkv, hd, page, q_lens, kv_lens, seed=37)
+    q = torch.randn((sum(q_lens), nh, hd), device="cuda").bfloat16()
+    ref, mag = attention_ref(q, dense, q_lens, kv_lens, nkv, 1 / math.sqrt(hd), window, cap)
+    sees = torch.zeros((sum(q_lens), nh), dtype=torch.bool, device="cuda")
+    at, group = 0, nh // nkv
+    for b, (a, t) in enumerate(zip(q_lens, kv_lens)):
+        bad = t - a + a // 2
+        cache.k[0][table[b, bad // page].long(), 0, bad % page, 5] = math.nan
+        pos = torch.arange(t - a, t, device="cuda")
+        see = pos >= bad
+        if window:
+            see &= pos - bad < window
+        sees[at:at + a, :group] = see[:, None]
+        at += a
+    batch = PagedBatch(cache, q_lens, kv_lens, table, num_heads=nh, window=window)
+    for dt in (torch.float32, torch.bfloat16):
+        out = paged_attention(cache, 0, batch, q, softcap=cap, out_dtype=dt)
+        batch.check()
+        assert torch.equal(out.isnan(), sees[..., None].expand_as(out))
+        keep = ~sees[..., None].expand_as(out)
+        check_attention(torch.where(keep, out, 0), torch.where(keep, ref, 0), torch.where(keep, mag, 0))

@@ -101,3 +101,48 @@ def test_outputs_belong_to_the_stream_that_fills_them(monkeypatch):
     assert lg.isfinite().all()
     dm.close()
     blk.close()
+
+
+def test_top_2_routing_matches_the_contiguous_model():
+    """Two of eight experts a token.  Where two experts are nearly equal a rounding may rightly swap them, so
+    the prompts compared are those whose contiguous logits stay within the bar when the output projections
+    are perturbed by up to 2^-7 of each element, at random and four times: twice the size of the paged
+    path's own roundings (2^-8) of what enters them."""
+    dm, blk, w = model(54, 4, 2, False, top_k=2)
+    rng = np.random.default_rng(4)
+    seqs = [rng.integers(0, 1000, size=n).tolist() for n in list(range(1, 25)) + [40, 60, 33, 50]]
+    cache, table = step_parts(dm, 2, [len(s) for s in seqs], 4)
+    rope = rope_table(128, 128)
+    as_ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")
+    batch = PagedBatch(cache, [len(s) for s in seqs], [len(s) for s in seqs], table, num_heads=4)
+    lg = dm.paged_step(blk, cache, batch, as_ints([t for s in seqs for t in s]), rope=rope).clone()
+    # the same last tokens again as single-token steps of up to eight sequences, after the others
+    one = torch.zeros_like(lg)
+    for i in range(0, len(seqs), 8):
+        part = seqs[i:i + 8]
+        c, t = step_parts(dm, 2, [len(s) for s in part], 4)
+        if any(len(s) > 1 for s in part):
+            b = PagedBatch(c, [len(s) - 1 for s in part], [len(s) - 1 for s in part], t, num_heads=4)
+            dm.paged_step(blk, c, b, as_ints([x for s in part for x in s[:-1]]), rope=rope)
+        b = PagedBatch(c, [1] * len(part), [len(s) for s in part], t, num_heads=4)
+        one[i:i + 8] = dm.paged_step(blk, c, b, as_ints([s[-1] for s in part]), rope=rope)
+        b.check()
+    dm.synchronize()
+    refs = [logits_of(dm, blk, s) for s in seqs]
+    steady = [True] * len(seqs)
+    g = torch.Generator().manual_seed(6)
+    wo = [torch.from_numpy(np.asarray(x)).view(torch.bfloat16).float() for x in w["wo"]]
+    for _ in range(4):
+        for L, x in enumerate(wo):
+            noise = 1 + 2.0 ** -7 * (2 * torch.rand(x.shape, generator=g) - 1)
+            dm.load("wo", (x * noise).bfloat16().view(torch.int16), L)
+        for b, s in enumerate(seqs):
+            moved = (logits_of(dm, blk, s) - refs[b]).abs().max()
+            steady[b] = steady[b] and bool(moved <= BAR * refs[b].abs().max())
+    assert sum(steady) >= len(seqs) // 4, sum(steady)
+    for b, ok in enumerate(steady):
+        if ok:
+            for got in (lg[b], one[b]):
+                assert (got - refs[b]).abs().max() <= BAR * refs[b].abs().max(), (b, len(seqs[b]))
+    dm.close()
+    blk.close()
