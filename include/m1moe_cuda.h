@@ -586,8 +586,11 @@ M1MOE_API m1moe_status m1moe_cuda_paged_step(m1moe_dense_ctx *ctx, m1moe_cuda_ct
  * exp(...) >= min_p.  The token is the first by index whose running kept
  * weight exceeds the part u of the kept weight (u and top_p in units of
  * 2^-24).  All sums are of whole numbers: the token depends on nothing but
- * its row and settings.  Temperature 0 (or below) takes the first rank; -inf
- * and NaN logits are never chosen; a row without any other gives -1.
+ * its row and settings.  Temperature 0 takes the first rank; -inf and NaN
+ * logits are never chosen; a row without any other gives -1.  A scalar setting
+ * that is negative or NaN (or a min_p above 1) is refused; in an array such a
+ * temperature or top_p keeps the first rank alone, a min_p above 1 or NaN the
+ * tokens equal to the largest, and one below 0 all.
  * Replaces the sampling of InferenceEngine.swift:550-575. */
 M1MOE_API m1moe_status m1moe_cuda_sample(const void *d_logits, int32_t dtype, int64_t row_stride, int32_t rows,
                                int32_t vocab, const float *d_u, const float *d_temperature,

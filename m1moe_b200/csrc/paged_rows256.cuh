@@ -91,9 +91,6 @@ __device__ __forceinline__ uint32_t umma_desc_lo(uint32_t smem, uint32_t lead) {
     return ((smem >> 4) & 0x3FFFu) | ((lead >> 4) << 16);
 }
 
-// The value of lane 0, known to the compiler to be the same in every lane.
-__device__ __forceinline__ uint32_t uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
-
 // True in one lane of the warp.
 __device__ __forceinline__ bool elect_one() {
     uint32_t r;

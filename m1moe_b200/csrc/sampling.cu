@@ -37,7 +37,7 @@ m1moe_status m1moe_cuda_sample(const void *d_logits, int32_t dtype, int64_t row_
     if (!d_logits || !d_u || !d_tokens) return fail(M1MOE_ERR_INVALID_ARG, "NULL pointer");
     m1::SampleParams p{};
     p.logits = d_logits;
-    p.bf16 = dtype == M1MOE_DTYPE_BF16;
+    const bool bf16 = dtype == M1MOE_DTYPE_BF16;
     p.stride = row_stride;
     p.vocab = vocab;
     p.u = d_u;
@@ -50,7 +50,7 @@ m1moe_status m1moe_cuda_sample(const void *d_logits, int32_t dtype, int64_t row_
     p.top_p1 = top_p;
     p.min_p1 = min_p;
     p.tokens = d_tokens;
-    const size_t size = p.bf16 ? 2 : 4;
+    const size_t size = bf16 ? 2 : 4;
     auto bytes_of = [&](int c) {  // a CTA's slice, 16 bytes of skew, and the own bins of a long one
         const int slice = (vocab + c - 1) / c;
         return ((size_t)slice * size + 16 + 15) / 16 * 16 +
@@ -68,7 +68,7 @@ m1moe_status m1moe_cuda_sample(const void *d_logits, int32_t dtype, int64_t row_
     p.slice = (vocab + c - 1) / c;
     const bool in_smem = bytes_of(c) <= kDynCap;
     const size_t bytes = in_smem ? bytes_of(c) : (size_t)m1::kSampleWide * m1::kSampleThreads * 8;
-    auto kern = p.bf16 ? (in_smem ? m1::k_sample<uint16_t, true> : m1::k_sample<uint16_t, false>)
+    auto kern = bf16 ? (in_smem ? m1::k_sample<uint16_t, true> : m1::k_sample<uint16_t, false>)
                        : (in_smem ? m1::k_sample<float, true> : m1::k_sample<float, false>);
     cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kDynCap);
     if (e != cudaSuccess) return cuda_fail(e, "k_sample shared memory");

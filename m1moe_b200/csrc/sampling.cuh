@@ -64,7 +64,6 @@ constexpr int kSampleOwn = 120;              // a thread's tokens between folds 
 
 struct SampleParams {
     const void *logits;
-    int bf16;
     long long stride;  // elements between rows
     int vocab, slice;  // slice: tokens per CTA of the cluster
     const float *u;
