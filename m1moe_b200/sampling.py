@@ -30,7 +30,7 @@ def sample(logits: torch.Tensor, u: torch.Tensor, *, temperature=1.0, top_k=0, t
     u f32 [rows] in [0, 1).  Each setting is a number or a CUDA tensor [rows] (f32; top_k int32).
     temperature 0: the largest logit; top_k <= 0, top_p >= 1 and min_p 0 leave that filter off; a
     row of -inf gives -1."""
-    if logits.dim() != 2 or not logits.is_cuda or (logits.numel() and logits.stride(1) != 1):
+    if logits.dim() != 2 or not logits.is_cuda or (logits.numel() and logits.shape[1] > 1 and logits.stride(1) != 1):
         raise ValueError("logits: a CUDA tensor [rows][vocab] of contiguous rows")
     rows, vocab = logits.shape
     dev = logits.device

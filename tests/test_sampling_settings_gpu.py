@@ -31,3 +31,10 @@ def test_settings_out_of_range(vocab, bad):
     for kw in ({"temperature": bad}, {"top_p": bad}, {"min_p": bad}):
         with pytest.raises(M1MoECudaError):
             sample(x, u, **kw)
+
+
+def test_one_token_may_have_any_stride():
+    """A vocabulary of one has no stride between tokens: what the tensor says of it is not looked at."""
+    x = torch.zeros((1, 5), device="cuda").t()
+    assert x.stride() == (1, 5)
+    assert sample(x, torch.rand(5, device="cuda")).tolist() == [0] * 5
