@@ -182,6 +182,13 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+// The same, NaN if an operand is.
+__device__ __forceinline__ float max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
 // 32 raw scores capped, in units of log2: by the polynomial, two at a time,
 // while |x| <= 1 throughout the warp, and score by score where not.  Up to a
 // cap of kFarCap the second form serves there for the small scores too: its
@@ -763,17 +770,13 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
                 for (int e = 0; e < 16; ++e) o[e] = __uint_as_float(v[e]);
             };
             const float f = a.prefix_run ? 1.f : ll == 0.f ? 0.f : 1.f / ll;
-            float odd = 0.f;  // NaN once an element of O is infinite or NaN
+            float odd[2] = {0.f, 0.f};  // the largest |element| of O; NaN if one is
 #pragma unroll 1
             for (int q = 0; q < HD / 16; ++q) {
                 float o[16];
                 read_o(q, o);
-                uint64_t t[4];
 #pragma unroll
-                for (int e = 0; e < 4; ++e) t[e] = add2(pack2(o[4 * e], o[4 * e + 1]), pack2(o[4 * e + 2], o[4 * e + 3]));
-                float ta, tb;
-                unpack2(add2(add2(t[0], t[1]), add2(t[2], t[3])), ta, tb);
-                odd = fmaf(ta + tb, 0.f, odd);
+                for (int e = 0; e < 16; e += 2) odd[e >> 3] = max3_nan(odd[e >> 3], fabsf(o[e]), fabsf(o[e + 1]));
                 if (whole) {
                     put(f, 16 * q, o);
                 } else if (live) {
@@ -786,7 +789,7 @@ __global__ void __launch_bounds__(kRows256Threads, 1) k_paged_rows256(const Page
             // A row's weight of a position that it does not see is 0, and so is its
             // product with that position's V, unless V is infinite or NaN there:
             // k_paged_join then sums such rows again.
-            if (odd != odd && live && !a.prefix_run) p.header[kPhOdd] = 1;
+            if (!(odd[0] + odd[1] < INFINITY) && live && !a.prefix_run) p.header[kPhOdd] = 1;
             if (live) {
                 if (!whole)
                     *part_ml_at(slot) = make_float2(mm, ll);
