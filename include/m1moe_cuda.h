@@ -538,10 +538,11 @@ M1MOE_API m1moe_status m1moe_cuda_paged_append(const m1moe_paged_cfg *cfg, const
  * q_stride elements apart, heads contiguous; d_out likewise (f32 or bf16).
  * A row's sums take the positions that it sees and no others, also where K or
  * V of another one is infinite or NaN.  fp32 scores, maxima, sums and
- * accumulators; the weights enter the second product as bf16.  The split over SMs depends on the lengths alone and
- * partials are merged in position order: the result is the same every time.
- * It uses the plan's partials, so calls on one plan must be ordered on one
- * stream.  Replaces encodeAttention (InferenceEngine.swift:349-399). */
+ * accumulators; the weights enter the second product as bf16 (their sum is
+ * taken before that rounding).  The split over SMs depends on the lengths
+ * alone and partials are merged in position order: the result is the same
+ * every time.  It uses the plan's partials, so calls on one plan must be
+ * ordered on one stream.  Replaces encodeAttention (InferenceEngine.swift:349-399). */
 M1MOE_API m1moe_status m1moe_cuda_paged_attention(const m1moe_paged_cfg *cfg, void *d_plan,
                                         const int32_t *d_page_table, const uint16_t *d_q, int64_t q_stride,
                                         const uint16_t *d_k_pages, const uint16_t *d_v_pages, float scale,
@@ -564,7 +565,10 @@ M1MOE_API m1moe_status m1moe_cuda_paged_status(void *d_plan, void *stream);
  * [num_layers] pools one after another, d_rope as in m1moe_cuda_paged_append
  * (the pairs i and i + rot_dim / 2).  Up to 8 tokens (and the MoE context's
  * max_batch) take the decode kernels, more the prefill ones of
- * m1moe_cuda_prefill_step.  The serving counterpart of InferenceEngine.forward
+ * m1moe_cuda_prefill_step.  Queries, attention weights and attention outputs
+ * are bf16 here (2^-9 of each), where m1moe_cuda_decode_step keeps them f32:
+ * the logits of the two may differ by about 1 % of the largest one (and by
+ * more where a rounding swaps two nearly equal experts).  The serving counterpart of InferenceEngine.forward
  * (:124-156), which runs one token of one sequence.  Buffers for total_q
  * tokens are allocated on the first call that needs them (synchronously; a call
  * that would have to while its stream is being captured is refused).  A

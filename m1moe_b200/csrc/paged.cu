@@ -112,7 +112,7 @@ m1moe_status make_shape(const m1moe_paged_cfg *c, int ctas, m1::PagedShape &s) {
     s.ctas = ctas;
     // 16-row items while a sequence's rows fit one, 256-row ones beyond (64
     // decode sequences: 113 us with 16 rows; a 8192-token prompt: 4226 us with
-    // 16 rows, 505 with 256)
+    // 16 rows, 518 with 256)
     const bool small = (long long)group * c->max_q <= m1::kPagedRowsSmall;
     s.rows = small ? m1::kPagedRowsSmall : m1::kPagedRowsLarge;
     s.unit = small ? m1::kPagedUnitSmall : m1::kPagedUnitLarge;

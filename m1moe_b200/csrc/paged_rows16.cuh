@@ -20,10 +20,12 @@
 // product (the sum takes them unrounded), an error of 2^-9 of each weight
 // beside the output's own rounding of 2^-9.
 //
-// Measured: one token over 2048 positions of 16 heads 12.0 us (four dependent
-// loads, one round of copies and two merges; 2.6 us at HBM rate);
-// 64 sequences of 37 to 16,000 positions, 32/8 heads, 113 us = 5.4 TB/s, 83 %
-// of the measured copy rate; 200 sequences of 20 to 1500, 78 us = 4.1 TB/s.
+// Measured back to back in a CUDA graph: one token over 2048 positions of 16
+// heads 12.3 us (four dependent loads, one round of copies and two merges; 2.6
+// us at HBM rate); 64 sequences of 37 to 16,000 positions, 32/8 heads, 113 us =
+// 5.4 TB/s, 83 % of the measured copy rate; 200 sequences of 20 to 1500, 79 us =
+// 4.1 TB/s; 32 sequences of 4 new tokens and up to 8,000 positions, 16/4 heads,
+// 28 us = 3.0 TB/s.
 #pragma once
 
 #include "paged.cuh"

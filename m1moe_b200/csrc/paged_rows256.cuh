@@ -32,10 +32,10 @@
 // is it rescaled.  Weights are at most 2^8 (bf16 has the same relative error
 // there), sums are fp32.
 //
-// Measured: 8192 tokens of 32/8 heads at hd 128, 505 us back to back = 1088
-// TFLOP/s over the visible pairs, 67 % of the measured GEMM rate (586 us = 938
-// in turn with other kernels); about 4,000 cycles a unit against 2,048 of
-// products.  The chain of one M-tile (scores out 170,
+// Measured: 8192 tokens of 32/8 heads at hd 128, 518 us back to back = 1061
+// TFLOP/s over the visible pairs, 65 % of the measured GEMM rate (585 us = 940
+// in turn with other kernels); 4096 tokens 161 us; about 4,000 cycles a unit
+// against 2,048 of products.  The chain of one M-tile (scores out 170,
 // maximum 260, exponentials 1,400, weights in 120, the two products 1,130 and
 // their hand-offs) is what bounds it: with every column of tensor memory
 // taken, the next scores cannot be computed beside it.  Tried and slower: two

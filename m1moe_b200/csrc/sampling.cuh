@@ -27,9 +27,10 @@
 // is held as two 18-bit limbs in 32-bit words (native shared-memory
 // atomics), folded into 64-bit registers before a limb could overflow.
 //
-// Measured: one row of 50,304 f32 10 us back to back (16 to 30 us amid other
+// Measured: one row of 50,304 f32 11 us back to back (16 to 30 us amid other
 // kernels: the code is read again), 192 rows of 32,000 f32 with mixed settings
-// 73 us, 48 rows of 150,001 bf16 101 us; 4 us and 2 us at HBM rate.  What
+// 73 us, 48 rows of 150,001 bf16 114 us (107 to 124 amid others); 4 us and 2 us
+// at HBM rate.  What
 // bounds it is the passes over the slice in shared memory (the maximum, the
 // first bins, one or two refinements, the tokens from the cut on), each at 10
 // to 20 instructions a token, and a block or cluster barrier a round.  One
