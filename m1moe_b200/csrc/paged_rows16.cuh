@@ -199,8 +199,10 @@ __device__ __forceinline__ SeenRow seen_row(const PagedShape &s, const RowsParam
     x.ref = m == -INFINITY ? 0.f : m;
     return x;
 }
-// Which of columns col .. col + n - 1 (n even, at most 64) of V at position p are infinite or NaN.
-__device__ __forceinline__ unsigned long long odd_columns(const SeenRow &r, int hd, int p, int col, int n) {
+// Which of columns col .. col + n - 1 (n even, at most 64) of V at position p are
+// infinite or NaN (bits above `from`: 0x7F7F) or NaN alone (0x7F80).
+__device__ __forceinline__ unsigned long long odd_columns(const SeenRow &r, int hd, int p, int col, int n,
+                                                          uint32_t from = 0x7F7Fu) {
     const long long row = seen_at(r, p);
     if (row < 0) return 0;
     const uint32_t *v = reinterpret_cast<const uint32_t *>(r.v + row * hd + col);
@@ -208,7 +210,7 @@ __device__ __forceinline__ unsigned long long odd_columns(const SeenRow &r, int 
 #pragma unroll 4
     for (int e = 0; e < n; e += 2) {
         const uint32_t b = v[e / 2];
-        odd |= (unsigned long long)(((b & 0x7F80u) == 0x7F80u ? 1 : 0) | ((b & 0x7F800000u) == 0x7F800000u ? 2 : 0)) << e;
+        odd |= (unsigned long long)(((b & 0x7FFFu) > from ? 1 : 0) | ((b >> 16 & 0x7FFFu) > from ? 2 : 0)) << e;
     }
     return odd;
 }
@@ -229,10 +231,10 @@ __device__ __noinline__ void mend_row(const PagedShape s, const RowsParams a, co
     }
     if (!odd) return;
     SeenRow x = seen_row<HD>(s, a, it, g, row, 0, 0.f);
-    // (with such a value at its own position the result is none but these)
-    if (x.p1 >= 0) odd &= ~odd_columns(x, HD, x.p1, col, n);
+    // (a NaN at its own position makes the result NaN, whatever else came in)
+    if (x.p1 >= 0) odd &= ~odd_columns(x, HD, x.p1, col, n, 0x7F80u);
     const int p0 = it.len - it.nq + fdiv(it.row0, s.by_group), p1 = it.len - it.nq + fdiv(it.row0 + it.nrows - 1, s.by_group);
-    const int end = p1 < 0 ? 0 : min(it.len, (p1 / s.unit + 1) * s.unit);  // of the item's last unit
+    const int end = min(it.len, (max(p1, 0) / s.unit + 1) * s.unit);  // of the item's last unit (it has one at least)
     for (int p = first_seen(p0, s.window); p < x.p0; ++p) why |= odd_columns(x, HD, p, col, n);
     for (int p = max(0, x.p1 + 1); p < end; ++p) why |= odd_columns(x, HD, p, col, n);
     odd &= why;

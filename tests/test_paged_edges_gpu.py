@@ -166,3 +166,43 @@ def test_keys_that_are_not_finite_reach_only_the_rows_that_see_them(nh, nkv, hd,
         assert torch.equal(out.isnan(), sees[..., None].expand_as(out))
         keep = ~sees[..., None].expand_as(out)
         check_attention(torch.where(keep, out, 0), torch.where(keep, ref, 0), torch.where(keep, mag, 0))
+
+
+@pytest.mark.parametrize("nh,nkv,hd,q_lens,kv_lens,window", [
+    (16, 4, 128, [4], [30], 0), (8, 4, 64, [8], [100], 1), (8, 2, 128, [60], [300], 0), (4, 4, 64, [270], [270], 2)])
+def test_a_hidden_nan_does_not_change_an_infinite_result(nh, nkv, hd, q_lens, kv_lens, window):
+    """Rows whose own value is infinite beside later ones that are NaN or of the other sign, in one column."""
+    cache, table, dense = make(nkv, hd, 16, q_lens, kv_lens, seed=38)
+    t, a = kv_lens[0], q_lens[0]
+    v = dense[0][1].clone()
+    at = t - a + a // 2
+    for pos, value in ((at, math.inf), (at + 1, -math.inf if window == 1 else math.inf), (t - 1, math.nan)):
+        v[pos, 1, 7] = value
+        cache.v[0][table[0, pos // 16].long(), 1, pos % 16, 7] = value
+    q = torch.randn((a, nh, hd), device="cuda").bfloat16()
+    ref, mag = attention_seen(q, [(dense[0][0], v)], q_lens, kv_lens, nkv, 1 / math.sqrt(hd), window)
+    finite = ref.isfinite()
+    assert ref.isinf().any() and ref.isnan().any()
+    batch = PagedBatch(cache, q_lens, kv_lens, table, num_heads=nh, window=window)
+    out = paged_attention(cache, 0, batch, q, out_dtype=torch.float32)
+    batch.check()
+    assert torch.equal(out[~finite].nan_to_num(7.0, 8.0, 9.0).double(), ref[~finite].nan_to_num(7.0, 8.0, 9.0))
+    check_attention(torch.where(finite, out, 0), torch.where(finite, ref, 0), torch.where(finite, mag, 0))
+
+
+@pytest.mark.parametrize("nh,nkv,hd,q_lens,kv_lens", [(16, 4, 128, [4, 3], [2, 1]), (8, 4, 64, [331, 20], [134, 20]),
+                                                      (4, 4, 128, [600], [40])])
+def test_rows_before_position_0_stay_zero(nh, nkv, hd, q_lens, kv_lens):
+    """Tokens that a sequence is too short for see nothing, whatever the positions beside them hold."""
+    cache, table, _ = make(nkv, hd, 16, q_lens, kv_lens, seed=39)
+    for b, t in enumerate(kv_lens):
+        cache.v[0][table[b, (t - 1) // 16].long(), :, (t - 1) % 16] = math.nan
+    q = torch.randn((sum(q_lens), nh, hd), device="cuda").bfloat16()
+    batch = PagedBatch(cache, q_lens, kv_lens, table, num_heads=nh)
+    out = paged_attention(cache, 0, batch, q)
+    batch.check()
+    at = 0
+    for a, t in zip(q_lens, kv_lens):
+        rows = out[at:at + a]
+        assert not rows[:max(0, a - t)].any() and rows[:a - 1].isfinite().all() and rows[a - 1].isnan().all()
+        at += a
