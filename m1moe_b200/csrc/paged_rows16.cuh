@@ -183,10 +183,9 @@ __device__ __noinline__ Columns<N> sum_seen(const SeenRow r, int col) {
     }
     return o;
 }
-// Row `row` of an item, from position `from` on; m: its largest score.
+// Row `row` of an item.
 template <int HD>
-__device__ __forceinline__ SeenRow seen_row(const PagedShape &s, const RowsParams &a, const PagedItem &it, int g, int row,
-                                            int from, float m) {
+__device__ __forceinline__ SeenRow seen_row(const PagedShape &s, const RowsParams &a, const PagedItem &it, int g, int row) {
     const int tok = fdiv(row, s.by_group);
     SeenRow x;
     x.q = a.q + (long long)(it.q0 + tok) * a.q_stride + (long long)(g * s.group + row - tok * s.group) * HD;
@@ -194,9 +193,9 @@ __device__ __forceinline__ SeenRow seen_row(const PagedShape &s, const RowsParam
     x.pages = a.table + (size_t)it.seq * s.max_pages;
     x.nkv = s.nkv, x.g = g, x.page_shift = s.page_shift, x.num_pages = s.num_pages;
     x.p1 = it.len - it.nq + tok;
-    x.p0 = max(from, first_seen(x.p1, s.window));
+    x.p0 = first_seen(x.p1, s.window);
     x.scale_log2 = a.scale * kLog2e, x.cap = a.cap, x.cs = a.cap > 0.f ? a.scale / a.cap : 0.f;
-    x.ref = m == -INFINITY ? 0.f : m;
+    x.ref = 0.f;
     return x;
 }
 // Which of columns col .. col + n - 1 (n even, at most 64) of V at position p are
@@ -230,7 +229,7 @@ __device__ __noinline__ void mend_row(const PagedShape s, const RowsParams a, co
         odd |= (unsigned long long)(y * 0.f != 0.f) << c;
     }
     if (!odd) return;
-    SeenRow x = seen_row<HD>(s, a, it, g, row, 0, 0.f);
+    SeenRow x = seen_row<HD>(s, a, it, g, row);
     // (a NaN at its own position makes the result NaN, whatever else came in)
     if (x.p1 >= 0) odd &= ~odd_columns(x, HD, x.p1, col, n, 0x7F80u);
     const int p0 = it.len - it.nq + fdiv(it.row0, s.by_group), p1 = it.len - it.nq + fdiv(it.row0 + it.nrows - 1, s.by_group);
