@@ -825,7 +825,8 @@ __device__ __noinline__ void mend_whole_items(const PagedShape s, const PagedPla
 
 // The items that the split cut: block (c, M-tile, 32 columns) joins, in
 // position order, the partials of the item that begins in CTA c's run and
-// does not end there (a run begins at most one such item).  A thread a row.
+// does not end there (a run begins at most one such item).  A thread a row.  Then,
+// where there is need, the rows that infinities or NaN have spoilt are mended.
 template <int HD>
 __device__ __forceinline__ void join_cut_item(const PagedShape &s, const PagedPlanView &p, const Rows256Params &a, int units,
                                               int per, int odd) {
